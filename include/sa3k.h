@@ -30,6 +30,7 @@ extern "C" {
 #define SA3K_TYPE_F16 1
 #define SA3K_TYPE_Q8_0 8
 #define SA3K_TYPE_Q4_K 12
+#define SA3K_TYPE_BF16 30   /* activations of the transformer-block operators only */
 
 typedef struct sa3k_ctx sa3k_ctx;
 typedef struct sa3k_weight sa3k_weight;
@@ -341,6 +342,92 @@ int sa3k_head_prep_fwd(sa3k_ctx* ctx, const float* y, int T, int ncols, int H,
 int sa3k_head_prep_bwd(sa3k_ctx* ctx, const float* g, int64_t g_ld, const float* y, int T, int ncols,
                        int H, const sa3k_head_slice* slice, int tokens_per_sample, int rot,
                        float rope_base, float* dy, char* err, int err_len);
+
+/* ------------------------------------------------------- transformer-block operators
+ * Layer normalisation, attention over a sliding window with sink tokens, and the frozen linear with
+ * activation and residual: what a pre-norm transformer block is made of, forward and backward.
+ * Besides the conventions above:
+ *   - the calls are asynchronous on the context's stream, and allocate only when a context's scratch
+ *     has to grow; scratch that a stream capture has used stays valid for the context's life, and a
+ *     call that would have to grow it during a capture fails.  Graphs captured from one context
+ *     share its scratch: replay them one after another, as the context's own calls run;
+ *   - a size of 0 (rows, S, B, Sq, Sk) is allowed and launches nothing for what is empty;
+ *   - outputs must not overlap inputs or one another;
+ *   - the current CUDA device is left as the caller had it. */
+
+/* y = (x - mean) * rstd * gamma + beta per row of x[rows][cols], mean and rstd = 1 / sqrt(var + eps)
+ * of the row (population variance).  x and y are F32, F16 or BF16 (SA3K_TYPE_*, each its own), row
+ * strides x_ld, y_ld in elements; gamma, beta f32 [cols] (NULL: 1 and 0); mean, rstd f32 [rows]
+ * (NULL, or kept for the backward).  Arithmetic in f32.  Rows of a multiple of 8 columns with
+ * 16-byte aligned bases and row strides run fastest.  The norm of a pre-norm block without the adaLN
+ * modulation; counterpart of nn::rms_norm (src/nn.h:40-42) with mean and offset. */
+int sa3k_layernorm_fwd(sa3k_ctx* ctx, int64_t rows, int64_t cols, int x_type, const void* x, int64_t x_ld,
+                       const float* gamma, const float* beta, float eps, int y_type, void* y, int64_t y_ld,
+                       float* mean, float* rstd, char* err, int err_len);
+
+/* Backward for upstream dy (of type y_type): dx (x's type; NULL: not wanted) and the parameter
+ * gradients dgamma, dbeta f32 [cols] (each may be NULL; accumulate != 0 adds into them).  The
+ * parameter gradients are summed over the rows in a fixed order. */
+int sa3k_layernorm_bwd(sa3k_ctx* ctx, int64_t rows, int64_t cols, int x_type, const void* x, int64_t x_ld,
+                       const float* gamma, const float* mean, const float* rstd, int y_type, const void* dy,
+                       int64_t dy_ld, void* dx, int64_t dx_ld, float* dgamma, float* dbeta, int accumulate, char* err,
+                       int err_len);
+
+/* Attention over a sliding window in which the first `sinks` keys stay visible.  Query row i of a
+ * batch entry stands at position p = i, or (align_end) p = i + kv_len - q_len, and sees key j iff
+ *   j < kv_len,  j <= p + right,  and  (j < sinks  or  j >= p - left);
+ * left or right < 0: no bound on that side.  right = 0 is causal; left = right = w is the symmetric
+ * band of sa3k_attention_fwd with the memory tokens kept in view.  align_end is the form of a cache:
+ * the queries are the newest q_len tokens (one, when decoding). */
+typedef struct sa3k_sink_attn {
+  int type;                 /* SA3K_TYPE_F16 or SA3K_TYPE_BF16: q, k, v, o and their gradients */
+  int B, H, H_kv;           /* H_kv key / value heads, each shared by H / H_kv query heads; B H <= 65535 */
+  int Sq, Sk, head_dim;     /* rows of the buffers; head_dim 64 */
+  float scale;
+  int64_t left, right, sinks;
+  int align_end;
+  const int32_t* q_len;     /* device [B], the rows that each entry has (NULL: Sq and Sk; values are  */
+  const int32_t* kv_len;    /*   clamped to 0 .. Sq, Sk).  Rows behind them are not read and not written */
+} sa3k_sink_attn;
+
+/* o = softmax(scale q k^T over the visible keys) v and lse [B][H][Sq] (f32, log2 units; NULL: not
+ * wanted).  A row that sees no key gets o = 0 and lse = -inf.  Bases start on 16 bytes and strides
+ * are multiples of 8 elements.  Scores, softmax and sums are f32; the probabilities are rounded to
+ * the inputs' type for the product with v.  Keys and values inside kv_len have to be finite, whether
+ * a row sees them or not.  Counterpart of attn_sliding (src/nn.h:79-100) for a sequence with memory
+ * tokens in front (src/dit.h:154-155). */
+int sa3k_attention_sink_fwd(sa3k_ctx* ctx, const sa3k_sink_attn* p, const sa3k_tensor4* q, const sa3k_tensor4* k,
+                            const sa3k_tensor4* v, const sa3k_tensor4* o, float* lse, char* err, int err_len);
+
+/* Backward for upstream dO, from the forward's o and lse: dq, and dk, dv (both or neither NULL; a
+ * shared head's are summed over its query heads), in the inputs' type.  No atomics: results do not
+ * depend on timing. */
+int sa3k_attention_sink_bwd(sa3k_ctx* ctx, const sa3k_sink_attn* p, const sa3k_tensor4* q, const sa3k_tensor4* k,
+                            const sa3k_tensor4* v, const sa3k_tensor4* o, const sa3k_tensor4* dO, const float* lse,
+                            const sa3k_tensor4* dq, const sa3k_tensor4* dk, const sa3k_tensor4* dv, char* err,
+                            int err_len);
+
+#define SA3K_ACT_NONE 0
+#define SA3K_ACT_SILU 1
+#define SA3K_ACT_GELU 2        /* 0.5 z (1 + erf(z / sqrt 2)) */
+#define SA3K_ACT_GELU_TANH 3   /* 0.5 z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) */
+
+/* z = dit_lin(W, x) + bias as sa3k_linear_fwd computes it (with the adapter, when given) and
+ * y[S][out] = act(z) + residual.  x[S][in], residual, z, y[S][out] are F32 or F16 (`type`, all the
+ * same), contiguous; residual and z may be NULL (z: the pre-activation, kept for the backward).
+ * Products read IEEE half operands with f32 accumulation (SA3K_OPT notes above): x and W are
+ * rounded to half, activation and residual are applied to the f32 value, and y is rounded once.
+ * Replaces dit_lin followed by its activation and add (src/dit.h:244-254). */
+int sa3k_linear_act_fwd(sa3k_ctx* ctx, const sa3k_weight* w, const sa3k_adapter* ad, const float* bias, int act, int type,
+                        const void* x, int64_t S, const void* residual, void* z, void* y, char* err, int err_len);
+
+/* Backward for upstream dy, from the forward's z (not needed for SA3K_ACT_NONE without a dora
+ * adapter): dz = dy act'(z), dx[S][in] = dz W (+ the adapter's part; NULL: not wanted), dbias[out] =
+ * colsum dz (NULL: not wanted) and, with an adapter, dA, dB, dm as sa3k_linear_bwd (x is needed then).
+ * accumulate != 0 adds into dbias, dA, dB, dm; dx is overwritten.  The residual's gradient is dy. */
+int sa3k_linear_act_bwd(sa3k_ctx* ctx, const sa3k_weight* w, const sa3k_adapter* ad, const float* bias, int act, int type,
+                        const void* x, int64_t S, const void* z, const void* dy, void* dx, float* dbias, float* dA,
+                        float* dB, float* dm, int accumulate, char* err, int err_len);
 
 /* AdamW hyper-parameters, as TrainAdamWParams (src/train_optimizer.h:28-35). */
 typedef struct sa3k_adamw_params {

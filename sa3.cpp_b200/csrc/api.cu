@@ -24,25 +24,35 @@ static int fill_err(char* err, int len, const std::string& msg) {
   return 1;
 }
 
+// A buffer whose address went into a stream capture is never freed before the context: when it is
+// outgrown it is retired, since the captured graph may be replayed at any later time.
 void* scratch_get(Ctx* c, int slot, size_t bytes, std::string& err) {
   if ((int)c->scratch.size() <= slot) c->scratch.resize((size_t)slot + 1);
   Scratch& s = c->scratch[(size_t)slot];
+  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+  const bool capturing = cudaStreamIsCapturing(c->stream, &cs) == cudaSuccess && cs != cudaStreamCaptureStatusNone;
   if (s.bytes < bytes) {
     ++c->gen;   // recorded graphs may hold the old buffer
     if (s.ptr) {
-      cudaStreamSynchronize(c->stream);
-      cudaFree(s.ptr);
-      s.ptr = nullptr;
-      s.bytes = 0;
+      if (s.captured || capturing) {
+        c->retired.push_back(s.ptr);
+      } else {
+        cudaStreamSynchronize(c->stream);
+        cudaFree(s.ptr);
+      }
+      s = Scratch{};
     }
     const size_t want = (bytes + 255) & ~(size_t)255;
     if (cudaMalloc(&s.ptr, want) != cudaSuccess) {
       cudaGetLastError();
-      err = "out of device memory for scratch";
+      s.ptr = nullptr;
+      err = capturing ? "scratch cannot grow during a stream capture: make one eager call of this size first"
+                      : "out of device memory for scratch";
       return nullptr;
     }
     s.bytes = want;
   }
+  if (capturing) s.captured = true;
   return s.ptr;
 }
 
@@ -226,6 +236,7 @@ void sa3k_ctx_destroy(sa3k_ctx* ctx) {
   for (cudaEvent_t e : ctx->c.ev_pool) cudaEventDestroy(e);
   for (auto& s : ctx->c.scratch)
     if (s.ptr) cudaFree(s.ptr);
+  for (void* p : ctx->c.retired) cudaFree(p);
   if (ctx->c.d_err) cudaFree(ctx->c.d_err);
   if (ctx->c.own_stream) cudaStreamDestroy(ctx->c.stream);
   delete ctx;

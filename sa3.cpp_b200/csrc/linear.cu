@@ -103,6 +103,7 @@ int linear_backward(Ctx* c, const LinearBwd& b, std::string& err) {
   const bool dora = ad && ad->dora();
   const int64_t in = w->in, out = w->out;
   const int rank = ad ? ad->rank : 0;
+  const int64_t dz_ld = b.dz_ready && b.dz_ld ? b.dz_ld : out;
   if (!b.dz_ready) {
     if (dora && cudaMemsetAsync(b.dg, 0, sizeof(float) * out, c->stream) != cudaSuccess)
       return check_launch("memset", err);
@@ -111,11 +112,11 @@ int linear_backward(Ctx* c, const LinearBwd& b, std::string& err) {
       return 1;
   }
   if (ad && out % 32 == 0) {   // du = s dz B  [M][16], written as dut = f16(du)^T [16][ut_ld]
-    if (k_r16_proj(c, b.dz, (long)out, b.M, out, ad->bt_h, ad->s, b.dut, (long)b.ut_ld, "lora.du", err)) return 1;
+    if (k_r16_proj(c, b.dz, (long)dz_ld, b.M, out, ad->bt_h, ad->s, b.dut, (long)b.ut_ld, "lora.du", err)) return 1;
   } else if (ad) {
     GemmDesc g;   // (the GEMM engine for widths the rank-16 kernel does not take)
     g.M = (int)b.M; g.N = 16; g.K = (int)out;
-    g.a = b.dz; g.lda = out;
+    g.a = b.dz; g.lda = dz_ld;
     g.bsrc = kB_F16_KMAJOR; g.b = ad->bt_h; g.ldb = out;
     g.alpha = ad->s;
     g.out_h_t = b.dut; g.ldo_h_t = b.ut_ld;
@@ -126,7 +127,7 @@ int linear_backward(Ctx* c, const LinearBwd& b, std::string& err) {
   if (b.dx || b.dx_h) {
     GemmDesc g;   // dx = dz W + du A
     g.M = (int)b.M; g.N = (int)in; g.K = (int)out;
-    g.a = b.dz; g.lda = out;
+    g.a = b.dz; g.lda = dz_ld;
     g.bsrc = kB_WEIGHT_TN; g.w = w;
     if (ad) { g.ext_at = b.dut; g.ld_ext = b.ut_ld; g.ext_b = ad->at_x; }
     g.out = b.dx; g.ldo = in; g.accumulate = b.dx_accumulate;
@@ -140,7 +141,7 @@ int linear_backward(Ctx* c, const LinearBwd& b, std::string& err) {
   {
     GemmDesc g;   // dB = s dz^T u  [out][rank]
     g.M = (int)out; g.N = rank; g.K = (int)b.M;
-    g.a = b.dz; g.lda = out; g.a_mn = 1;
+    g.a = b.dz; g.lda = dz_ld; g.a_mn = 1;
     g.bsrc = kB_F16_KMAJOR; g.b = b.ut; g.ldb = b.ut_ld;
     g.alpha = ad->s;
     g.out = b.dB; g.ldo = rank; g.accumulate = b.grad_accumulate; g.bn = 16;

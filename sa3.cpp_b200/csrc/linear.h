@@ -73,6 +73,7 @@ struct LinearBwd {
   float* dB = nullptr;                 // [out][rank]
   float* dm = nullptr;                 // [out] (dora)
   int grad_accumulate = 0;
+  int64_t dz_ld = 0;                   // row stride of a ready dz (0: out)
   // scratch: dz [M][out] f16, dg [out], dut [16][ut_ld] f16,
   // cb [16][out] f16, c3 [256]
   __half* dz = nullptr;

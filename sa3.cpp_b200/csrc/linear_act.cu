@@ -1,0 +1,213 @@
+// linear_act.cu -- the adapted frozen linear with an activation and a residual.
+//
+//   z = g (x W^T + s (x A^T) B^T) + bias,   y = act(z) + residual
+//   backward: dz = dy act'(z);  dbias = colsum(dz);  dx and the adapter gradients as in linear.cu
+//             for the upstream gradient dz (the residual's gradient is dy itself)
+#include <cmath>
+
+#include "../../include/sa3k.h"
+#include "activation.cuh"
+#include "linear.h"
+#include "lora_kernels.h"
+#include "ops_api.h"
+#include "sa3k_common.cuh"
+
+namespace sa3k {
+namespace {
+
+// y = act(zf) + residual, z = zf rounded
+template <class T>
+__global__ void __launch_bounds__(256) act_residual_kernel(const float* zf, long n, int act, const T* residual, T* z, T* y) {
+  pdl_prologue();
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) {
+    const float v = zf[i];
+    if (z) z[i] = from_f32<T>(v);
+    y[i] = from_f32<T>(act_value(act, v) + (residual ? to_f32(residual[i]) : 0.f));
+  }
+}
+
+// dz = f16(g dy act'(z)); partial column sums of dy act'(z) and of dy act'(z) (z - bias) / g over
+// the block's rows: part[blockIdx.y][2][out].  Column per thread, kActRows rows per block.
+constexpr int kActRows = 32;
+template <class T>
+__global__ void __launch_bounds__(128) act_bwd_kernel(const T* dy, const T* z, const float* bias, const float* g, int act,
+                                                      long S, long out, __half* dz, long dz_ld, float* part) {
+  pdl_prologue();
+  const long o = (long)blockIdx.x * 128 + threadIdx.x;
+  if (o >= out) return;
+  const long t0 = (long)blockIdx.y * kActRows, t1 = min(S, t0 + kActRows);
+  const float go = g ? g[o] : 1.f, bo = bias ? bias[o] : 0.f, inv = 1.f / go;
+  float sb = 0.f, sg = 0.f;
+  for (long t = t0; t < t1; ++t) {
+    const float zv = z ? to_f32(z[t * out + o]) : 0.f;
+    const float d = to_f32(dy[t * out + o]) * act_slope(act, zv);
+    dz[t * dz_ld + o] = __float2half_rn(d * go);
+    sb += d;
+    sg = fmaf(d, (zv - bo) * inv, sg);
+  }
+  if (part) {
+    part[(long)blockIdx.y * 2 * out + o] = sb;
+    part[(long)blockIdx.y * 2 * out + out + o] = sg;
+  }
+}
+
+int64_t pad64(int64_t v) { return (v + 63) / 64 * 64; }
+size_t al(size_t b) { return (b + 255) & ~(size_t)255; }
+
+int check_args(const Ctx* c, const Weight* w, const sa3k_adapter* ad, int act, int type, const void* x, int64_t S,
+               std::string& err) {
+  if (w->device != c->device) { err = "linear_act: the weight is on another device than the context"; return 1; }
+  if (act < kActNone || act > kActGeluTanh) { err = "linear_act: unknown activation"; return 1; }
+  if (type != kTypeF32 && type != kTypeF16) { err = "linear_act: the type must be F32 or F16"; return 1; }
+  if (S < 0 || S > (1 << 30)) { err = "linear_act: S must be from 0 to 2^30"; return 1; }
+  if (S > 0 && (!x || !aligned16(x))) { err = "linear_act: x must be given and start on 16 bytes"; return 1; }
+  if (ad && (ad->rank < 1 || ad->rank > 16 || !ad->A || !ad->B)) { err = "adapter rank must be 1..16 with A and B"; return 1; }
+  if (ad && ad->magnitude && !ad->base_norm_sq) { err = "dora adapter needs base_norm_sq"; return 1; }
+  return 0;
+}
+
+// x as the f16 operand (converted into scratch when it is f32)
+int operand(Ctx* c, int type, const void* x, int64_t n, const __half*& x_h, std::string& err) {
+  if (type == kTypeF16) {
+    x_h = static_cast<const __half*>(x);
+    return 0;
+  }
+  __half* p = static_cast<__half*>(scratch_get(c, kSlotActX, (size_t)n * sizeof(__half), err));
+  if (!p || k_cvt_f16(c, static_cast<const float*>(x), n, p, err)) return 1;
+  x_h = p;
+  return 0;
+}
+
+// the adapter's derived operands and u^T, in one scratch buffer
+int prepare_adapter(Ctx* c, const Weight* w, const sa3k_adapter* ad, const __half* x_h, int64_t S, AdapterPrep& prep,
+                    __half*& ut, std::string& err) {
+  prep.rank = ad->rank; prep.in = w->in; prep.out = w->out; prep.s = ad->scale;
+  prep.A = ad->A; prep.B = ad->B; prep.m = ad->magnitude; prep.bns = ad->base_norm_sq;
+  const size_t pb = al(adapter_prep_bytes(w->in, w->out, ad->magnitude != nullptr));
+  char* mem = static_cast<char*>(scratch_get(c, kSlotActAdapter, pb + (size_t)(16 * pad64(S)) * sizeof(__half), err));
+  if (!mem) return 1;
+  adapter_bind(prep, mem);
+  ut = reinterpret_cast<__half*>(mem + pb);
+  return adapter_prepare(c, w, prep, err);
+}
+
+template <class T>
+int act_residual(Ctx* c, const float* zf, int64_t n, int act, const void* residual, void* z, void* y, std::string& err) {
+  ProfScope prof_(c, "linear_act.epilogue");
+  const unsigned grid = (unsigned)std::min<int64_t>((n + 255) / 256, (int64_t)c->sm_count * 8);
+  launch_pdl(c, act_residual_kernel<T>, dim3(grid), dim3(256), 0, zf, (long)n, act, static_cast<const T*>(residual),
+             static_cast<T*>(z), static_cast<T*>(y));
+  return check_launch("linear_act epilogue", err);
+}
+
+int linear_act_forward(Ctx* c, const Weight* w, const sa3k_adapter* ad, const float* bias, int act, int type,
+                       const void* x, int64_t S, const void* residual, void* z, void* y, std::string& err) {
+  const __half* x_h;
+  if (operand(c, type, x, S * w->in, x_h, err)) return 1;
+  AdapterPrep prep;
+  __half* ut = nullptr;
+  if (ad && prepare_adapter(c, w, ad, x_h, S, prep, ut, err)) return 1;
+  float* zf = static_cast<float*>(scratch_get(c, kSlotActZ, (size_t)(S * w->out) * sizeof(float), err));
+  if (!zf) return 1;
+  LinearFwd f;
+  f.w = w; f.ad = ad ? &prep : nullptr; f.bias = bias; f.x_h = x_h; f.M = S;
+  f.y = zf; f.ut = ut; f.ut_ld = pad64(S);
+  if (linear_forward(c, f, err)) return 1;
+  return type == kTypeF16 ? act_residual<__half>(c, zf, S * w->out, act, residual, z, y, err)
+                          : act_residual<float>(c, zf, S * w->out, act, residual, z, y, err);
+}
+
+template <class T>
+int act_bwd(Ctx* c, const void* dy, const void* z, const float* bias, const float* g, int act, int64_t S, int64_t out,
+            __half* dz, int64_t dz_ld, float* part, std::string& err) {
+  ProfScope prof_(c, "linear_act.dz");
+  launch_pdl(c, act_bwd_kernel<T>, dim3((unsigned)((out + 127) / 128), (unsigned)((S + kActRows - 1) / kActRows)),
+             dim3(128), 0, static_cast<const T*>(dy), static_cast<const T*>(z), bias, g, act, (long)S, (long)out, dz, (long)dz_ld, part);
+  return check_launch("linear_act dz", err);
+}
+
+int linear_act_backward(Ctx* c, const Weight* w, const sa3k_adapter* ad, const float* bias, int act, int type,
+                        const void* x, int64_t S, const void* z, const void* dy, void* dx, float* dbias, float* dA,
+                        float* dB, float* dm, int accumulate, std::string& err) {
+  const int64_t in = w->in, out = w->out;
+  const bool dora = ad && ad->magnitude;
+  const __half* x_h = nullptr;
+  AdapterPrep prep;
+  __half* ut = nullptr;
+  if (ad) {
+    if (operand(c, type, x, S * in, x_h, err)) return 1;
+    if (prepare_adapter(c, w, ad, x_h, S, prep, ut, err) || lora_u(c, x_h, S, in, prep, ut, pad64(S), err)) return 1;
+  }
+  const int64_t dz_ld = (out + 7) / 8 * 8;   // (TMA reads rows that start on 16 bytes)
+  // scratch: dz | dut | dg | cb | c3 | partial sums
+  const int chunks = (int)((S + kActRows - 1) / kActRows);
+  const bool sums = dbias || dora;
+  const size_t b_dz = al((size_t)(S * dz_ld) * 2), b_dut = ad ? al((size_t)(16 * pad64(S)) * 2) : 0,
+               b_dg = dora ? al((size_t)out * 4) : 0, b_cb = dora ? al((size_t)(16 * out) * 2) : 0, b_c3 = dora ? al(1024) : 0,
+               b_part = sums ? al((size_t)chunks * 2 * out * 4) : 0;
+  char* mem = static_cast<char*>(scratch_get(c, kSlotActPart, b_dz + b_dut + b_dg + b_cb + b_c3 + b_part, err));
+  if (!mem) return 1;
+  LinearBwd b;
+  b.w = w; b.ad = ad ? &prep : nullptr; b.bias = bias; b.x_h = x_h; b.M = S; b.ut = ut; b.ut_ld = pad64(S);
+  b.dz = reinterpret_cast<__half*>(mem);
+  b.dut = reinterpret_cast<__half*>(mem + b_dz);
+  b.dg = reinterpret_cast<float*>(mem + b_dz + b_dut);
+  b.cb = reinterpret_cast<__half*>(mem + b_dz + b_dut + b_dg);
+  b.c3 = reinterpret_cast<float*>(mem + b_dz + b_dut + b_dg + b_cb);
+  float* part = sums ? reinterpret_cast<float*>(mem + b_dz + b_dut + b_dg + b_cb + b_c3) : nullptr;
+  const float* g = dora ? prep.g : nullptr;
+  if (type == kTypeF16 ? act_bwd<__half>(c, dy, z, bias, g, act, S, out, b.dz, dz_ld, part, err)
+                       : act_bwd<float>(c, dy, z, bias, g, act, S, out, b.dz, dz_ld, part, err))
+    return 1;
+  if (sums && k_fold_partials(c, part, chunks, (int)out, dbias, dora ? b.dg : nullptr, accumulate, 0, err)) return 1;
+  b.dz_ready = true;
+  b.dz_ld = dz_ld;
+  if (type == kTypeF16) b.dx_h = static_cast<__half*>(dx);
+  else b.dx = static_cast<float*>(dx);
+  b.dA = dA; b.dB = dB; b.dm = dm; b.grad_accumulate = accumulate;
+  return linear_backward(c, b, err);
+}
+
+}  // namespace
+}  // namespace sa3k
+
+using namespace sa3k;
+
+extern "C" {
+
+int sa3k_linear_act_fwd(sa3k_ctx* ctx, const sa3k_weight* w, const sa3k_adapter* ad, const float* bias, int act, int type,
+                        const void* x, int64_t S, const void* residual, void* z, void* y, char* err, int err_len) {
+  return api_call(ctx, err, err_len, [&](Ctx* c, std::string& e) {
+    if (!w) { e = "linear_act: the weight is NULL"; return 1; }
+    if (check_args(c, &w->w, ad, act, type, x, S, e)) return 1;
+    if (S == 0) return 0;
+    if (!y) { e = "linear_act: y is NULL"; return 1; }
+    return linear_act_forward(c, &w->w, ad, bias, act, type, x, S, residual, z, y, e);
+  });
+}
+
+int sa3k_linear_act_bwd(sa3k_ctx* ctx, const sa3k_weight* w, const sa3k_adapter* ad, const float* bias, int act, int type,
+                        const void* x, int64_t S, const void* z, const void* dy, void* dx, float* dbias, float* dA,
+                        float* dB, float* dm, int accumulate, char* err, int err_len) {
+  return api_call(ctx, err, err_len, [&](Ctx* c, std::string& e) {
+    if (!w) { e = "linear_act: the weight is NULL"; return 1; }
+    const bool dora = ad && ad->magnitude;
+    if (check_args(c, &w->w, ad, act, type, ad ? x : (x ? x : dy), S, e)) return 1;
+    if (ad && (!dA || !dB || (dora && !dm))) { e = "linear_act: an adapter needs dA and dB, and dm for dora"; return 1; }
+    if (S > 0 && !dy) { e = "linear_act: dy is NULL"; return 1; }
+    if (S > 0 && !z && (act != kActNone || dora)) { e = "linear_act: the backward needs the forward's z"; return 1; }
+    if (S > 0 && dx && !aligned16(dx)) { e = "linear_act: dx must start on 16 bytes"; return 1; }
+    if (S == 0) {
+      if (accumulate) return 0;
+      const size_t n[4] = {(size_t)w->w.out, ad ? (size_t)(ad->rank * w->w.in) : 0, ad ? (size_t)(ad->rank * w->w.out) : 0,
+                           dora ? (size_t)w->w.out : 0};
+      float* p[4] = {dbias, dA, dB, dm};
+      for (int i = 0; i < 4; ++i)
+        if (p[i] && n[i] && cudaMemsetAsync(p[i], 0, n[i] * 4, c->stream) != cudaSuccess) return check_launch("linear_act memset", e);
+      return 0;
+    }
+    return linear_act_backward(c, &w->w, ad, bias, act, type, x, S, z, dy, dx, dbias, dA, dB, dm, accumulate, e);
+  });
+}
+
+}  // extern "C"

@@ -36,6 +36,7 @@ struct Weight {
 struct Scratch {
   void* ptr = nullptr;
   size_t bytes = 0;
+  bool captured = false;             // a stream capture has taken this address
 };
 
 // Per launch-class counters (the counterpart of the reference's SA3_TRAIN_PROFILE timers,
@@ -54,6 +55,7 @@ struct Ctx {
   bool own_stream = false;
   int* d_err = nullptr;              // device error word written by bounded waits
   std::vector<Scratch> scratch;      // indexed by the slot enums of the callers
+  std::vector<void*> retired;        // outgrown scratch that a captured graph may still address
   size_t sm_count = 148;
   bool timing = false;
   bool timing_graph = false;         // timing events live in a captured CUDA graph
@@ -136,7 +138,8 @@ inline int check_launch(const char* what, std::string& err) {
 
 // Scratch slots owned by a context (see api.cu for the linear path's slots).
 enum : int { kSlotSplitK = 63, kSlotHeadSlices = 62, kSlotRope = 61, kSlotSplitCnt = 60, kSlotChainX = 59,
-             kSlotChainU = 58 };
+             kSlotChainU = 58, kSlotLnPart = 56, kSlotSinkD = 55, kSlotActX = 54,
+             kSlotActZ = 53, kSlotActPart = 52, kSlotActAdapter = 51 };   // (57: materialize.cu)
 
 // Scratch slot `slot` of at least `bytes` (grows; contents are not preserved on growth).
 void* scratch_get(Ctx* c, int slot, size_t bytes, std::string& err);

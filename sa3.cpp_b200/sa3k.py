@@ -13,7 +13,7 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libsa3k.so")
 
-TYPE_IDS = {"f32": 0, "f16": 1, "q8_0": 8, "q4_k": 12}
+TYPE_IDS = {"f32": 0, "f16": 1, "q8_0": 8, "q4_k": 12, "bf16": 30}
 
 # every symbol include/sa3k.h declares
 ABI_SYMBOLS = (
@@ -30,12 +30,17 @@ ABI_SYMBOLS = (
     "sa3k_dit_load_checkpoint", "sa3k_adapter_gguf_write", "sa3k_gguf_get_string", "sa3k_gguf_get_u64",
     "sa3k_gguf_get_u64_array", "sa3k_gguf_get_f32", "sa3k_lora_chain_build", "sa3k_lora_chain_free",
     "sa3k_lora_chain_info", "sa3k_linear_fwd_chain", "sa3k_mat_effective_weight", "sa3k_linear_mat_fwd",
-    "sa3k_linear_mat_fwd_bwd", "sa3k_dit_adapter_layout", "sa3k_dit_set_xs_bases",
+    "sa3k_linear_mat_fwd_bwd", "sa3k_dit_adapter_layout", "sa3k_dit_set_xs_bases", "sa3k_layernorm_fwd", "sa3k_layernorm_bwd",
+    "sa3k_attention_sink_fwd", "sa3k_attention_sink_bwd", "sa3k_linear_act_fwd", "sa3k_linear_act_bwd",
 )
+ACTIVATIONS = {"none": 0, "silu": 1, "gelu": 2, "gelu_tanh": 3}
 OPT_WEIGHT_F16_CACHE, OPT_SMEM_DEQUANT, OPT_GEMM_TILE_N, OPT_GEMM_PAIR, OPT_ATTN_TC, OPT_PDL = 1, 2, 3, 4, 5, 6
 OPT_STEP_GRAPH = 7
 OPT_DEQUANT_TMEM = 8
 OPT_FUSE_HEAD_PREP = 9
+
+
+_TORCH_TYPES = {"torch.float32": "f32", "torch.float16": "f16", "torch.bfloat16": "bf16"}
 
 
 class Sa3kError(RuntimeError):
@@ -50,6 +55,31 @@ class Adapter(ctypes.Structure):
 class Tensor4(ctypes.Structure):
     _fields_ = [("data", ctypes.c_void_p), ("batch_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
                 ("row_stride", ctypes.c_int64)]
+
+
+class SinkAttnC(ctypes.Structure):
+    """sa3k_sink_attn: an attention over a sliding window with sink tokens (made by sink_attn())."""
+    _fields_ = [("type", ctypes.c_int), ("B", ctypes.c_int), ("H", ctypes.c_int), ("H_kv", ctypes.c_int),
+                ("Sq", ctypes.c_int), ("Sk", ctypes.c_int), ("head_dim", ctypes.c_int), ("scale", ctypes.c_float),
+                ("left", ctypes.c_int64), ("right", ctypes.c_int64), ("sinks", ctypes.c_int64),
+                ("align_end", ctypes.c_int), ("q_len", ctypes.c_void_p), ("kv_len", ctypes.c_void_p)]
+
+
+def sink_attn(B, H, Sq, Sk, scale, left=-1, right=0, sinks=0, heads_kv=None, dtype="f16", align_end=False, q_len=None,
+              kv_len=None, head_dim=64):
+    """The description of an attention over the window [p - left, p + right] (< 0: no bound) and the first
+    `sinks` keys; q_len, kv_len: int32 CUDA tensors [B] or None.  See sa3k_sink_attn in sa3k.h."""
+    if dtype not in ("f16", "bf16"):
+        raise Sa3kError("sink_attn: dtype must be f16 or bf16")
+    p = SinkAttnC(TYPE_IDS[dtype], B, H, H if heads_kv is None else heads_kv, Sq, Sk, head_dim, scale, left, right,
+                  sinks, 1 if align_end else 0, None, None)
+    p.keep = (q_len, kv_len)     # the tensors live as long as the description
+    for name, t in (("q_len", q_len), ("kv_len", kv_len)):
+        if t is not None:
+            if str(t.dtype) != "torch.int32" or t.numel() != B or not t.is_contiguous() or not t.is_cuda:
+                raise Sa3kError(f"sink_attn: {name} must be a contiguous int32 CUDA tensor of B values")
+            setattr(p, name, t.data_ptr())
+    return p
 
 
 class HeadSliceC(ctypes.Structure):
@@ -161,6 +191,13 @@ def lib():
         L.sa3k_attention_fwd.argtypes = [P, I, I, I, I, I, F, I, T4, T4, T4, T4, P, E, I]
         L.sa3k_attention_bwd.argtypes = [P, I, I, I, I, I, F, I, T4, T4, T4, T4, T4, P, T4, T4, T4, E, I]
         L.sa3k_attention_bwd_noalloc.argtypes = [P, I, I, I, I, I, F, I, T4, T4, T4, T4, T4, P, T4, T4, T4, E, I]
+        SA = ctypes.POINTER(SinkAttnC)
+        L.sa3k_attention_sink_fwd.argtypes = [P, SA, T4, T4, T4, T4, P, E, I]
+        L.sa3k_attention_sink_bwd.argtypes = [P, SA, T4, T4, T4, T4, T4, P, T4, T4, T4, E, I]
+        L.sa3k_layernorm_fwd.argtypes = [P, I64, I64, I, P, I64, P, P, F, I, P, I64, P, P, E, I]
+        L.sa3k_layernorm_bwd.argtypes = [P, I64, I64, I, P, I64, P, P, P, I, P, I64, P, I64, P, P, I, E, I]
+        L.sa3k_linear_act_fwd.argtypes = [P, P, P, P, I, I, P, I64, P, P, P, E, I]
+        L.sa3k_linear_act_bwd.argtypes = [P, P, P, P, I, I, P, I64, P, P, P, P, P, P, P, I, E, I]
         L.sa3k_head_prep_fwd.argtypes = [P, P, I, I, I, ctypes.POINTER(HeadSliceC), I, I, F, I, F, P, E, I]
         L.sa3k_head_prep_bwd.argtypes = [P, P, I64, P, I, I, I, ctypes.POINTER(HeadSliceC), I, I, F, P, E, I]
         L.sa3k_dp_unique_id.argtypes = [P, I, E, I]
@@ -304,6 +341,101 @@ class Context:
                                                 ctypes.byref(k), ctypes.byref(v), ctypes.byref(o), ctypes.byref(dO),
                                                 _ptr(lse), ctypes.byref(dq), ctypes.byref(dk) if dk else None,
                                                 ctypes.byref(dv) if dv else None, err, 512), err)
+
+    # ------------------------------------------------------- transformer-block operators
+    def _on_device(self, what, *tensors):
+        for t in tensors:
+            if t is not None and t.device.index != self.device:
+                raise Sa3kError(f"{what}: a tensor is on {t.device}, the context on cuda:{self.device}")
+
+    @staticmethod
+    def _type_id(what, t):
+        name = _TORCH_TYPES.get(str(t.dtype))
+        if name is None:
+            raise Sa3kError(f"{what}: unsupported type {t.dtype}")
+        return TYPE_IDS[name]
+
+    @staticmethod
+    def _f32_vector(what, n, *tensors):
+        for t in tensors:
+            if t is not None and (str(t.dtype) != "torch.float32" or t.numel() != n or not t.is_contiguous()):
+                raise Sa3kError(f"{what}: expected a contiguous float32 vector of {n} values")
+
+    @staticmethod
+    def _matrix(what, shape, *tensors):
+        for t in tensors:
+            if t is not None and (tuple(t.shape) != tuple(shape) or (t.shape[1] > 1 and t.stride(1) != 1)):
+                raise Sa3kError(f"{what}: expected a [{shape[0]}][{shape[1]}] matrix with contiguous rows")
+
+    def layernorm_fwd(self, x, y, gamma=None, beta=None, eps=1e-5, mean=None, rstd=None):
+        """y = layer norm of the rows of x [rows][cols] (f32, f16 or bf16 each); mean, rstd [rows] are kept
+        when given."""
+        rows, cols = x.shape
+        self._matrix("layernorm", (rows, cols), x, y)
+        self._f32_vector("layernorm", cols, gamma, beta)
+        self._f32_vector("layernorm", rows, mean, rstd)
+        self._on_device("layernorm", x, y, gamma, beta, mean, rstd)
+        err = ctypes.create_string_buffer(512)
+        _check(lib().sa3k_layernorm_fwd(self._h, rows, cols, self._type_id("layernorm", x), x.data_ptr(), x.stride(0),
+                                        _vp(gamma), _vp(beta), eps, self._type_id("layernorm", y), y.data_ptr(),
+                                        y.stride(0), _vp(mean), _vp(rstd), err, 512), err)
+
+    def layernorm_bwd(self, x, dy, dx, mean, rstd, gamma=None, dgamma=None, dbeta=None, accumulate=False):
+        """dx (x's type, or None), dgamma and dbeta (f32, or None) for upstream dy."""
+        rows, cols = x.shape
+        self._matrix("layernorm", (rows, cols), x, dy, dx)
+        self._f32_vector("layernorm", cols, gamma, dgamma, dbeta)
+        self._f32_vector("layernorm", rows, mean, rstd)
+        self._on_device("layernorm", x, dy, dx, mean, rstd, gamma, dgamma, dbeta)
+        if dx is not None and dx.dtype != x.dtype:
+            raise Sa3kError("layernorm: dx has x's type")
+        err = ctypes.create_string_buffer(512)
+        _check(lib().sa3k_layernorm_bwd(self._h, rows, cols, self._type_id("layernorm", x), x.data_ptr(), x.stride(0),
+                                        _vp(gamma), _vp(mean), _vp(rstd), self._type_id("layernorm", dy), dy.data_ptr(),
+                                        dy.stride(0), _vp(dx), 0 if dx is None else dx.stride(0), _vp(dgamma),
+                                        _vp(dbeta), 1 if accumulate else 0, err, 512), err)
+
+    def attention_sink_fwd(self, p, q, k, v, o, lse=None):
+        """Forward of the attention that p (sink_attn()) describes; q, k, v, o are t4() tensors."""
+        err = ctypes.create_string_buffer(512)
+        _check(lib().sa3k_attention_sink_fwd(self._h, ctypes.byref(p), ctypes.byref(q), ctypes.byref(k), ctypes.byref(v),
+                                             ctypes.byref(o), _vp(lse), err, 512), err)
+
+    def attention_sink_bwd(self, p, q, k, v, o, dO, lse, dq, dk=None, dv=None):
+        err = ctypes.create_string_buffer(512)
+        _check(lib().sa3k_attention_sink_bwd(self._h, ctypes.byref(p), ctypes.byref(q), ctypes.byref(k), ctypes.byref(v),
+                                             ctypes.byref(o), ctypes.byref(dO), _vp(lse), ctypes.byref(dq),
+                                             ctypes.byref(dk) if dk else None, ctypes.byref(dv) if dv else None, err,
+                                             512), err)
+
+    def _act_args(self, w, act, S, ins, outs, vectors):
+        if act not in ACTIVATIONS:
+            raise Sa3kError(f"linear_act: unknown activation {act!r}")
+        kind = next(t.dtype for t in ins + outs if t is not None)
+        for t, n in [(t, w.inn) for t in ins] + [(t, w.out) for t in outs]:
+            if t is not None and (tuple(t.shape) != (S, n) or not t.is_contiguous() or t.dtype != kind):
+                raise Sa3kError(f"linear_act: expected contiguous [{S}][{n}] tensors of one type")
+        self._f32_vector("linear_act", w.out, *vectors)
+        self._on_device("linear_act", *ins, *outs, *vectors)
+        return ACTIVATIONS[act], TYPE_IDS.get(_TORCH_TYPES.get(str(kind)), -1)
+
+    def linear_act_fwd(self, w, x, y, act="none", bias=None, residual=None, z=None, ad=None):
+        """y = act(dit_lin(w, x) + bias) + residual; x, y, residual, z contiguous f16 or f32 (one type)."""
+        S = x.shape[0]
+        a, t = self._act_args(w, act, S, (x,), (y, residual, z), (bias,))
+        err = ctypes.create_string_buffer(512)
+        _check(lib().sa3k_linear_act_fwd(self._h, w._h, ctypes.byref(ad) if ad else None, _vp(bias), a, t, x.data_ptr(),
+                                         S, _vp(residual), _vp(z), y.data_ptr(), err, 512), err)
+
+    def linear_act_bwd(self, w, x, z, dy, dx, act="none", bias=None, dbias=None, ad=None, dA=None, dB=None, dm=None,
+                       accumulate=False):
+        """dx, dbias and the adapter gradients for upstream dy (x may be None without an adapter)."""
+        S = dy.shape[0]
+        a, t = self._act_args(w, act, S, (x, dx), (z, dy), (bias, dbias))
+        err = ctypes.create_string_buffer(512)
+        _check(lib().sa3k_linear_act_bwd(self._h, w._h, ctypes.byref(ad) if ad else None, _vp(bias), a, t, _vp(x), S,
+                                         _vp(z), dy.data_ptr(), _vp(dx), _vp(dbias), _vp(dA), _vp(dB), _vp(dm),
+                                         1 if accumulate else 0, err, 512), err)
 
     def head_prep_fwd(self, y, T, ncols, H, slices, tps, eps, rot, base, out):
         err = ctypes.create_string_buffer(512)
