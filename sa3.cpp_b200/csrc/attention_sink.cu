@@ -9,204 +9,852 @@
 // Rows that see nothing get o = 0 and lse = -inf, and take no part in the gradients.
 #include "attention_sink.h"
 
-#include <climits>
+#include <algorithm>
 #include <cmath>
 
 #include "../../include/sa3k.h"
+#include "attn_prims.cuh"
 #include "sa3k_common.cuh"
 
 namespace sa3k {
 namespace {
 
-template <class T>
-__device__ __forceinline__ const T* row_ptr(const SinkTensor& t, int b, int h, int r) {
-  return static_cast<const T*>(t.p) + (long)b * t.sb + (long)h * t.sh + (long)r * t.ld;
-}
-template <class T>
-__device__ __forceinline__ T* row_out(const SinkTensor& t, int b, int h, int r) {
-  return static_cast<T*>(t.p) + (long)b * t.sb + (long)h * t.sh + (long)r * t.ld;
+// ---------------------------------------------------------------------------- tensor-core tiles
+// The kernels below share one shape: tiles of 64 rows x 64 values (8 KB, 128-byte swizzle) stream
+// in by TMA, S = Q K^T and its like are formed in tensor memory, threads own one TMEM lane (tile
+// row) each, and P / dS go back to tensor memory as packed 16-bit pairs to be the next product's A
+// operand.  Two CTAs of 8 softmax warps share an SM (each holds half of its tensor memory), so one
+// CTA's softmax and the start and end of its tiles run under the other's products.  The first tile
+// of a window, the last of a sequence and the tiles at its edges are masked; tiles that no row of
+// the CTA sees are never loaded, so the work follows the window and not the sequence.
+constexpr int kSoftWarps = 8, kSinkThreads = 32 * (kSoftWarps + 2);
+constexpr int kTile = 8192;                 // 64 rows x 64 values x 2 bytes
+
+struct SeqMap {       // a tensor map whose (head, row, batch) dimensions are sorted by stride
+  CUtensorMap m;
+  int h, s, b;        // coordinate (1 .. 3) of each dimension
+  int hmul, bmul;     // 0 where the tensor is broadcast over that dimension
+};
+
+__device__ __forceinline__ void load_tile(void* dst, const SeqMap& t, uint64_t* bar, int b, int h, int row) {
+  const int hc = h * t.hmul, bc = b * t.bmul;
+  auto pick = [&](int k) { return t.h == k ? hc : t.s == k ? row : bc; };
+  tma_load_4d(dst, &t.m, bar, 0, pick(1), pick(2), pick(3));
 }
 
-template <class T>
-__device__ __forceinline__ float dot64(const float* x, const T* y) {
-  float s = 0.f;
-#pragma unroll
-  for (int c = 0; c < 64; c += 8) {
-    float v[8];
-    load8(y + c, v);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) s = fmaf(x[c + e], v[e], s);
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if (BF) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
   }
-  return s;
+  return pack_f16x2(lo, hi);
 }
 
-// A warp per query row: lanes take 32 keys at a time for the scores, then two columns each of o.
-template <class T>
-__global__ void __launch_bounds__(128) sink_fwd_rows_kernel(const SinkArgs a) {
-  __shared__ float sq[4][64];
-  pdl_prologue();
-  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long row = (long)blockIdx.x * 4 + w;
-  if (row >= (long)a.B * a.H * a.Sq) return;
-  const int i = (int)(row % a.Sq), h = (int)(row / a.Sq % a.H), b = (int)(row / a.Sq / a.H);
-  const SinkSeq s = sink_seq(a, b);
-  if (i >= s.qn) return;
-  const T* q = row_ptr<T>(a.q, b, h, i);
-  sq[w][lane] = to_f32(q[lane]);
-  sq[w][lane + 32] = to_f32(q[lane + 32]);
-  __syncwarp();
-  const int p = s.pos0 + i, hk = h / a.group;
-  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-  const int hi = min(s.kn, p + a.right + 1);
-  for (int j0 = 0; j0 < hi; j0 += 32) {
-    if (j0 >= a.sinks && j0 + 31 < p - a.left) continue;
-    const int j = j0 + lane;
-    const bool see = sink_sees(a, s, p, j);
-    const float x = see ? dot64(sq[w], row_ptr<T>(a.k, b, hk, j)) * a.sl2 : -INFINITY;
-    float mx = x;
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    if (mx == -INFINITY) continue;
-    const float mn = fmaxf(m, mx), al = exp2f(m - mn), pr = see ? exp2f(x - mn) : 0.f;
-    m = mn;
-    l = l * al + warp_sum(pr);
-    o0 *= al;
-    o1 *= al;
-    for (int t = 0; t < 32; ++t) {
-      const float pt = __shfl_sync(0xffffffffu, pr, t);
-      const bool st = __shfl_sync(0xffffffffu, (int)see, t);
-      if (!st) continue;
-      const T* v = row_ptr<T>(a.v, b, hk, j0 + t);
-      o0 = fmaf(pt, to_f32(v[2 * lane]), o0);
-      o1 = fmaf(pt, to_f32(v[2 * lane + 1]), o1);
+template <bool BF>
+__device__ __forceinline__ float2 unpack2(uint32_t v) {
+  if (BF) return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v));
+  return __half22float2(*reinterpret_cast<__half2*>(&v));
+}
+
+// kind::f16 instruction descriptor: M = 128, N = 64, A K-major, both operands f16 or both bf16
+template <bool BF>
+__host__ __device__ constexpr uint32_t sink_idesc(int b_mn) {
+  return make_idesc_f16(128, 64, 0, b_mn) | (BF ? (1u << 7) | (1u << 10) : 0u);
+}
+
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
+// The 64-key tiles that rows at positions [plo, phi] see: the sink tiles [0, ns), then the window's
+// [w0, w0 + n - ns).
+struct KeyTiles {
+  int ns, w0, n;
+  __device__ __forceinline__ int tile(int j) const { return j < ns ? j : w0 + (j - ns); }
+  __device__ __forceinline__ bool has(int t) const { return t < ns || (t >= w0 && t < w0 + (n - ns)); }
+};
+__device__ __forceinline__ KeyTiles key_tiles(const SinkArgs& a, const SinkSeq& s, int plo, int phi) {
+  KeyTiles k{0, 0, 0};
+  const int hi = min(s.kn, phi + a.right + 1);
+  if (hi <= 0 || phi < plo) return k;
+  k.ns = (min(a.sinks, hi) + 63) >> 6;
+  k.w0 = max(max(0, plo - a.left) >> 6, k.ns);
+  k.n = k.ns + max(0, ((hi + 63) >> 6) - k.w0);
+  return k;
+}
+
+// Every row at positions [plo, phi] sees every key of [k0, k0 + 64).
+__device__ __forceinline__ bool tile_all_seen(const SinkArgs& a, const SinkSeq& s, int plo, int phi, int k0) {
+  return k0 + 64 <= s.kn && k0 + 63 <= plo + a.right && (k0 + 63 < a.sinks || k0 >= phi - a.left);
+}
+
+__device__ __forceinline__ uint64_t low_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1ull; }
+
+// bit c: position p sees key k0 + c
+__device__ __forceinline__ uint64_t seen_mask(const SinkArgs& a, const SinkSeq& s, int p, int k0) {
+  return low_bits(min(s.kn, p + a.right + 1) - k0) & (low_bits(a.sinks - k0) | ~low_bits(p - a.left - k0));
+}
+
+// Rows [from, 64) of a 64-row tile in shared memory become zeros (t of n threads).  What a buffer
+// holds behind a sequence's end may be NaN, and 0 x NaN would spoil a product.
+__device__ __forceinline__ void zero_rows(uint8_t* tile, int from, int t, int n) {
+  for (int i = from * 8 + t; i < 512; i += n) reinterpret_cast<uint4*>(tile)[i] = make_uint4(0u, 0u, 0u, 0u);
+}
+
+// =================================================================================== forward
+// CTA: one or two groups of 128 query rows of one (batch entry, head), a softmax warpgroup each.
+// TMEM, group g at 128 g: S [0, 64) (P overwrites [0, 32)), O [64, 128).
+// smem: Q 2 x 16 KB | ring of (K 8 KB, V 8 KB) | barriers
+// One warp issues every product, in the order P V(j - 1), S(j) per group: products of one thread
+// complete in order, so the commit of S(j) also says that O holds tile j - 1 and that S's columns,
+// where P(j - 1) lay, are free.
+constexpr int kFwdStages = 4;
+constexpr int kFwdSmem = 32768 + kFwdStages * 2 * kTile + 256 + 1024;
+
+template <bool BF>
+__global__ void __launch_bounds__(kSinkThreads, 2)
+    sink_fwd_kernel(const __grid_constant__ SeqMap mq, const __grid_constant__ SeqMap mk, const __grid_constant__ SeqMap mv,
+                    const __grid_constant__ SinkArgs a, int groups) {
+  extern __shared__ uint8_t smem_raw[];
+  pdl_trigger();
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sKV = smem + 32768;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + kFwdStages * 2 * kTile);
+  uint64_t* q_full = bars;
+  uint64_t* kv_full = q_full + 1;
+  uint64_t* kv_empty = kv_full + kFwdStages;
+  uint64_t* s_full = kv_empty + kFwdStages;   // [2] S of the group's next tile
+  uint64_t* p_full = s_full + 2;              // [2] P written
+  uint64_t* o_full = p_full + 2;              // [2] the group's last P V done
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp == kSoftWarps && lane == 0) {
+    mbar_init(q_full, 1);
+    for (int s = 0; s < kFwdStages; ++s) {
+      mbar_init(&kv_full[s], 1);
+      mbar_init(&kv_empty[s], 1);
     }
-  }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  T* o = row_out<T>(a.o, b, h, i);
-  o[2 * lane] = from_f32<T>(o0 * inv);
-  o[2 * lane + 1] = from_f32<T>(o1 * inv);
-  if (lane == 0 && a.lse) a.lse[row] = l > 0.f ? m + log2f(l) : -INFINITY;
-}
-
-// A warp per query row: D, then dq.
-template <class T>
-__global__ void __launch_bounds__(128) sink_dq_rows_kernel(const SinkArgs a) {
-  __shared__ float sq[4][64], sd[4][64];
-  pdl_prologue();
-  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long row = (long)blockIdx.x * 4 + w;
-  if (row >= (long)a.B * a.H * a.Sq) return;
-  const int i = (int)(row % a.Sq), h = (int)(row / a.Sq % a.H), b = (int)(row / a.Sq / a.H);
-  const SinkSeq s = sink_seq(a, b);
-  if (i >= s.qn) return;
-  const T* q = row_ptr<T>(a.q, b, h, i);
-  const T* d = row_ptr<T>(a.dO, b, h, i);
-  const T* ov = row_ptr<T>(a.o, b, h, i);
-  float D = 0.f;
-  for (int c = lane; c < 64; c += 32) {
-    sq[w][c] = to_f32(q[c]);
-    sd[w][c] = to_f32(d[c]);
-    D = fmaf(sd[w][c], to_f32(ov[c]), D);
-  }
-  D = warp_sum(D);
-  __syncwarp();
-  if (lane == 0) a.D[row] = D;
-  const int p = s.pos0 + i, hk = h / a.group;
-  const float lse = a.lse[row];
-  float g0 = 0.f, g1 = 0.f;
-  const int hi = lse == -INFINITY ? 0 : min(s.kn, p + a.right + 1);
-  for (int j0 = 0; j0 < hi; j0 += 32) {
-    if (j0 >= a.sinks && j0 + 31 < p - a.left) continue;
-    const int j = j0 + lane;
-    const bool see = sink_sees(a, s, p, j);
-    float ds = 0.f;
-    if (see) {
-      const float pr = exp2f(dot64(sq[w], row_ptr<T>(a.k, b, hk, j)) * a.sl2 - lse);
-      ds = pr * (dot64(sd[w], row_ptr<T>(a.v, b, hk, j)) - D);
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(&s_full[g], 1);
+      mbar_init(&p_full[g], 4);
+      mbar_init(&o_full[g], 1);
     }
-    for (int t = 0; t < 32; ++t) {
-      const float dt = __shfl_sync(0xffffffffu, ds, t);
-      if (!__shfl_sync(0xffffffffu, (int)see, t)) continue;
-      const T* k = row_ptr<T>(a.k, b, hk, j0 + t);
-      g0 = fmaf(dt, to_f32(k[2 * lane]), g0);
-      g1 = fmaf(dt, to_f32(k[2 * lane + 1]), g1);
-    }
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&mq.m);
+    tma_prefetch_desc(&mk.m);
+    tma_prefetch_desc(&mv.m);
   }
-  T* dq = row_out<T>(a.dq, b, h, i);
-  dq[2 * lane] = from_f32<T>(g0 * a.scale);
-  dq[2 * lane + 1] = from_f32<T>(g1 * a.scale);
-}
+  if (warp == kSoftWarps + 1) {
+    tmem_alloc(tmem_slot, 256);
+    tmem_relinquish();
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = *tmem_slot;
+  pdl_wait();
 
-// A warp per key row: dk and dv over every query row and query head that sees it.
-template <class T>
-__global__ void __launch_bounds__(128) sink_dkdv_rows_kernel(const SinkArgs a) {
-  __shared__ float sk[4][64], sv[4][64];
-  pdl_prologue();
-  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long row = (long)blockIdx.x * 4 + w;
-  if (row >= (long)a.B * a.Hkv * a.Sk) return;
-  const int j = (int)(row % a.Sk), hk = (int)(row / a.Sk % a.Hkv), b = (int)(row / a.Sk / a.Hkv);
+  const int bh = blockIdx.y, b = bh / a.H, h = bh % a.H;
+  const int qbase = blockIdx.x * 128 * groups;
   const SinkSeq s = sink_seq(a, b);
-  if (j >= s.kn) return;
-  const T* k = row_ptr<T>(a.k, b, hk, j);
-  const T* v = row_ptr<T>(a.v, b, hk, j);
-  for (int c = lane; c < 64; c += 32) {
-    sk[w][c] = to_f32(k[c]);
-    sv[w][c] = to_f32(v[c]);
-  }
-  __syncwarp();
-  float k0 = 0.f, k1 = 0.f, v0 = 0.f, v1 = 0.f;
-  // positions p with p + right >= j, and p - left <= j unless j is a sink
-  const int lo = max(0, j - a.right - s.pos0);
-  const int hi = j < a.sinks ? s.qn : (int)min((long)s.qn, (long)j + a.left - s.pos0 + 1);
-  for (int h = hk * a.group; h < (hk + 1) * a.group; ++h)
-    for (int i0 = lo; i0 < hi; i0 += 32) {
-      const int i = i0 + lane;
-      const long r = ((long)b * a.H + h) * a.Sq + i;
-      bool see = i < hi && sink_sees(a, s, s.pos0 + i, j);
-      float pr = 0.f, ds = 0.f;
-      if (see) {
-        const float lse = a.lse[r];
-        pr = exp2f(dot64(sk[w], row_ptr<T>(a.q, b, h, i)) * a.sl2 - lse);
-        ds = pr * (dot64(sv[w], row_ptr<T>(a.dO, b, h, i)) - a.D[r]);
+  auto group_tiles = [&](int g0, int ng) {   // of groups [g0, g0 + ng)
+    const int r0 = qbase + 128 * g0, r1 = min(s.qn, r0 + 128 * ng);
+    return key_tiles(a, s, s.pos0 + r0, s.pos0 + r1 - 1);
+  };
+  const KeyTiles kt = group_tiles(0, groups);
+  const KeyTiles k0t = group_tiles(0, 1), k1t = groups > 1 ? group_tiles(1, 1) : KeyTiles{0, 0, 0};
+  const Waiter wait{abort_flag, a.err};
+  const WaiterW<> waitw{abort_flag, a.err};
+
+  if (warp == kSoftWarps) {
+    if (lane == 0 && kt.n > 0) {
+      mbar_arrive_expect_tx(q_full, (uint32_t)(2 * kTile * groups));
+      for (int g = 0; g < 2 * groups; ++g) load_tile(sQ + kTile * g, mq, q_full, b, h, qbase + 64 * g);
+      for (int j = 0; j < kt.n; ++j) {
+        const int st = j % kFwdStages;
+        if (j >= kFwdStages && !wait(&kv_empty[st], (uint32_t)((j / kFwdStages) & 1) ^ 1u, kErrTimeoutEmpty)) break;
+        uint8_t* p = sKV + st * 2 * kTile;
+        mbar_arrive_expect_tx(&kv_full[st], 2 * kTile);
+        load_tile(p, mk, &kv_full[st], b, h / a.group, kt.tile(j) * 64);
+        load_tile(p + kTile, mv, &kv_full[st], b, h / a.group, kt.tile(j) * 64);
       }
-      for (int t = 0; t < 32; ++t) {
-        const float pt = __shfl_sync(0xffffffffu, pr, t), dt = __shfl_sync(0xffffffffu, ds, t);
-        if (!__shfl_sync(0xffffffffu, (int)see, t)) continue;
-        const T* q = row_ptr<T>(a.q, b, h, i0 + t);
-        const T* d = row_ptr<T>(a.dO, b, h, i0 + t);
-        k0 = fmaf(dt, to_f32(q[2 * lane]), k0);
-        k1 = fmaf(dt, to_f32(q[2 * lane + 1]), k1);
-        v0 = fmaf(pt, to_f32(d[2 * lane]), v0);
-        v1 = fmaf(pt, to_f32(d[2 * lane + 1]), v1);
+    }
+  } else if (warp == kSoftWarps + 1) {
+    constexpr uint32_t id_s = sink_idesc<BF>(0), id_o = sink_idesc<BF>(1);
+    int cnt[2] = {0, 0}, pend[2] = {-1, -1};   // tiles of each group so far; the ring slot whose P V is due
+    bool ok = kt.n > 0 && waitw(q_full, 0, kErrTimeoutFull);
+    auto flush = [&](int g) {                  // P V of the group's last tile
+      if (pend[g] < 0) return true;
+      if (!waitw(&p_full[g], (uint32_t)((cnt[g] - 1) & 1), kErrTimeoutReady)) return false;
+      tc_fence_after();
+      const uint64_t vd = mndesc0(smem_u32(sKV + pend[g] * 2 * kTile + kTile));
+      const uint32_t tP = tbase + 128 * g;
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+        umma_ts_w(tP + 64, tP + kk * 8, mnstep(vd, kk), id_o, (cnt[g] > 1 || kk > 0) ? 1u : 0u);
+      pend[g] = -1;
+      return true;
+    };
+    for (int j = 0; j < kt.n && ok; ++j) {
+      const int st = j % kFwdStages, t = kt.tile(j);
+      if (!waitw(&kv_full[st], (uint32_t)((j / kFwdStages) & 1), kErrTimeoutFull)) { ok = false; break; }
+      tc_fence_after();
+      const uint64_t kd = kdesc0(smem_u32(sKV + st * 2 * kTile));
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        if (!ok) break;
+        if (!(ok = flush(g))) break;
+        if (!(g ? k1t : k0t).has(t)) continue;
+        const uint64_t qd = kdesc0(smem_u32(sQ + 2 * kTile * g));
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) umma_f16_w(tbase + 128 * g, kstep(qd, kk), kstep(kd, kk), id_s, kk > 0 ? 1u : 0u);
+        umma_commit_w(&s_full[g]);
+        ++cnt[g];
+        pend[g] = st;
+      }
+      if (ok && j > 0) umma_commit_w(&kv_empty[(j - 1) % kFwdStages]);   // its P V are all issued
+    }
+    for (int g = 0; g < 2 && ok; ++g) {
+      ok = flush(g);
+      if (ok && cnt[g] > 0) umma_commit_w(&o_full[g]);
+    }
+  } else {
+    const int g = warp >> 2, quarter = warp & 3, row = 32 * quarter + lane;
+    const int r0 = qbase + 128 * g, i = r0 + row;
+    const uint32_t tS = tbase + 128 * g + ((uint32_t)(32 * quarter) << 16), tO = tS + 64;
+    const int rows = g < groups ? min(128, s.qn - r0) : 0;
+    if (rows > 0) {
+      const KeyTiles my = g ? k1t : k0t;
+      const int plo = s.pos0 + r0, phi = plo + rows - 1, p = plo + row;
+      float m_used = -INFINITY, l = 0.f;
+      bool ok = true;
+      int c = 0;
+      for (int j = 0; j < kt.n; ++j) {
+        const int t = kt.tile(j);
+        if (!my.has(t)) continue;
+        if (!waitw(&s_full[g], (uint32_t)(c & 1), kErrTimeoutAccum)) { ok = false; break; }
+        tc_fence_after();
+        uint32_t v[64];
+        tmem_ld32(tS, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
+        tmem_ld32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
+        tmem_ld_wait();
+        if (!tile_all_seen(a, s, plo, phi, t * 64)) {
+          const uint64_t mask = seen_mask(a, s, p, t * 64);
+          const uint32_t ml = (uint32_t)mask, mh = (uint32_t)(mask >> 32);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            if (!((ml >> e) & 1u)) v[e] = 0xff800000u;
+            if (!((mh >> e) & 1u)) v[32 + e] = 0xff800000u;
+          }
+        }
+        const float mx = rowmax64(v) * a.sl2;
+        // the exponent's base stays unless the row's maximum grew by more than 2^8: P then stays
+        // below 2^8 and O is rescaled rarely
+        const bool grow = mx > m_used + 8.f;
+        float alpha = 1.f;
+        if (grow) {
+          alpha = m_used == -INFINITY ? 0.f : ex2(m_used - mx);
+          m_used = mx;
+        }
+        if (__any_sync(0xffffffffu, grow && c > 0)) {
+#pragma unroll 1
+          for (int q = 0; q < 4; ++q) {
+            uint32_t o[16];
+            tmem_ld16(tO + 16 * q, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st16(tO + 16 * q, o);
+          }
+        }
+        l *= alpha;
+        const float mb = m_used == -INFINITY ? 0.f : m_used;
+        const uint64_t sc2 = f2(a.sl2, a.sl2), nb2 = f2(-mb, -mb);
+        uint64_t ls[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float x0, x1;
+            f2split(ffma2(f2(__uint_as_float(v[32 * q + 2 * e]), __uint_as_float(v[32 * q + 2 * e + 1])), sc2, nb2), x0, x1);
+            const float p0 = ex2(x0), p1 = ex2(x1);
+            ls[e & 1] = fadd2(ls[e & 1], f2(p0, p1));
+            pk[e] = pack2<BF>(p0, p1);
+          }
+          tmem_st16(tS + 16 * q, pk);
+        }
+        float l0, l1, l2, l3;
+        f2split(ls[0], l0, l1);
+        f2split(ls[1], l2, l3);
+        l += (l0 + l1) + (l2 + l3);
+        if (t * 64 + 64 > s.kn && s.kn < a.Sk) {   // values behind the sequence's end
+          const int st = j % kFwdStages;
+          if (!waitw(&kv_full[st], (uint32_t)((j / kFwdStages) & 1), kErrTimeoutFull)) { ok = false; break; }
+          zero_rows(sKV + st * 2 * kTile + kTile, max(0, s.kn - t * 64), row, 128);
+          fence_proxy_async_smem();
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[g]);
+        ++c;
+      }
+      const bool have = ok && c > 0 && waitw(&o_full[g], 0, kErrTimeoutAccum);
+      tc_fence_after();
+      const float inv = l > 0.f ? 1.f / l : l;     // (0 for an empty row; NaN stays)
+      uint32_t o[64];
+      if (have) {
+        tmem_ld32(tO, *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
+        tmem_ld32(tO + 32, *reinterpret_cast<uint32_t(*)[32]>(&o[32]));
+        tmem_ld_wait();
+      }
+      if (ok && (have || c == 0) && row < rows) {
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.o.p) + (long)b * a.o.sb + (long)h * a.o.sh + (long)i * a.o.ld);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            w[e] = l == 0.f ? 0u
+                            : pack2<BF>(__uint_as_float(o[8 * q + 2 * e]) * inv, __uint_as_float(o[8 * q + 2 * e + 1]) * inv);
+          dst[q] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        if (a.lse) a.lse[(long)bh * a.Sq + i] = l == 0.f ? -INFINITY : m_used + log2f(l);
       }
     }
-  T* dk = row_out<T>(a.dk, b, hk, j);
-  T* dv = row_out<T>(a.dv, b, hk, j);
-  dk[2 * lane] = from_f32<T>(k0 * a.scale);
-  dk[2 * lane + 1] = from_f32<T>(k1 * a.scale);
-  dv[2 * lane] = from_f32<T>(v0);
-  dv[2 * lane + 1] = from_f32<T>(v1);
+  }
+  __syncthreads();
+  if (warp == kSoftWarps + 1) {
+    tc_fence_after();
+    tmem_dealloc(tbase, 256);
+  }
 }
 
-template <class T>
+// ======================================================================================== dq
+// CTA: 128 query rows of one (batch entry, head); both warpgroups hold all of them and take 32 of
+// a tile's 64 keys each.  The threads copy S and dP to registers and give their columns back at
+// once, so the next tile's products run under this tile's exponentials; dS has columns of its own.
+// TMEM: S [0, 64), dP [64, 128), dQ [128, 192), dS in two buffers of 32 columns at 192 and 224.
+constexpr int kDqStages = 4;
+constexpr int kDqSmem = 32768 + kDqStages * 2 * kTile + 256 + 1024;
+
+template <bool BF>
+__global__ void __launch_bounds__(kSinkThreads, 2)
+    sink_dq_kernel(const __grid_constant__ SeqMap mq, const __grid_constant__ SeqMap mdo, const __grid_constant__ SeqMap mk,
+                   const __grid_constant__ SeqMap mv, const __grid_constant__ SinkArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  pdl_trigger();
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;                   // Q 16 KB | dO 16 KB
+  uint8_t* sKV = smem + 32768;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + kDqStages * 2 * kTile);
+  uint64_t* q_full = bars;
+  uint64_t* kv_full = q_full + 1;
+  uint64_t* kv_empty = kv_full + kDqStages;
+  uint64_t* s_full = kv_empty + kDqStages;
+  uint64_t* s_read = s_full + 1;
+  uint64_t* ds_full = s_read + 1;
+  uint64_t* ds_free = ds_full + 1;      // [2]
+  uint64_t* acc_full = ds_free + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp == kSoftWarps && lane == 0) {
+    mbar_init(q_full, 1);
+    for (int s = 0; s < kDqStages; ++s) {
+      mbar_init(&kv_full[s], 1);
+      mbar_init(&kv_empty[s], 1);
+    }
+    mbar_init(s_full, 1);
+    mbar_init(s_read, kSoftWarps);
+    mbar_init(ds_full, kSoftWarps);
+    mbar_init(&ds_free[0], 1);
+    mbar_init(&ds_free[1], 1);
+    mbar_init(acc_full, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&mq.m);
+    tma_prefetch_desc(&mdo.m);
+    tma_prefetch_desc(&mk.m);
+    tma_prefetch_desc(&mv.m);
+  }
+  if (warp == kSoftWarps + 1) {
+    tmem_alloc(tmem_slot, 256);
+    tmem_relinquish();
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = *tmem_slot;
+  pdl_wait();
+
+  const int bh = blockIdx.y, b = bh / a.H, h = bh % a.H, r0 = blockIdx.x * 128;
+  const SinkSeq s = sink_seq(a, b);
+  const int rows = min(128, s.qn - r0), plo = s.pos0 + r0, phi = plo + rows - 1;
+  const KeyTiles kt = rows > 0 ? key_tiles(a, s, plo, phi) : KeyTiles{0, 0, 0};
+  const Waiter wait{abort_flag, a.err};
+  const WaiterW<> waitw{abort_flag, a.err};
+
+  if (warp == kSoftWarps) {
+    if (lane == 0 && kt.n > 0) {
+      mbar_arrive_expect_tx(q_full, 4 * kTile);
+      for (int g = 0; g < 2; ++g) {
+        load_tile(sQ + kTile * g, mq, q_full, b, h, r0 + 64 * g);
+        load_tile(sQ + 2 * kTile + kTile * g, mdo, q_full, b, h, r0 + 64 * g);
+      }
+      for (int j = 0; j < kt.n; ++j) {
+        const int st = j % kDqStages;
+        if (j >= kDqStages && !wait(&kv_empty[st], (uint32_t)((j / kDqStages) & 1) ^ 1u, kErrTimeoutEmpty)) break;
+        uint8_t* p = sKV + st * 2 * kTile;
+        mbar_arrive_expect_tx(&kv_full[st], 2 * kTile);
+        load_tile(p, mk, &kv_full[st], b, h / a.group, kt.tile(j) * 64);
+        load_tile(p + kTile, mv, &kv_full[st], b, h / a.group, kt.tile(j) * 64);
+      }
+    }
+  } else if (warp == kSoftWarps + 1) {
+    constexpr uint32_t id_s = sink_idesc<BF>(0), id_g = sink_idesc<BF>(1);
+    const uint64_t qd = kdesc0(smem_u32(sQ)), dd = kdesc0(smem_u32(sQ + 2 * kTile));
+    bool ok = kt.n > 0 && waitw(q_full, 0, kErrTimeoutFull);
+    auto grad = [&](int j) {     // dQ += dS K of tile j
+      if (!waitw(ds_full, (uint32_t)(j & 1), kErrTimeoutReady)) return false;
+      tc_fence_after();
+      const uint64_t kmn = mndesc0(smem_u32(sKV + (j % kDqStages) * 2 * kTile));
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+        umma_ts_w(tbase + 128, tbase + 192 + 32 * (j & 1) + kk * 8, mnstep(kmn, kk), id_g, (j > 0 || kk > 0) ? 1u : 0u);
+      umma_commit_w(&ds_free[j & 1]);
+      umma_commit_w(&kv_empty[j % kDqStages]);
+      return true;
+    };
+    for (int j = 0; j < kt.n && ok; ++j) {
+      const int st = j % kDqStages;
+      if (!waitw(&kv_full[st], (uint32_t)((j / kDqStages) & 1), kErrTimeoutFull)) { ok = false; break; }
+      if (j > 0 && !waitw(s_read, (uint32_t)((j - 1) & 1), kErrTimeoutOther)) { ok = false; break; }
+      tc_fence_after();
+      const uint64_t kd = kdesc0(smem_u32(sKV + st * 2 * kTile)), vd = kdesc0(smem_u32(sKV + st * 2 * kTile + kTile));
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) umma_f16_w(tbase, kstep(qd, kk), kstep(kd, kk), id_s, kk > 0 ? 1u : 0u);
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) umma_f16_w(tbase + 64, kstep(dd, kk), kstep(vd, kk), id_s, kk > 0 ? 1u : 0u);
+      umma_commit_w(s_full);
+      if (j > 0) ok = grad(j - 1);
+    }
+    if (ok) ok = grad(kt.n - 1);
+    if (ok) umma_commit_w(acc_full);
+  } else if (rows > 0) {
+    const int g = warp >> 2, quarter = warp & 3, row = 32 * quarter + lane, i = r0 + row, p = plo + row;
+    const uint32_t lane_off = (uint32_t)(32 * quarter) << 16;
+    const uint32_t tS = tbase + lane_off + 32 * g, tP = tS + 64;
+    const bool mine = row < rows;
+    float lse = INFINITY, D = 0.f;
+    if (mine) {
+      lse = a.lse[(long)bh * a.Sq + i];
+      if (lse == -INFINITY) lse = INFINITY;      // a row that sees nothing: P = 0
+      const long off_o = (long)b * a.o.sb + (long)h * a.o.sh + (long)i * a.o.ld;
+      const long off_d = (long)b * a.dO.sb + (long)h * a.dO.sh + (long)i * a.dO.ld;
+      const uint4* po = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.o.p) + off_o);
+      const uint4* pd = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.dO.p) + off_d);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const uint4 x = po[q], y = pd[q];
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 u = unpack2<BF>(xs[e]), w = unpack2<BF>(ys[e]);
+          D = fmaf(u.x, w.x, D);
+          D = fmaf(u.y, w.y, D);
+        }
+      }
+      if (g == 0) a.D[(long)bh * a.Sq + i] = D;
+    }
+    const uint64_t sc2 = f2(a.sl2, a.sl2), nl2 = f2(-lse, -lse), nd2 = f2(-D, -D);
+    bool ok = true;
+    for (int j = 0; j < kt.n; ++j) {
+      const int t = kt.tile(j);
+      if (!waitw(s_full, (uint32_t)(j & 1), kErrTimeoutAccum)) { ok = false; break; }
+      tc_fence_after();
+      uint32_t sv[32], pv[32];
+      tmem_ld32(tS, sv);
+      tmem_ld32(tP, pv);
+      tmem_ld_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(s_read);
+      uint32_t mask = 0xffffffffu;
+      const bool edge = !tile_all_seen(a, s, plo, phi, t * 64);
+      if (edge) mask = (uint32_t)(seen_mask(a, s, p, t * 64) >> (32 * g));
+      uint32_t pk[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        float x0, x1, d0, d1;
+        f2split(ffma2(f2(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), sc2, nl2), x0, x1);
+        const float p0 = ex2(x0), p1 = ex2(x1);
+        f2split(fmul2(f2(p0, p1), fadd2(f2(__uint_as_float(pv[2 * e]), __uint_as_float(pv[2 * e + 1])), nd2)), d0, d1);
+        if (edge) {
+          if (!((mask >> (2 * e)) & 1u)) d0 = 0.f;
+          if (!((mask >> (2 * e + 1)) & 1u)) d1 = 0.f;
+        }
+        pk[e] = pack2<BF>(d0, d1);
+      }
+      if (j >= 2 && !waitw(&ds_free[j & 1], (uint32_t)(((j >> 1) - 1) & 1), kErrTimeoutOther)) { ok = false; break; }
+      tc_fence_after();
+      tmem_st16(tbase + lane_off + 192 + 32 * (j & 1) + 16 * g, pk);
+      if (t * 64 + 64 > s.kn && s.kn < a.Sk) {   // keys behind the sequence's end
+        const int st = j % kDqStages;
+        if (!waitw(&kv_full[st], (uint32_t)((j / kDqStages) & 1), kErrTimeoutFull)) { ok = false; break; }
+        zero_rows(sKV + st * 2 * kTile, max(0, s.kn - t * 64), (int)threadIdx.x, 32 * kSoftWarps);
+        fence_proxy_async_smem();
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ds_full);
+    }
+    const bool have = ok && kt.n > 0 && waitw(acc_full, 0, kErrTimeoutAccum);
+    tc_fence_after();
+    uint32_t o[32];
+    if (have) {
+      tmem_ld32(tbase + lane_off + 128 + 32 * g, o);
+      tmem_ld_wait();
+    }
+    if (mine && ok && (have || kt.n == 0)) {
+      uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.dq.p) + (long)b * a.dq.sb + (long)h * a.dq.sh +
+                                            (long)i * a.dq.ld + 32 * g);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          w[e] = kt.n == 0 ? 0u
+                           : pack2<BF>(__uint_as_float(o[8 * q + 2 * e]) * a.scale, __uint_as_float(o[8 * q + 2 * e + 1]) * a.scale);
+        dst[q] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  }
+  __syncthreads();
+  if (warp == kSoftWarps + 1) {
+    tc_fence_after();
+    tmem_dealloc(tbase, 256);
+  }
+}
+
+// ==================================================================================== dk, dv
+// CTA: 128 keys of one (batch entry, key / value head); the 64-row query tiles that see them, of
+// every query head of the group, stream past.  Threads own a key row; the warpgroups take 32 of a
+// tile's 64 query columns each.
+// TMEM: S^T [0, 64) and dP^T [64, 128) (P^T, dS^T of columns 32 g .. overwrite the first 16 columns
+// of their own halves), dV [128, 192), dK [192, 256).
+constexpr int kDkvStages = 4;
+constexpr int kDkvSmem = 32768 + kDkvStages * 2 * kTile + 2048 + 256 + 1024;
+
+template <bool BF>
+__global__ void __launch_bounds__(kSinkThreads, 2)
+    sink_dkdv_kernel(const __grid_constant__ SeqMap mk, const __grid_constant__ SeqMap mv, const __grid_constant__ SeqMap mq,
+                     const __grid_constant__ SeqMap mdo, const __grid_constant__ SinkArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  pdl_trigger();
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sK = smem;                   // K 16 KB | V 16 KB
+  uint8_t* sQd = smem + 32768;
+  float* s_ld = reinterpret_cast<float*>(sQd + kDkvStages * 2 * kTile);   // [2 groups][2][16 column pairs][lse 2 | D 2]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sQd + kDkvStages * 2 * kTile + 2048);
+  uint64_t* kv_full = bars;
+  uint64_t* q_full = kv_full + 1;
+  uint64_t* q_empty = q_full + kDkvStages;
+  uint64_t* s_full = q_empty + kDkvStages;
+  uint64_t* ds_full = s_full + 1;
+  uint64_t* acc_full = ds_full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp == kSoftWarps && lane == 0) {
+    mbar_init(kv_full, 1);
+    for (int s = 0; s < kDkvStages; ++s) {
+      mbar_init(&q_full[s], 1);
+      mbar_init(&q_empty[s], 1);
+    }
+    mbar_init(s_full, 1);
+    mbar_init(ds_full, kSoftWarps);
+    mbar_init(acc_full, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&mk.m);
+    tma_prefetch_desc(&mv.m);
+    tma_prefetch_desc(&mq.m);
+    tma_prefetch_desc(&mdo.m);
+  }
+  if (warp == kSoftWarps + 1) {
+    tmem_alloc(tmem_slot, 256);
+    tmem_relinquish();
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = *tmem_slot;
+  pdl_wait();
+
+  // first the tiles with sinks, which the most queries see, of every head
+  const int nbh = a.B * a.Hkv, bh = blockIdx.x % nbh, b = bh / a.Hkv, hk = bh % a.Hkv, k0 = (int)(blockIdx.x / nbh) * 128;
+  const SinkSeq s = sink_seq(a, b);
+  const int keys = min(128, s.kn - k0);
+  int qt0 = 0, nt = 0;                  // query tiles [qt0, qt0 + nt) of each head
+  if (keys > 0) {
+    const int lo = max(0, k0 - a.right - s.pos0);
+    const int hi = k0 < a.sinks ? s.qn : min(s.qn, k0 + keys + a.left - s.pos0);
+    if (lo < hi) {
+      qt0 = lo >> 6;
+      nt = ((hi + 63) >> 6) - qt0;
+    }
+  }
+  const int n = nt * a.group;
+  auto head_of = [&](int j) { return hk * a.group + j / nt; };
+  auto tile_of = [&](int j) { return qt0 + j % nt; };
+  const Waiter wait{abort_flag, a.err};
+  const WaiterW<> waitw{abort_flag, a.err};
+
+  if (warp == kSoftWarps) {
+    if (lane == 0 && n > 0) {
+      mbar_arrive_expect_tx(kv_full, 4 * kTile);
+      for (int g = 0; g < 2; ++g) {
+        load_tile(sK + kTile * g, mk, kv_full, b, hk, k0 + 64 * g);
+        load_tile(sK + 2 * kTile + kTile * g, mv, kv_full, b, hk, k0 + 64 * g);
+      }
+      for (int j = 0; j < n; ++j) {
+        const int st = j % kDkvStages;
+        if (j >= kDkvStages && !wait(&q_empty[st], (uint32_t)((j / kDkvStages) & 1) ^ 1u, kErrTimeoutEmpty)) break;
+        uint8_t* p = sQd + st * 2 * kTile;
+        mbar_arrive_expect_tx(&q_full[st], 2 * kTile);
+        load_tile(p, mq, &q_full[st], b, head_of(j), tile_of(j) * 64);
+        load_tile(p + kTile, mdo, &q_full[st], b, head_of(j), tile_of(j) * 64);
+      }
+    }
+  } else if (warp == kSoftWarps + 1) {
+    constexpr uint32_t id_s = sink_idesc<BF>(0), id_g = sink_idesc<BF>(1);
+    const uint64_t kd = kdesc0(smem_u32(sK)), vd = kdesc0(smem_u32(sK + 2 * kTile));
+    bool ok = n > 0 && waitw(kv_full, 0, kErrTimeoutFull);
+    auto grad = [&](int j) {     // dV += P^T dO, dK += dS^T Q of step j
+      if (!waitw(ds_full, (uint32_t)(j & 1), kErrTimeoutReady)) return false;
+      tc_fence_after();
+      const uint32_t qa = smem_u32(sQd + (j % kDkvStages) * 2 * kTile);
+      const uint64_t qmn = mndesc0(qa), dmn = mndesc0(qa + kTile);
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+        umma_ts_w(tbase + 128, tbase + 32 * (kk >> 1) + 8 * (kk & 1), mnstep(dmn, kk), id_g, (j > 0 || kk > 0) ? 1u : 0u);
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+        umma_ts_w(tbase + 192, tbase + 64 + 32 * (kk >> 1) + 8 * (kk & 1), mnstep(qmn, kk), id_g, (j > 0 || kk > 0) ? 1u : 0u);
+      umma_commit_w(&q_empty[j % kDkvStages]);
+      return true;
+    };
+    for (int j = 0; j < n && ok; ++j) {
+      const int st = j % kDkvStages;
+      if (!waitw(&q_full[st], (uint32_t)((j / kDkvStages) & 1), kErrTimeoutFull)) { ok = false; break; }
+      if (j > 0 && !(ok = grad(j - 1))) break;
+      tc_fence_after();
+      const uint32_t qa = smem_u32(sQd + st * 2 * kTile);
+      const uint64_t qd = kdesc0(qa), dd = kdesc0(qa + kTile);
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) umma_f16_w(tbase, kstep(kd, kk), kstep(qd, kk), id_s, kk > 0 ? 1u : 0u);
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) umma_f16_w(tbase + 64, kstep(vd, kk), kstep(dd, kk), id_s, kk > 0 ? 1u : 0u);
+      umma_commit_w(s_full);
+    }
+    if (ok) ok = grad(n - 1);
+    if (ok) umma_commit_w(acc_full);
+  } else if (keys > 0) {
+    const int g = warp >> 2, quarter = warp & 3, row = 32 * quarter + lane, kj = k0 + row;
+    const int t = (int)threadIdx.x & 127;       // within the warpgroup
+    const uint32_t lane_off = (uint32_t)(32 * quarter) << 16;
+    const uint32_t tS = tbase + lane_off + 32 * g, tP = tS + 64;
+    // thread t < 32 fetches the lse of the group's column t one step ahead, 32 <= t < 64 the D
+    auto fetch = [&](int j) -> float {
+      const int i = tile_of(j) * 64 + 32 * g + (t & 31);
+      if (i >= s.qn) return t < 32 ? INFINITY : 0.f;
+      const long r = ((long)b * a.H + head_of(j)) * a.Sq + i;
+      if (t >= 32) return a.D[r];
+      const float x = a.lse[r];
+      return x == -INFINITY ? INFINITY : x;
+    };
+    const uint64_t sc2 = f2(a.sl2, a.sl2);
+    bool ok = true;
+    float next = n > 0 && t < 64 ? fetch(0) : 0.f;
+    for (int j = 0; j < n; ++j) {
+      float* ldb = s_ld + 128 * g + 64 * (j & 1);
+      if (t < 64) {
+        ldb[4 * ((t & 31) >> 1) + (t >= 32 ? 2 : 0) + (t & 1)] = next;
+        if (j + 1 < n) next = fetch(j + 1);
+      }
+      if (g == 0) named_bar(1, 128);   // (every warp of the group passes it once per step, also after an abort)
+      else named_bar(2, 128);
+      if (ok) ok = waitw(s_full, (uint32_t)(j & 1), kErrTimeoutAccum);
+      if (!ok) continue;
+      tc_fence_after();
+      const int q0 = tile_of(j) * 64, pq = s.pos0 + q0;
+      // queries of the tile that see key kj: position from kj - right to kj + left (any, for a sink)
+      const bool edge = q0 + 64 > s.qn || k0 + 128 > s.kn || k0 + 127 > pq + a.right ||
+                        !(k0 + 127 < a.sinks || k0 >= pq + 63 - a.left);
+      uint32_t mask = 0xffffffffu;
+      if (edge) {
+        uint64_t m = low_bits(s.qn - q0) & ~low_bits(kj - a.right - pq);
+        if (kj >= a.sinks) m &= low_bits(kj + a.left - pq + 1);
+        mask = kj < s.kn ? (uint32_t)(m >> (32 * g)) : 0u;
+      }
+      const float4* ld4 = reinterpret_cast<const float4*>(ldb);
+#pragma unroll 1
+      for (int hf = 0; hf < 2; ++hf) {
+        uint32_t sv[16], pv[16], pk[8], dk[8];
+        tmem_ld16(tS + 16 * hf, sv);
+        tmem_ld16(tP + 16 * hf, pv);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float4 w4 = ld4[8 * hf + e];     // lse and D of two queries, one broadcast read
+          float x0, x1, d0, d1;
+          f2split(ffma2(f2(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), sc2, f2(-w4.x, -w4.y)), x0, x1);
+          float p0 = ex2(x0), p1 = ex2(x1);
+          f2split(fmul2(f2(p0, p1), fadd2(f2(__uint_as_float(pv[2 * e]), __uint_as_float(pv[2 * e + 1])), f2(-w4.z, -w4.w))),
+                  d0, d1);
+          if (edge) {
+            const uint32_t mm = mask >> (16 * hf);
+            if (!((mm >> (2 * e)) & 1u)) p0 = d0 = 0.f;
+            if (!((mm >> (2 * e + 1)) & 1u)) p1 = d1 = 0.f;
+          }
+          pk[e] = pack2<BF>(p0, p1);
+          dk[e] = pack2<BF>(d0, d1);
+        }
+        tmem_st8(tS + 8 * hf, pk);      // (over the columns that this thread has read)
+        tmem_st8(tP + 8 * hf, dk);
+      }
+      if (q0 + 64 > s.qn && s.qn < a.Sq) {   // query rows behind the sequence's end
+        const int st = j % kDkvStages;
+        if (waitw(&q_full[st], (uint32_t)((j / kDkvStages) & 1), kErrTimeoutFull)) {
+          zero_rows(sQd + st * 2 * kTile, s.qn - q0, (int)threadIdx.x, 32 * kSoftWarps);
+          zero_rows(sQd + st * 2 * kTile + kTile, s.qn - q0, (int)threadIdx.x, 32 * kSoftWarps);
+          fence_proxy_async_smem();
+        }
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ds_full);
+    }
+    const bool have = ok && n > 0 && waitw(acc_full, 0, kErrTimeoutAccum);
+    tc_fence_after();
+    uint32_t o[64];
+    if (have) {       // warpgroup 0 writes dV, warpgroup 1 dK
+      tmem_ld32(tbase + lane_off + 128 + 64 * g, *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
+      tmem_ld32(tbase + lane_off + 160 + 64 * g, *reinterpret_cast<uint32_t(*)[32]>(&o[32]));
+      tmem_ld_wait();
+    }
+    if (row < keys && ok && (have || n == 0)) {
+      const SinkTensor& out = g == 0 ? a.dv : a.dk;
+      const float mul = g == 0 ? 1.f : a.scale;
+      uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(out.p) + (long)b * out.sb + (long)hk * out.sh + (long)kj * out.ld);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          w[e] = n == 0 ? 0u : pack2<BF>(__uint_as_float(o[8 * q + 2 * e]) * mul, __uint_as_float(o[8 * q + 2 * e + 1]) * mul);
+        dst[q] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  }
+  __syncthreads();
+  if (warp == kSoftWarps + 1) {
+    tc_fence_after();
+    tmem_dealloc(tbase, 256);
+  }
+}
+
+// Tensor map of 64-row tiles over a strided tensor; its head, row and batch dimensions go in by
+// growing stride.
+int make_seq_map(SeqMap* t, bool bf, const SinkTensor& x, int B, int H, int S, std::string& err) {
+  PFN_encodeTiled enc = encode_tiled_fn(err);
+  if (!enc) return 1;
+  struct Dim { long stride, n; int which; } d[3] = {{x.sh, H, 0}, {x.ld, S, 1}, {x.sb, B, 2}};
+  t->hmul = t->bmul = 1;
+  if (d[0].n < 2 || x.sh == 0) { d[0].n = 1; t->hmul = 0; }
+  if (d[2].n < 2 || x.sb == 0) { d[2].n = 1; t->bmul = 0; }
+  std::stable_sort(d, d + 3, [](const Dim& p, const Dim& q) {
+    if ((p.n > 1) != (q.n > 1)) return p.n > 1;
+    return p.stride < q.stride;
+  });
+  cuuint64_t dims[4] = {64, 1, 1, 1}, strides[3];
+  cuuint32_t box[4] = {64, 1, 1, 1}, estr[4] = {1, 1, 1, 1};
+  long below = 64;
+  for (int k = 0; k < 3; ++k) {
+    const long st = d[k].n > 1 ? d[k].stride : below;    // (a dimension of one entry: any valid stride)
+    dims[k + 1] = (cuuint64_t)d[k].n;
+    strides[k] = (cuuint64_t)st * 2;
+    (d[k].which == 0 ? t->h : d[k].which == 1 ? t->s : t->b) = k + 1;
+    if (d[k].which == 1) box[k + 1] = 64;
+    below = st * d[k].n;
+  }
+  const CUresult r = enc(&t->m, bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, x.p, dims, strides,
+                         box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    err = "attention_sink: cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")";
+    return 1;
+  }
+  return 0;
+}
+
+template <bool BF>
 int forward(Ctx* c, const SinkArgs& a, std::string& err) {
-  const long rows = (long)a.B * a.H * a.Sq;
+  // (a stand-in key tensor for a forward without keys: its map is never loaded from)
+  const bool nokeys = a.Sk == 0;
+  SeqMap mq, mk, mv;
+  if (make_seq_map(&mq, BF, a.q, a.B, a.H, a.Sq, err) ||
+      make_seq_map(&mk, BF, nokeys ? a.q : a.k, a.B, nokeys ? a.H : a.Hkv, nokeys ? a.Sq : a.Sk, err) ||
+      make_seq_map(&mv, BF, nokeys ? a.q : a.v, a.B, nokeys ? a.H : a.Hkv, nokeys ? a.Sq : a.Sk, err))
+    return 1;
+  auto kern = sink_fwd_kernel<BF>;
+  if (smem_attr(reinterpret_cast<const void*>(kern), kFwdSmem, c->device, "attention_sink smem attribute", err)) return 1;
+  // 256 rows per CTA share each key tile; 128 where that would leave SMs without a CTA
+  const long ctas = (long)a.B * a.H * ((a.Sq + 255) / 256);
+  const int groups = ctas >= 2 * (long)c->sm_count && a.Sq > 128 ? 2 : 1;
   ProfScope prof_(c, "attn_sink.fwd");
-  launch_pdl(c, sink_fwd_rows_kernel<T>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, a);
+  launch_pdl(c, kern, dim3((unsigned)((a.Sq + 128 * groups - 1) / (128 * groups)), (unsigned)(a.B * a.H)), dim3(kSinkThreads),
+             (size_t)kFwdSmem, mq, mk, mv, a, groups);
   return check_launch("attention with sinks, forward", err);
 }
 
-template <class T>
+template <bool BF>
 int backward(Ctx* c, const SinkArgs& a, std::string& err) {
-  const long rows = (long)a.B * a.H * a.Sq, keys = (long)a.B * a.Hkv * a.Sk;
-  if (rows > 0) {
+  const bool noq = a.Sq == 0, nokeys = a.Sk == 0;
+  if (noq && nokeys) return 0;
+  SeqMap mq, mdo, mk, mv;
+  const SinkTensor &tq = noq ? a.k : a.q, &td = noq ? a.k : a.dO, &tk = nokeys ? a.q : a.k, &tv = nokeys ? a.q : a.v;
+  const int hq = noq ? a.Hkv : a.H, sq = noq ? a.Sk : a.Sq, hk = nokeys ? a.H : a.Hkv, sk = nokeys ? a.Sq : a.Sk;
+  if (make_seq_map(&mq, BF, tq, a.B, hq, sq, err) || make_seq_map(&mdo, BF, td, a.B, hq, sq, err) ||
+      make_seq_map(&mk, BF, tk, a.B, hk, sk, err) || make_seq_map(&mv, BF, tv, a.B, hk, sk, err))
+    return 1;
+  if (!noq) {
+    auto kern = sink_dq_kernel<BF>;
+    if (smem_attr(reinterpret_cast<const void*>(kern), kDqSmem, c->device, "attention_sink smem attribute", err)) return 1;
     ProfScope prof_(c, "attn_sink.dq");
-    launch_pdl(c, sink_dq_rows_kernel<T>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, a);
+    launch_pdl(c, kern, dim3((unsigned)((a.Sq + 127) / 128), (unsigned)(a.B * a.H)), dim3(kSinkThreads), (size_t)kDqSmem, mq,
+               mdo, mk, mv, a);
     if (check_launch("attention with sinks, dq", err)) return 1;
   }
-  if (!a.dk.p || keys == 0) return 0;
+  if (!a.dk.p || nokeys) return 0;
+  auto kern = sink_dkdv_kernel<BF>;
+  if (smem_attr(reinterpret_cast<const void*>(kern), kDkvSmem, c->device, "attention_sink smem attribute", err)) return 1;
   ProfScope prof_(c, "attn_sink.dkdv");
-  launch_pdl(c, sink_dkdv_rows_kernel<T>, dim3((unsigned)((keys + 3) / 4)), dim3(128), 0, a);
+  launch_pdl(c, kern, dim3((unsigned)((long)a.B * a.Hkv * ((a.Sk + 127) / 128))), dim3(kSinkThreads), (size_t)kDkvSmem,
+             mk, mv, mq, mdo, a);
   return check_launch("attention with sinks, dk / dv", err);
 }
 
@@ -228,21 +876,20 @@ int check_tensor(const char* what, const sa3k_tensor4* t, int B, int H, int S, b
     err = std::string("attention_sink: the strides of ") + what + " must be from 0 to 2^38";
     return 1;
   }
-  // rows of 64 values must not overlap where they are written: every stride holds a row, and the
-  // dimensions nest (sorted by stride, each holds the extent of those below it)
-  if (out) {
-    long st[3] = {d.sb, d.sh, d.ld}, n[3] = {B, H, S};
-    long below = 64;
-    bool used[3] = {false, false, false};
-    for (int k = 0; k < 3; ++k) {
-      int best = -1;
-      for (int i = 0; i < 3; ++i)
-        if (!used[i] && (best < 0 || n[i] < 2 || (n[best] > 1 && st[i] < st[best]))) best = i;
-      used[best] = true;
-      if (n[best] < 2) continue;
-      if (st[best] < below) { err = std::string("attention_sink: rows of ") + what + " overlap"; return 1; }
-      below = st[best] * (n[best] - 1) + below;
-    }
+  // the dimensions have to nest: by growing stride, each holds the extent of those below it (an input
+  // may be broadcast over heads or batch with stride 0)
+  long st[3] = {d.sh, d.ld, d.sb}, n[3] = {H, S, B};
+  long below = 64;
+  bool used[3] = {false, false, false};
+  for (int k = 0; k < 3; ++k) {
+    int best = -1;
+    for (int i = 0; i < 3; ++i)
+      if (!used[i] && n[i] > 1 && (best < 0 || st[i] < st[best])) best = i;
+    if (best < 0) break;
+    used[best] = true;
+    if (!out && best != 1 && st[best] == 0) continue;
+    if (st[best] < below) { err = std::string("attention_sink: rows of ") + what + " overlap"; return 1; }
+    below = st[best] * (n[best] - 1) + below;
   }
   return 0;
 }
@@ -257,6 +904,10 @@ int set_args(Ctx* c, const sa3k_sink_attn* p, SinkArgs& a, std::string& err) {
   }
   if (p->Sq >= kFar / 2 || p->Sk >= kFar / 2) { err = "attention_sink: Sq and Sk must be below 2^28"; return 1; }
   if ((int64_t)p->B * p->H > 65535) { err = "attention_sink: B * H must be at most 65535"; return 1; }
+  if ((int64_t)p->B * p->H * ((p->Sk + 127) / 128) >= (1ll << 31)) {
+    err = "attention_sink: too many key tiles for one launch";
+    return 1;
+  }
   if (!(p->scale > 0.f) || !std::isfinite(p->scale)) { err = "attention_sink: scale must be positive"; return 1; }
   if (p->sinks < 0) { err = "attention_sink: sinks must not be negative"; return 1; }
   a.B = p->B; a.H = p->H; a.Hkv = p->H_kv; a.group = p->H / p->H_kv;
@@ -291,7 +942,7 @@ int sa3k_attention_sink_fwd(sa3k_ctx* ctx, const sa3k_sink_attn* p, const sa3k_t
                      check_tensor("v", v, a.B, a.Hkv, a.Sk, false, a.v, e)))
       return 1;
     a.lse = lse;
-    return p->type == kTypeF16 ? forward<__half>(c, a, e) : forward<__nv_bfloat16>(c, a, e);
+    return p->type == kTypeF16 ? forward<false>(c, a, e) : forward<true>(c, a, e);
   });
 }
 
@@ -320,7 +971,7 @@ int sa3k_attention_sink_bwd(sa3k_ctx* ctx, const sa3k_sink_attn* p, const sa3k_t
     a.lse = const_cast<float*>(lse);
     a.D = static_cast<float*>(scratch_get(c, kSlotSinkD, (size_t)std::max<long>(1, (long)a.B * a.H * a.Sq) * sizeof(float), e));
     if (!a.D) return 1;
-    return p->type == kTypeF16 ? backward<__half>(c, a, e) : backward<__nv_bfloat16>(c, a, e);
+    return p->type == kTypeF16 ? backward<false>(c, a, e) : backward<true>(c, a, e);
   });
 }
 
