@@ -23,8 +23,8 @@ namespace {
 // The kernels below share one shape: tiles of 64 rows x 64 values (8 KB, 128-byte swizzle) stream
 // in by TMA, S = Q K^T and its like are formed in tensor memory, threads own one TMEM lane (tile
 // row) each, and P / dS go back to tensor memory as packed 16-bit pairs to be the next product's A
-// operand.  Two CTAs of 8 softmax warps share an SM (each holds half of its tensor memory), so one
-// CTA's softmax and the start and end of its tiles run under the other's products.  The first tile
+// operand.  Several CTAs share an SM and its tensor memory (four of the forward, two of the backward
+// kernels), so one CTA's softmax and the start and end of its work run under the others' products.  The first tile
 // of a window, the last of a sequence and the tiles at its edges are masked; tiles that no row of
 // the CTA sees are never loaded, so the work follows the window and not the sequence.
 constexpr int kSoftWarps = 8, kSinkThreads = 32 * (kSoftWarps + 2);
@@ -104,55 +104,69 @@ __device__ __forceinline__ void zero_rows(uint8_t* tile, int from, int t, int n)
   for (int i = from * 8 + t; i < 512; i += n) reinterpret_cast<uint4*>(tile)[i] = make_uint4(0u, 0u, 0u, 0u);
 }
 
+// A warp's 32 rows of 8 NC values (NC chunks of 16 bytes per lane, its lane's row) to global memory
+// by way of shared memory, so that a store instruction writes whole 128- or 64-byte rows instead of
+// 16 bytes of 32 rows (measured on the forward's 128-row tiles: 6000 cycles a CTA against 1500).
+// `buf`: 32 rows x 128 bytes of this warp's own; `out`: row 0's first value; rows at or past n stay.
+template <int NC>
+__device__ __forceinline__ void store_rows(uint8_t* buf, const uint4 (&w)[NC], uint16_t* out, long ld, int n, int lane) {
+#pragma unroll
+  for (int q = 0; q < NC; ++q) *reinterpret_cast<uint4*>(buf + lane * 128 + ((q ^ (lane & 7)) << 4)) = w[q];
+  __syncwarp();
+  constexpr int PER = 32 / NC;       // rows per store
+#pragma unroll
+  for (int k = 0; k < 32 / PER; ++k) {
+    const int r = k * PER + lane / NC, q = lane % NC;
+    const uint4 v = *reinterpret_cast<const uint4*>(buf + r * 128 + ((q ^ (r & 7)) << 4));
+    if (r < n) *reinterpret_cast<uint4*>(out + (long)r * ld + 8 * q) = v;
+  }
+}
+
 // =================================================================================== forward
-// CTA: one or two groups of 128 query rows of one (batch entry, head), a softmax warpgroup each.
-// TMEM, group g at 128 g: S [0, 64) (P overwrites [0, 32)), O [64, 128).
-// smem: Q 2 x 16 KB | ring of (K 8 KB, V 8 KB) | barriers
-// One warp issues every product, in the order P V(j - 1), S(j) per group: products of one thread
-// complete in order, so the commit of S(j) also says that O holds tile j - 1 and that S's columns,
-// where P(j - 1) lay, are free.
-constexpr int kFwdStages = 4;
-constexpr int kFwdSmem = 32768 + kFwdStages * 2 * kTile + 256 + 1024;
+// CTA: 128 query rows of one (batch entry, head): four softmax warps and one that issues the
+// products.  TMEM: S [0, 64) (P overwrites [0, 32)), O [64, 128).  smem: Q 16 KB | 2 x (K 8 KB, V 8 KB).
+// Four CTAs share an SM (half as much of everything as the kernels below take), so while one loads
+// its first tiles or stores its rows, three others compute: with two CTAs of 256 rows those phases
+// were a third of the time.  The products of one thread complete in order (P V(c - 1), S(c), ...),
+// so when S(c) is there, O holds tile c - 1 and both S's columns, where P(c - 1) lay, and tile
+// c - 1's K and V are free: the thread that sees it loads tile c + 1 there.
+constexpr int kFwdThreads = 160;
+constexpr int kFwdSmem = 16384 + 2 * 2 * kTile + 128 + 1024;
 
 template <bool BF>
-__global__ void __launch_bounds__(kSinkThreads, 2)
+__global__ void __launch_bounds__(kFwdThreads, 4)
     sink_fwd_kernel(const __grid_constant__ SeqMap mq, const __grid_constant__ SeqMap mk, const __grid_constant__ SeqMap mv,
-                    const __grid_constant__ SinkArgs a, int groups) {
+                    const __grid_constant__ SinkArgs a) {
   extern __shared__ uint8_t smem_raw[];
   pdl_trigger();
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;
-  uint8_t* sKV = smem + 32768;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + kFwdStages * 2 * kTile);
+  uint8_t* sKV = smem + 16384;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + 4 * kTile);
   uint64_t* q_full = bars;
-  uint64_t* kv_full = q_full + 1;
-  uint64_t* kv_empty = kv_full + kFwdStages;
-  uint64_t* s_full = kv_empty + kFwdStages;   // [2] S of the group's next tile
-  uint64_t* p_full = s_full + 2;              // [2] P written
-  uint64_t* o_full = p_full + 2;              // [2] the group's last P V done
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
+  uint64_t* kv_full = bars + 1;     // [2]
+  uint64_t* s_full = bars + 3;
+  uint64_t* p_full = bars + 4;
+  uint64_t* o_full = bars + 5;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 6);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (warp == kSoftWarps && lane == 0) {
+  if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
-    for (int s = 0; s < kFwdStages; ++s) {
-      mbar_init(&kv_full[s], 1);
-      mbar_init(&kv_empty[s], 1);
-    }
-    for (int g = 0; g < 2; ++g) {
-      mbar_init(&s_full[g], 1);
-      mbar_init(&p_full[g], 4);
-      mbar_init(&o_full[g], 1);
-    }
+    mbar_init(&kv_full[0], 1);
+    mbar_init(&kv_full[1], 1);
+    mbar_init(s_full, 1);
+    mbar_init(p_full, 4);
+    mbar_init(o_full, 1);
     *abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&mq.m);
     tma_prefetch_desc(&mk.m);
     tma_prefetch_desc(&mv.m);
   }
-  if (warp == kSoftWarps + 1) {
-    tmem_alloc(tmem_slot, 256);
+  if (warp == 4) {
+    tmem_alloc(tmem_slot, 128);
     tmem_relinquish();
     tc_fence_before();
   }
@@ -161,109 +175,114 @@ __global__ void __launch_bounds__(kSinkThreads, 2)
   const uint32_t tbase = *tmem_slot;
   pdl_wait();
 
-  const int bh = blockIdx.y, b = bh / a.H, h = bh % a.H;
-  const int qbase = blockIdx.x * 128 * groups;
+  const int bh = blockIdx.y, b = bh / a.H, h = bh % a.H, r0 = blockIdx.x * 128;
   const SinkSeq s = sink_seq(a, b);
-  auto group_tiles = [&](int g0, int ng) {   // of groups [g0, g0 + ng)
-    const int r0 = qbase + 128 * g0, r1 = min(s.qn, r0 + 128 * ng);
-    return key_tiles(a, s, s.pos0 + r0, s.pos0 + r1 - 1);
-  };
-  const KeyTiles kt = group_tiles(0, groups);
-  const KeyTiles k0t = group_tiles(0, 1), k1t = groups > 1 ? group_tiles(1, 1) : KeyTiles{0, 0, 0};
-  const Waiter wait{abort_flag, a.err};
+  const int rows = min(128, s.qn - r0), plo = s.pos0 + r0, phi = plo + rows - 1;
+  const KeyTiles kt = rows > 0 ? key_tiles(a, s, plo, phi) : KeyTiles{0, 0, 0};
   const WaiterW<> waitw{abort_flag, a.err};
 
-  if (warp == kSoftWarps) {
-    if (lane == 0 && kt.n > 0) {
-      mbar_arrive_expect_tx(q_full, (uint32_t)(2 * kTile * groups));
-      for (int g = 0; g < 2 * groups; ++g) load_tile(sQ + kTile * g, mq, q_full, b, h, qbase + 64 * g);
-      for (int j = 0; j < kt.n; ++j) {
-        const int st = j % kFwdStages;
-        if (j >= kFwdStages && !wait(&kv_empty[st], (uint32_t)((j / kFwdStages) & 1) ^ 1u, kErrTimeoutEmpty)) break;
-        uint8_t* p = sKV + st * 2 * kTile;
-        mbar_arrive_expect_tx(&kv_full[st], 2 * kTile);
-        load_tile(p, mk, &kv_full[st], b, h / a.group, kt.tile(j) * 64);
-        load_tile(p + kTile, mv, &kv_full[st], b, h / a.group, kt.tile(j) * 64);
-      }
-    }
-  } else if (warp == kSoftWarps + 1) {
+  if (warp == 4) {
     constexpr uint32_t id_s = sink_idesc<BF>(0), id_o = sink_idesc<BF>(1);
-    int cnt[2] = {0, 0}, pend[2] = {-1, -1};   // tiles of each group so far; the ring slot whose P V is due
+    const uint64_t qd = kdesc0(smem_u32(sQ)), kd = kdesc0(smem_u32(sKV)), vd = mndesc0(smem_u32(sKV) + kTile);
+    constexpr uint64_t kStage = 2 * kTile >> 4;
     bool ok = kt.n > 0 && waitw(q_full, 0, kErrTimeoutFull);
-    auto flush = [&](int g) {                  // P V of the group's last tile
-      if (pend[g] < 0) return true;
-      if (!waitw(&p_full[g], (uint32_t)((cnt[g] - 1) & 1), kErrTimeoutReady)) return false;
+    auto pv = [&](int c) {       // O += P V of tile c
+      if (!waitw(p_full, (uint32_t)(c & 1), kErrTimeoutReady)) return false;
       tc_fence_after();
-      const uint64_t vd = mndesc0(smem_u32(sKV + pend[g] * 2 * kTile + kTile));
-      const uint32_t tP = tbase + 128 * g;
+      const uint64_t v = vd + (c & 1) * kStage;
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk)
-        umma_ts_w(tP + 64, tP + kk * 8, mnstep(vd, kk), id_o, (cnt[g] > 1 || kk > 0) ? 1u : 0u);
-      pend[g] = -1;
+      for (int kk = 0; kk < 4; ++kk) umma_ts_w(tbase + 64, tbase + kk * 8, mnstep(v, kk), id_o, (c > 0 || kk > 0) ? 1u : 0u);
       return true;
     };
-    for (int j = 0; j < kt.n && ok; ++j) {
-      const int st = j % kFwdStages, t = kt.tile(j);
-      if (!waitw(&kv_full[st], (uint32_t)((j / kFwdStages) & 1), kErrTimeoutFull)) { ok = false; break; }
+    for (int c = 0; c < kt.n && ok; ++c) {
+      if (c > 0 && !(ok = pv(c - 1))) break;
+      if (!waitw(&kv_full[c & 1], (uint32_t)((c >> 1) & 1), kErrTimeoutFull)) { ok = false; break; }
       tc_fence_after();
-      const uint64_t kd = kdesc0(smem_u32(sKV + st * 2 * kTile));
+      const uint64_t k = kd + (c & 1) * kStage;
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        if (!ok) break;
-        if (!(ok = flush(g))) break;
-        if (!(g ? k1t : k0t).has(t)) continue;
-        const uint64_t qd = kdesc0(smem_u32(sQ + 2 * kTile * g));
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) umma_f16_w(tbase + 128 * g, kstep(qd, kk), kstep(kd, kk), id_s, kk > 0 ? 1u : 0u);
-        umma_commit_w(&s_full[g]);
-        ++cnt[g];
-        pend[g] = st;
+      for (int kk = 0; kk < 4; ++kk) umma_f16_w(tbase, kstep(qd, kk), kstep(k, kk), id_s, kk > 0 ? 1u : 0u);
+      umma_commit_w(s_full);
+    }
+    if (ok && pv(kt.n - 1)) umma_commit_w(o_full);
+  } else if (rows > 0) {
+    const int row = 32 * warp + lane, i = r0 + row, p = plo + row;
+    const uint32_t tS = tbase + ((uint32_t)(32 * warp) << 16), tO = tS + 64;
+    auto load_kv = [&](int c) {      // (one thread)
+      uint8_t* st = sKV + (c & 1) * 2 * kTile;
+      mbar_arrive_expect_tx(&kv_full[c & 1], 2 * kTile);
+      load_tile(st, mk, &kv_full[c & 1], b, h / a.group, kt.tile(c) * 64);
+      load_tile(st + kTile, mv, &kv_full[c & 1], b, h / a.group, kt.tile(c) * 64);
+    };
+    if (threadIdx.x == 0 && kt.n > 0) {
+      mbar_arrive_expect_tx(q_full, 2 * kTile);
+      load_tile(sQ, mq, q_full, b, h, r0);
+      load_tile(sQ + kTile, mq, q_full, b, h, r0 + 64);
+      load_kv(0);
+      if (kt.n > 1) load_kv(1);
+    }
+    // tiles that every row sees whole: sink tiles below fs, window tiles of [f0, f1)
+    const int top = min(plo + a.right + 1, s.kn);
+    const int fs = max(0, min(a.sinks, top)) >> 6, f0 = (max(0, phi - a.left) + 63) >> 6, f1 = max(f0, top >> 6);
+    const uint64_t sc2 = f2(a.sl2, a.sl2);
+    float m_used = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int c = 0; c < kt.n; ++c) {
+      const int t = kt.tile(c);
+      if (!waitw(s_full, (uint32_t)(c & 1), kErrTimeoutAccum)) { ok = false; break; }
+      tc_fence_after();
+      if (threadIdx.x == 0 && c > 0 && c + 1 < kt.n) load_kv(c + 1);
+      uint32_t ml = 0xffffffffu, mh = 0xffffffffu;
+      const bool edge = !(t < fs || (t >= f0 && t < f1));
+      if (edge) {
+        const uint64_t mask = seen_mask(a, s, p, t * 64);
+        ml = (uint32_t)mask;
+        mh = (uint32_t)(mask >> 32);
       }
-      if (ok && j > 0) umma_commit_w(&kv_empty[(j - 1) % kFwdStages]);   // its P V are all issued
-    }
-    for (int g = 0; g < 2 && ok; ++g) {
-      ok = flush(g);
-      if (ok && cnt[g] > 0) umma_commit_w(&o_full[g]);
-    }
-  } else {
-    const int g = warp >> 2, quarter = warp & 3, row = 32 * quarter + lane;
-    const int r0 = qbase + 128 * g, i = r0 + row;
-    const uint32_t tS = tbase + 128 * g + ((uint32_t)(32 * quarter) << 16), tO = tS + 64;
-    const int rows = g < groups ? min(128, s.qn - r0) : 0;
-    if (rows > 0) {
-      const KeyTiles my = g ? k1t : k0t;
-      const int plo = s.pos0 + r0, phi = plo + rows - 1, p = plo + row;
-      float m_used = -INFINITY, l = 0.f;
-      bool ok = true;
-      int c = 0;
-      for (int j = 0; j < kt.n; ++j) {
-        const int t = kt.tile(j);
-        if (!my.has(t)) continue;
-        if (!waitw(&s_full[g], (uint32_t)(c & 1), kErrTimeoutAccum)) { ok = false; break; }
-        tc_fence_after();
-        uint32_t v[64];
-        tmem_ld32(tS, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
-        tmem_ld32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
-        tmem_ld_wait();
-        if (!tile_all_seen(a, s, plo, phi, t * 64)) {
-          const uint64_t mask = seen_mask(a, s, p, t * 64);
-          const uint32_t ml = (uint32_t)mask, mh = (uint32_t)(mask >> 32);
+      // P = 2^(x - m) in one pass with the base m of the tiles before, while the row's maximum is
+      // taken; the base stays unless the maximum is more than 2^8 above it (P then stays below 2^8,
+      // and O is rescaled rarely).  Otherwise, as in the first tile, the pass is made again.
+      uint32_t pk[32];
+      float lt;
+      while (true) {
+        const float mb = m_used == -INFINITY ? 0.f : m_used;
+        const uint64_t nb2 = f2(-mb, -mb);
+        uint64_t ls[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            if (!((ml >> e) & 1u)) v[e] = 0xff800000u;
-            if (!((mh >> e) & 1u)) v[32 + e] = 0xff800000u;
+        for (int q = 0; q < 2; ++q) {
+          uint32_t v[32];
+          tmem_ld32(tS + 32 * q, v);
+          tmem_ld_wait();
+          if (edge) {
+            const uint32_t mm = q ? mh : ml;
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!((mm >> e) & 1u)) v[e] = 0xff800000u;
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            mx[e & 3] = max3(mx[e & 3], __uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
+            float x0, x1;
+            f2split(ffma2(f2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), sc2, nb2), x0, x1);
+            const float p0 = ex2(x0), p1 = ex2(x1);
+            ls[e & 1] = fadd2(ls[e & 1], f2(p0, p1));
+            pk[16 * q + e] = pack2<BF>(p0, p1);
           }
         }
-        const float mx = rowmax64(v) * a.sl2;
-        // the exponent's base stays unless the row's maximum grew by more than 2^8: P then stays
-        // below 2^8 and O is rescaled rarely
-        const bool grow = mx > m_used + 8.f;
+        const float top_x = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.sl2;
+        float l0, l1, l2, l3;
+        f2split(ls[0], l0, l1);
+        f2split(ls[1], l2, l3);
+        lt = (l0 + l1) + (l2 + l3);
+        const bool grow = top_x > m_used + 8.f;
+        if (!__any_sync(0xffffffffu, grow)) break;
         float alpha = 1.f;
         if (grow) {
-          alpha = m_used == -INFINITY ? 0.f : ex2(m_used - mx);
-          m_used = mx;
+          alpha = m_used == -INFINITY ? 0.f : ex2(m_used - top_x);
+          m_used = top_x;
         }
-        if (__any_sync(0xffffffffu, grow && c > 0)) {
+        l *= alpha;
+        if (c > 0) {
 #pragma unroll 1
           for (int q = 0; q < 4; ++q) {
             uint32_t o[16];
@@ -274,67 +293,50 @@ __global__ void __launch_bounds__(kSinkThreads, 2)
             tmem_st16(tO + 16 * q, o);
           }
         }
-        l *= alpha;
-        const float mb = m_used == -INFINITY ? 0.f : m_used;
-        const uint64_t sc2 = f2(a.sl2, a.sl2), nb2 = f2(-mb, -mb);
-        uint64_t ls[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            float x0, x1;
-            f2split(ffma2(f2(__uint_as_float(v[32 * q + 2 * e]), __uint_as_float(v[32 * q + 2 * e + 1])), sc2, nb2), x0, x1);
-            const float p0 = ex2(x0), p1 = ex2(x1);
-            ls[e & 1] = fadd2(ls[e & 1], f2(p0, p1));
-            pk[e] = pack2<BF>(p0, p1);
-          }
-          tmem_st16(tS + 16 * q, pk);
-        }
-        float l0, l1, l2, l3;
-        f2split(ls[0], l0, l1);
-        f2split(ls[1], l2, l3);
-        l += (l0 + l1) + (l2 + l3);
-        if (t * 64 + 64 > s.kn && s.kn < a.Sk) {   // values behind the sequence's end
-          const int st = j % kFwdStages;
-          if (!waitw(&kv_full[st], (uint32_t)((j / kFwdStages) & 1), kErrTimeoutFull)) { ok = false; break; }
-          zero_rows(sKV + st * 2 * kTile + kTile, max(0, s.kn - t * 64), row, 128);
-          fence_proxy_async_smem();
-        }
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[g]);
-        ++c;
       }
-      const bool have = ok && c > 0 && waitw(&o_full[g], 0, kErrTimeoutAccum);
-      tc_fence_after();
-      const float inv = l > 0.f ? 1.f / l : l;     // (0 for an empty row; NaN stays)
-      uint32_t o[64];
-      if (have) {
-        tmem_ld32(tO, *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
-        tmem_ld32(tO + 32, *reinterpret_cast<uint32_t(*)[32]>(&o[32]));
-        tmem_ld_wait();
+      l += lt;
+      tmem_st16(tS, *reinterpret_cast<uint32_t(*)[16]>(&pk[0]));
+      tmem_st16(tS + 16, *reinterpret_cast<uint32_t(*)[16]>(&pk[16]));
+      if (t * 64 + 64 > s.kn && s.kn < a.Sk) {   // values behind the sequence's end (its last tile)
+        if (!waitw(&kv_full[c & 1], (uint32_t)((c >> 1) & 1), kErrTimeoutFull)) { ok = false; break; }
+        zero_rows(sKV + (c & 1) * 2 * kTile + kTile, max(0, s.kn - t * 64), row, 128);
+        fence_proxy_async_smem();
       }
-      if (ok && (have || c == 0) && row < rows) {
-        uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.o.p) + (long)b * a.o.sb + (long)h * a.o.sh + (long)i * a.o.ld);
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          uint32_t w[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            w[e] = l == 0.f ? 0u
-                            : pack2<BF>(__uint_as_float(o[8 * q + 2 * e]) * inv, __uint_as_float(o[8 * q + 2 * e + 1]) * inv);
-          dst[q] = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-        if (a.lse) a.lse[(long)bh * a.Sq + i] = l == 0.f ? -INFINITY : m_used + log2f(l);
-      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full);
     }
+    const bool have = ok && kt.n > 0 && waitw(o_full, 0, kErrTimeoutAccum);
+    tc_fence_after();
+    const bool empty = m_used == -INFINITY && l == l;   // no visible key (a NaN score stays a NaN)
+    const float inv = 1.f / l;
+    uint16_t* out = static_cast<uint16_t*>(a.o.p) + (long)b * a.o.sb + (long)h * a.o.sh + (long)(r0 + 32 * warp) * a.o.ld;
+    if (have) {
+      uint32_t o[64];
+      tmem_ld32(tO, *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
+      tmem_ld32(tO + 32, *reinterpret_cast<uint32_t(*)[32]>(&o[32]));
+      tmem_ld_wait();
+      uint4 w[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        uint32_t x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          x[e] = empty ? 0u : pack2<BF>(__uint_as_float(o[8 * q + 2 * e]) * inv, __uint_as_float(o[8 * q + 2 * e + 1]) * inv);
+        w[q] = make_uint4(x[0], x[1], x[2], x[3]);
+      }
+      store_rows<8>(sQ + 4096 * warp, w, out, a.o.ld, rows - 32 * warp, lane);   // (the products have read Q)
+    } else if (ok && row < rows) {      // no row sees a key
+#pragma unroll
+      for (int q = 0; q < 8; ++q) *reinterpret_cast<uint4*>(out + (long)lane * a.o.ld + 8 * q) = make_uint4(0u, 0u, 0u, 0u);
+    }
+    if (ok && a.lse && row < rows) a.lse[(long)bh * a.Sq + i] = empty ? -INFINITY : m_used + log2f(l);
   }
   __syncthreads();
-  if (warp == kSoftWarps + 1) {
+  if (warp == 4) {
     tc_fence_after();
-    tmem_dealloc(tbase, 256);
+    tmem_dealloc(tbase, 128);
   }
 }
 
@@ -343,26 +345,26 @@ __global__ void __launch_bounds__(kSinkThreads, 2)
 // a tile's 64 keys each.  The threads copy S and dP to registers and give their columns back at
 // once, so the next tile's products run under this tile's exponentials; dS has columns of its own.
 // TMEM: S [0, 64), dP [64, 128), dQ [128, 192), dS in two buffers of 32 columns at 192 and 224.
-constexpr int kDqStages = 4;
-constexpr int kDqSmem = 32768 + kDqStages * 2 * kTile + 256 + 1024;
+constexpr int kDqStages = 3;
+constexpr int kDqSmem = 49152 + kDqStages * 2 * kTile + 256 + 1024;
 
 template <bool BF>
 __global__ void __launch_bounds__(kSinkThreads, 2)
-    sink_dq_kernel(const __grid_constant__ SeqMap mq, const __grid_constant__ SeqMap mdo, const __grid_constant__ SeqMap mk,
-                   const __grid_constant__ SeqMap mv, const __grid_constant__ SinkArgs a) {
+    sink_dq_kernel(const __grid_constant__ SeqMap mq, const __grid_constant__ SeqMap mdo, const __grid_constant__ SeqMap mo,
+                   const __grid_constant__ SeqMap mk, const __grid_constant__ SeqMap mv, const __grid_constant__ SinkArgs a) {
   extern __shared__ uint8_t smem_raw[];
   pdl_trigger();
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sQ = smem;                   // Q 16 KB | dO 16 KB
-  uint8_t* sKV = smem + 32768;
+  uint8_t* sQ = smem;                   // Q 16 KB | dO 16 KB | O 16 KB
+  uint8_t* sKV = smem + 49152;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + kDqStages * 2 * kTile);
   uint64_t* q_full = bars;
   uint64_t* kv_full = q_full + 1;
   uint64_t* kv_empty = kv_full + kDqStages;
   uint64_t* s_full = kv_empty + kDqStages;
   uint64_t* s_read = s_full + 1;
-  uint64_t* ds_full = s_read + 1;
-  uint64_t* ds_free = ds_full + 1;      // [2]
+  uint64_t* ds_full = s_read + 1;       // [2] per dS buffer: with one barrier, the next tile's phase could
+  uint64_t* ds_free = ds_full + 2;      // [2]   end before the issuing warp has seen this one's
   uint64_t* acc_full = ds_free + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -376,7 +378,8 @@ __global__ void __launch_bounds__(kSinkThreads, 2)
     }
     mbar_init(s_full, 1);
     mbar_init(s_read, kSoftWarps);
-    mbar_init(ds_full, kSoftWarps);
+    mbar_init(&ds_full[0], kSoftWarps);
+    mbar_init(&ds_full[1], kSoftWarps);
     mbar_init(&ds_free[0], 1);
     mbar_init(&ds_free[1], 1);
     mbar_init(acc_full, 1);
@@ -384,6 +387,7 @@ __global__ void __launch_bounds__(kSinkThreads, 2)
     fence_barrier_init();
     tma_prefetch_desc(&mq.m);
     tma_prefetch_desc(&mdo.m);
+    tma_prefetch_desc(&mo.m);
     tma_prefetch_desc(&mk.m);
     tma_prefetch_desc(&mv.m);
   }
@@ -405,11 +409,12 @@ __global__ void __launch_bounds__(kSinkThreads, 2)
   const WaiterW<> waitw{abort_flag, a.err};
 
   if (warp == kSoftWarps) {
-    if (lane == 0 && kt.n > 0) {
-      mbar_arrive_expect_tx(q_full, 4 * kTile);
+    if (lane == 0 && rows > 0) {
+      mbar_arrive_expect_tx(q_full, 6 * kTile);
       for (int g = 0; g < 2; ++g) {
         load_tile(sQ + kTile * g, mq, q_full, b, h, r0 + 64 * g);
         load_tile(sQ + 2 * kTile + kTile * g, mdo, q_full, b, h, r0 + 64 * g);
+        load_tile(sQ + 4 * kTile + kTile * g, mo, q_full, b, h, r0 + 64 * g);
       }
       for (int j = 0; j < kt.n; ++j) {
         const int st = j % kDqStages;
@@ -425,7 +430,7 @@ __global__ void __launch_bounds__(kSinkThreads, 2)
     const uint64_t qd = kdesc0(smem_u32(sQ)), dd = kdesc0(smem_u32(sQ + 2 * kTile));
     bool ok = kt.n > 0 && waitw(q_full, 0, kErrTimeoutFull);
     auto grad = [&](int j) {     // dQ += dS K of tile j
-      if (!waitw(ds_full, (uint32_t)(j & 1), kErrTimeoutReady)) return false;
+      if (!waitw(&ds_full[j & 1], (uint32_t)((j >> 1) & 1), kErrTimeoutReady)) return false;
       tc_fence_after();
       const uint64_t kmn = mndesc0(smem_u32(sKV + (j % kDqStages) * 2 * kTile));
 #pragma unroll
@@ -459,13 +464,13 @@ __global__ void __launch_bounds__(kSinkThreads, 2)
     if (mine) {
       lse = a.lse[(long)bh * a.Sq + i];
       if (lse == -INFINITY) lse = INFINITY;      // a row that sees nothing: P = 0
-      const long off_o = (long)b * a.o.sb + (long)h * a.o.sh + (long)i * a.o.ld;
-      const long off_d = (long)b * a.dO.sb + (long)h * a.dO.sh + (long)i * a.dO.ld;
-      const uint4* po = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.o.p) + off_o);
-      const uint4* pd = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.dO.p) + off_d);
+    }
+    bool ok = waitw(q_full, 0, kErrTimeoutFull);
+    if (ok) {
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
-        const uint4 x = po[q], y = pd[q];
+        const int off = row * 128 + ((q ^ (row & 7)) << 4);
+        const uint4 x = *reinterpret_cast<const uint4*>(sQ + 2 * kTile + off), y = *reinterpret_cast<const uint4*>(sQ + 4 * kTile + off);
         const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -474,11 +479,10 @@ __global__ void __launch_bounds__(kSinkThreads, 2)
           D = fmaf(u.y, w.y, D);
         }
       }
-      if (g == 0) a.D[(long)bh * a.Sq + i] = D;
+      if (g == 0 && mine) a.D[(long)bh * a.Sq + i] = D;
     }
     const uint64_t sc2 = f2(a.sl2, a.sl2), nl2 = f2(-lse, -lse), nd2 = f2(-D, -D);
-    bool ok = true;
-    for (int j = 0; j < kt.n; ++j) {
+    for (int j = 0; j < kt.n && ok; ++j) {
       const int t = kt.tile(j);
       if (!waitw(s_full, (uint32_t)(j & 1), kErrTimeoutAccum)) { ok = false; break; }
       tc_fence_after();
@@ -517,7 +521,7 @@ __global__ void __launch_bounds__(kSinkThreads, 2)
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(ds_full);
+      if (lane == 0) mbar_arrive(&ds_full[j & 1]);
     }
     const bool have = ok && kt.n > 0 && waitw(acc_full, 0, kErrTimeoutAccum);
     tc_fence_after();
@@ -526,18 +530,22 @@ __global__ void __launch_bounds__(kSinkThreads, 2)
       tmem_ld32(tbase + lane_off + 128 + 32 * g, o);
       tmem_ld_wait();
     }
-    if (mine && ok && (have || kt.n == 0)) {
-      uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.dq.p) + (long)b * a.dq.sb + (long)h * a.dq.sh +
-                                            (long)i * a.dq.ld + 32 * g);
+    uint16_t* out = static_cast<uint16_t*>(a.dq.p) + (long)b * a.dq.sb + (long)h * a.dq.sh + (long)(r0 + 32 * quarter) * a.dq.ld + 32 * g;
+    if (have) {
+      uint4 w[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        uint32_t w[4];
+        uint32_t x[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          w[e] = kt.n == 0 ? 0u
-                           : pack2<BF>(__uint_as_float(o[8 * q + 2 * e]) * a.scale, __uint_as_float(o[8 * q + 2 * e + 1]) * a.scale);
-        dst[q] = make_uint4(w[0], w[1], w[2], w[3]);
+          x[e] = pack2<BF>(__uint_as_float(o[8 * q + 2 * e]) * a.scale, __uint_as_float(o[8 * q + 2 * e + 1]) * a.scale);
+        w[q] = make_uint4(x[0], x[1], x[2], x[3]);
       }
+      // (the products have read Q and dO: 32 KB for the 8 warps' rows)
+      store_rows<4>(sQ + 4096 * warp, w, out, a.dq.ld, rows - 32 * quarter, lane);
+    } else if (ok && mine) {      // no row sees a key
+#pragma unroll
+      for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(out + (long)lane * a.dq.ld + 8 * q) = make_uint4(0u, 0u, 0u, 0u);
     }
   }
   __syncthreads();
@@ -617,8 +625,15 @@ __global__ void __launch_bounds__(kSinkThreads, 2)
     }
   }
   const int n = nt * a.group;
-  auto head_of = [&](int j) { return hk * a.group + j / nt; };
-  auto tile_of = [&](int j) { return qt0 + j % nt; };
+  // step j: query head hk group + j / nt, tile qt0 + j % nt; walked with a cursor
+  struct Step {
+    int h, t;
+    __device__ __forceinline__ void next(int end, int first) {
+      if (++t == end) { t = first; ++h; }
+    }
+  };
+  Step at{hk * a.group, qt0};
+  const int qt1 = qt0 + nt;
   const Waiter wait{abort_flag, a.err};
   const WaiterW<> waitw{abort_flag, a.err};
 
@@ -634,8 +649,9 @@ __global__ void __launch_bounds__(kSinkThreads, 2)
         if (j >= kDkvStages && !wait(&q_empty[st], (uint32_t)((j / kDkvStages) & 1) ^ 1u, kErrTimeoutEmpty)) break;
         uint8_t* p = sQd + st * 2 * kTile;
         mbar_arrive_expect_tx(&q_full[st], 2 * kTile);
-        load_tile(p, mq, &q_full[st], b, head_of(j), tile_of(j) * 64);
-        load_tile(p + kTile, mdo, &q_full[st], b, head_of(j), tile_of(j) * 64);
+        load_tile(p, mq, &q_full[st], b, at.h, at.t * 64);
+        load_tile(p + kTile, mdo, &q_full[st], b, at.h, at.t * 64);
+        at.next(qt1, qt0);
       }
     }
   } else if (warp == kSoftWarps + 1) {
@@ -677,29 +693,30 @@ __global__ void __launch_bounds__(kSinkThreads, 2)
     const uint32_t lane_off = (uint32_t)(32 * quarter) << 16;
     const uint32_t tS = tbase + lane_off + 32 * g, tP = tS + 64;
     // thread t < 32 fetches the lse of the group's column t one step ahead, 32 <= t < 64 the D
-    auto fetch = [&](int j) -> float {
-      const int i = tile_of(j) * 64 + 32 * g + (t & 31);
+    auto fetch = [&](const Step& x) -> float {
+      const int i = x.t * 64 + 32 * g + (t & 31);
       if (i >= s.qn) return t < 32 ? INFINITY : 0.f;
-      const long r = ((long)b * a.H + head_of(j)) * a.Sq + i;
+      const long r = ((long)b * a.H + x.h) * a.Sq + i;
       if (t >= 32) return a.D[r];
-      const float x = a.lse[r];
-      return x == -INFINITY ? INFINITY : x;
+      const float v = a.lse[r];
+      return v == -INFINITY ? INFINITY : v;
     };
     const uint64_t sc2 = f2(a.sl2, a.sl2);
     bool ok = true;
-    float next = n > 0 && t < 64 ? fetch(0) : 0.f;
+    float next = n > 0 && t < 64 ? fetch(at) : 0.f;
     for (int j = 0; j < n; ++j) {
+      const int q0 = at.t * 64, pq = s.pos0 + q0;
+      at.next(qt1, qt0);
       float* ldb = s_ld + 128 * g + 64 * (j & 1);
       if (t < 64) {
         ldb[4 * ((t & 31) >> 1) + (t >= 32 ? 2 : 0) + (t & 1)] = next;
-        if (j + 1 < n) next = fetch(j + 1);
+        if (j + 1 < n) next = fetch(at);
       }
       if (g == 0) named_bar(1, 128);   // (every warp of the group passes it once per step, also after an abort)
       else named_bar(2, 128);
       if (ok) ok = waitw(s_full, (uint32_t)(j & 1), kErrTimeoutAccum);
       if (!ok) continue;
       tc_fence_after();
-      const int q0 = tile_of(j) * 64, pq = s.pos0 + q0;
       // queries of the tile that see key kj: position from kj - right to kj + left (any, for a sink)
       const bool edge = q0 + 64 > s.qn || k0 + 128 > s.kn || k0 + 127 > pq + a.right ||
                         !(k0 + 127 < a.sinks || k0 >= pq + 63 - a.left);
@@ -756,18 +773,22 @@ __global__ void __launch_bounds__(kSinkThreads, 2)
       tmem_ld32(tbase + lane_off + 160 + 64 * g, *reinterpret_cast<uint32_t(*)[32]>(&o[32]));
       tmem_ld_wait();
     }
-    if (row < keys && ok && (have || n == 0)) {
+    if (ok && (have || n == 0)) {
       const SinkTensor& out = g == 0 ? a.dv : a.dk;
       const float mul = g == 0 ? 1.f : a.scale;
-      uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(out.p) + (long)b * out.sb + (long)hk * out.sh + (long)kj * out.ld);
+      uint4 w[8];
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
-        uint32_t w[4];
+        uint32_t x[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          w[e] = n == 0 ? 0u : pack2<BF>(__uint_as_float(o[8 * q + 2 * e]) * mul, __uint_as_float(o[8 * q + 2 * e + 1]) * mul);
-        dst[q] = make_uint4(w[0], w[1], w[2], w[3]);
+          x[e] = n == 0 ? 0u : pack2<BF>(__uint_as_float(o[8 * q + 2 * e]) * mul, __uint_as_float(o[8 * q + 2 * e + 1]) * mul);
+        w[q] = make_uint4(x[0], x[1], x[2], x[3]);
       }
+      // (the products have read K and V)
+      store_rows<8>(sK + 4096 * warp, w,
+                    static_cast<uint16_t*>(out.p) + (long)b * out.sb + (long)hk * out.sh + (long)(k0 + 32 * quarter) * out.ld, out.ld,
+                    keys - 32 * quarter, lane);
     }
   }
   __syncthreads();
@@ -822,12 +843,9 @@ int forward(Ctx* c, const SinkArgs& a, std::string& err) {
     return 1;
   auto kern = sink_fwd_kernel<BF>;
   if (smem_attr(reinterpret_cast<const void*>(kern), kFwdSmem, c->device, "attention_sink smem attribute", err)) return 1;
-  // 256 rows per CTA share each key tile; 128 where that would leave SMs without a CTA
-  const long ctas = (long)a.B * a.H * ((a.Sq + 255) / 256);
-  const int groups = ctas >= 2 * (long)c->sm_count && a.Sq > 128 ? 2 : 1;
   ProfScope prof_(c, "attn_sink.fwd");
-  launch_pdl(c, kern, dim3((unsigned)((a.Sq + 128 * groups - 1) / (128 * groups)), (unsigned)(a.B * a.H)), dim3(kSinkThreads),
-             (size_t)kFwdSmem, mq, mk, mv, a, groups);
+  launch_pdl(c, kern, dim3((unsigned)((a.Sq + 127) / 128), (unsigned)(a.B * a.H)), dim3(kFwdThreads), (size_t)kFwdSmem, mq, mk,
+             mv, a);
   return check_launch("attention with sinks, forward", err);
 }
 
@@ -835,10 +853,12 @@ template <bool BF>
 int backward(Ctx* c, const SinkArgs& a, std::string& err) {
   const bool noq = a.Sq == 0, nokeys = a.Sk == 0;
   if (noq && nokeys) return 0;
-  SeqMap mq, mdo, mk, mv;
+  SeqMap mq, mdo, mo, mk, mv;
+  const SinkTensor &to = noq ? a.k : a.o;
   const SinkTensor &tq = noq ? a.k : a.q, &td = noq ? a.k : a.dO, &tk = nokeys ? a.q : a.k, &tv = nokeys ? a.q : a.v;
   const int hq = noq ? a.Hkv : a.H, sq = noq ? a.Sk : a.Sq, hk = nokeys ? a.H : a.Hkv, sk = nokeys ? a.Sq : a.Sk;
   if (make_seq_map(&mq, BF, tq, a.B, hq, sq, err) || make_seq_map(&mdo, BF, td, a.B, hq, sq, err) ||
+      make_seq_map(&mo, BF, to, a.B, hq, sq, err) ||
       make_seq_map(&mk, BF, tk, a.B, hk, sk, err) || make_seq_map(&mv, BF, tv, a.B, hk, sk, err))
     return 1;
   if (!noq) {
@@ -846,7 +866,7 @@ int backward(Ctx* c, const SinkArgs& a, std::string& err) {
     if (smem_attr(reinterpret_cast<const void*>(kern), kDqSmem, c->device, "attention_sink smem attribute", err)) return 1;
     ProfScope prof_(c, "attn_sink.dq");
     launch_pdl(c, kern, dim3((unsigned)((a.Sq + 127) / 128), (unsigned)(a.B * a.H)), dim3(kSinkThreads), (size_t)kDqSmem, mq,
-               mdo, mk, mv, a);
+               mdo, mo, mk, mv, a);
     if (check_launch("attention with sinks, dq", err)) return 1;
   }
   if (!a.dk.p || nokeys) return 0;
