@@ -23,7 +23,7 @@ namespace {
 // The kernels below share one shape: tiles of 64 rows x 64 values (8 KB, 128-byte swizzle) stream
 // in by TMA, S = Q K^T and its like are formed in tensor memory, threads own one TMEM lane (tile
 // row) each, and P / dS go back to tensor memory as packed 16-bit pairs to be the next product's A
-// operand.  Several CTAs share an SM and its tensor memory (four of the forward, two of the backward
+// operand.  Several CTAs share an SM and its tensor memory (three of the forward, two of the backward
 // kernels), so one CTA's softmax and the start and end of its work run under the others' products.  The first tile
 // of a window, the last of a sequence and the tiles at its edges are masked; tiles that no row of
 // the CTA sees are never loaded, so the work follows the window and not the sequence.
@@ -67,6 +67,37 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8])
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
                "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
+}
+
+// 2^x of a pair without the MUFU unit, whose 16 values a clock per SM would bound the softmax alone:
+// x = n + f with n = round(x) (adding 1.5 * 2^23 leaves n in the low mantissa bits) and a polynomial
+// for 2^f on [-1/2, 1/2], degree 4, fitted here by iteratively reweighted least squares for the least
+// relative error (2.6e-6, of either sign), n added into the exponent field.  x is clamped at -125:
+// what lies below gives 2^-125.
+__device__ __forceinline__ void ex2_pair(float x0, float x1, float& y0, float& y1) {
+  constexpr float kMagic = 12582912.f;
+  const uint64_t x = f2(fmaxf(x0, -125.f), fmaxf(x1, -125.f));
+  const uint64_t t = fadd2(x, f2(kMagic, kMagic));
+  const uint64_t f = ffma2(fadd2(t, f2(-kMagic, -kMagic)), f2(-1.f, -1.f), x);
+  uint64_t p = ffma2(f2(0.009570101f, 0.009570101f), f, f2(0.05591786f, 0.05591786f));
+  p = ffma2(p, f, f2(0.24024744f, 0.24024744f));
+  p = ffma2(p, f, f2(0.6931218f, 0.6931218f));
+  p = ffma2(p, f, f2(0.9999993f, 0.9999993f));
+  float p0, p1, t0, t1;
+  f2split(p, p0, p1);
+  f2split(t, t0, t1);
+  y0 = __uint_as_float((__float_as_uint(t0) << 23) + __float_as_uint(p0));   // (the magic's own bits leave the word)
+  y1 = __uint_as_float((__float_as_uint(t1) << 23) + __float_as_uint(p1));
+}
+// pair e of a row: one of every kPolyOf by the polynomial
+constexpr int kPolyOf = 4;
+__device__ __forceinline__ void ex2_at(int e, float x0, float x1, float& y0, float& y1) {
+  if (e % kPolyOf == 1) {
+    ex2_pair(x0, x1, y0, y1);
+  } else {
+    y0 = ex2(x0);
+    y1 = ex2(x1);
+  }
 }
 
 // The 64-key tiles that rows at positions [plo, phi] see: the sink tiles [0, ns), then the window's
@@ -123,42 +154,49 @@ __device__ __forceinline__ void store_rows(uint8_t* buf, const uint4 (&w)[NC], u
 }
 
 // =================================================================================== forward
-// CTA: 128 query rows of one (batch entry, head): four softmax warps and one that issues the
-// products.  TMEM: S [0, 64) (P overwrites [0, 32)), O [64, 128).  smem: Q 16 KB | 2 x (K 8 KB, V 8 KB).
-// Four CTAs share an SM (half as much of everything as the kernels below take), so while one loads
-// its first tiles or stores its rows, three others compute: with two CTAs of 256 rows those phases
-// were a third of the time.  The products of one thread complete in order (P V(c - 1), S(c), ...),
-// so when S(c) is there, O holds tile c - 1 and both S's columns, where P(c - 1) lay, and tile
-// c - 1's K and V are free: the thread that sees it loads tile c + 1 there.
+// CTA: 128 query rows of one (batch entry, head): four softmax warps (a thread per row), and one warp
+// that issues loads and products.  Three CTAs share an SM.
+// TMEM: S [0, 64), O [64, 128).  smem: Q 16 KB | P 16 KB | 2 x K 8 KB | 2 x V 8 KB | barriers.
+// The threads copy S to registers and give its columns back at once, and P goes through shared
+// memory, so S of the next tile is formed under this tile's exponentials, and P V under the next
+// one's: a tile's chain is the softmax alone (with P over S's columns the products' latency was 40%
+// of it).  What then bounds the kernel is the exponentials: 16 a clock per SM, 512 clocks a tile.
 constexpr int kFwdThreads = 160;
-constexpr int kFwdSmem = 16384 + 2 * 2 * kTile + 128 + 1024;
+constexpr int kFwdSmem = 32768 + 4 * kTile + 128 + 1024;
 
 template <bool BF>
-__global__ void __launch_bounds__(kFwdThreads, 4)
+__global__ void __launch_bounds__(kFwdThreads, 3)
     sink_fwd_kernel(const __grid_constant__ SeqMap mq, const __grid_constant__ SeqMap mk, const __grid_constant__ SeqMap mv,
                     const __grid_constant__ SinkArgs a) {
   extern __shared__ uint8_t smem_raw[];
   pdl_trigger();
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;
-  uint8_t* sKV = smem + 16384;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + 4 * kTile);
+  uint8_t* sP = smem + 16384;
+  uint8_t* sK = smem + 32768;             // [2]
+  uint8_t* sV = sK + 2 * kTile;           // [2]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + 2 * kTile);
   uint64_t* q_full = bars;
-  uint64_t* kv_full = bars + 1;     // [2]
-  uint64_t* s_full = bars + 3;
-  uint64_t* p_full = bars + 4;
-  uint64_t* o_full = bars + 5;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 6);
+  uint64_t* k_full = bars + 1;            // [2]
+  uint64_t* v_full = bars + 3;            // [2]
+  uint64_t* s_full = bars + 5;            // S of a tile is there
+  uint64_t* s_read = bars + 6;            // it is in the threads' registers
+  uint64_t* p_full = bars + 7;            // P is in shared memory (and the tile before's P V is done)
+  uint64_t* pv_done = bars + 8;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 9);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == 128) {
     mbar_init(q_full, 1);
-    mbar_init(&kv_full[0], 1);
-    mbar_init(&kv_full[1], 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&v_full[i], 1);
+    }
     mbar_init(s_full, 1);
+    mbar_init(s_read, 4);
     mbar_init(p_full, 4);
-    mbar_init(o_full, 1);
+    mbar_init(pv_done, 1);
     *abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&mq.m);
@@ -166,6 +204,7 @@ __global__ void __launch_bounds__(kFwdThreads, 4)
     tma_prefetch_desc(&mv.m);
   }
   if (warp == 4) {
+    __syncwarp();
     tmem_alloc(tmem_slot, 128);
     tmem_relinquish();
     tc_fence_before();
@@ -183,43 +222,55 @@ __global__ void __launch_bounds__(kFwdThreads, 4)
 
   if (warp == 4) {
     constexpr uint32_t id_s = sink_idesc<BF>(0), id_o = sink_idesc<BF>(1);
-    const uint64_t qd = kdesc0(smem_u32(sQ)), kd = kdesc0(smem_u32(sKV)), vd = mndesc0(smem_u32(sKV) + kTile);
-    constexpr uint64_t kStage = 2 * kTile >> 4;
-    bool ok = kt.n > 0 && waitw(q_full, 0, kErrTimeoutFull);
-    auto pv = [&](int c) {       // O += P V of tile c
-      if (!waitw(p_full, (uint32_t)(c & 1), kErrTimeoutReady)) return false;
-      tc_fence_after();
-      const uint64_t v = vd + (c & 1) * kStage;
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk) umma_ts_w(tbase + 64, tbase + kk * 8, mnstep(v, kk), id_o, (c > 0 || kk > 0) ? 1u : 0u);
-      return true;
+    constexpr uint64_t kSlot = kTile >> 4;
+    const uint64_t qd = kdesc0(smem_u32(sQ)), pd = kdesc0(smem_u32(sP)), kd = kdesc0(smem_u32(sK)), vd = mndesc0(smem_u32(sV));
+    const int hk = h / a.group;
+    auto load = [&](uint8_t* dst, const SeqMap& m, uint64_t* bar, int c) {
+      if (lane == 0) {
+        mbar_arrive_expect_tx(bar, kTile);
+        load_tile(dst + (c & 1) * kTile, m, bar, b, hk, kt.tile(c) * 64);
+      }
+      __syncwarp();
     };
-    for (int c = 0; c < kt.n && ok; ++c) {
-      if (c > 0 && !(ok = pv(c - 1))) break;
-      if (!waitw(&kv_full[c & 1], (uint32_t)((c >> 1) & 1), kErrTimeoutFull)) { ok = false; break; }
+    auto scores = [&](int c) {       // S = Q K^T of tile c
+      if (!waitw(&k_full[c & 1], (uint32_t)((c >> 1) & 1), kErrTimeoutFull)) return false;
       tc_fence_after();
-      const uint64_t k = kd + (c & 1) * kStage;
+      const uint64_t k = kd + (c & 1) * kSlot;
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) umma_f16_w(tbase, kstep(qd, kk), kstep(k, kk), id_s, kk > 0 ? 1u : 0u);
       umma_commit_w(s_full);
+      return true;
+    };
+    bool ok = kt.n > 0;
+    if (ok) {
+      if (lane == 0) {
+        mbar_arrive_expect_tx(q_full, 2 * kTile);
+        load_tile(sQ, mq, q_full, b, h, r0);
+        load_tile(sQ + kTile, mq, q_full, b, h, r0 + 64);
+      }
+      for (int c = 0; c < min(2, kt.n); ++c) {
+        load(sK, mk, &k_full[c], c);
+        load(sV, mv, &v_full[c], c);
+      }
+      ok = waitw(q_full, 0, kErrTimeoutFull) && scores(0);
     }
-    if (ok && pv(kt.n - 1)) umma_commit_w(o_full);
+    for (int c = 0; c < kt.n && ok; ++c) {
+      if (!waitw(s_read, (uint32_t)(c & 1), kErrTimeoutOther)) break;
+      if (c + 1 < kt.n && !scores(c + 1)) break;
+      if (c + 2 < kt.n) load(sK, mk, &k_full[c & 1], c + 2);                       // (S(c) has read its K)
+      if (!waitw(p_full, (uint32_t)(c & 1), kErrTimeoutReady)) break;
+      if (!waitw(&v_full[c & 1], (uint32_t)((c >> 1) & 1), kErrTimeoutFull)) break;
+      tc_fence_after();
+      const uint64_t v = vd + (c & 1) * kSlot;
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) umma_f16_w(tbase + 64, kstep(pd, kk), mnstep(v, kk), id_o, (c > 0 || kk > 0) ? 1u : 0u);
+      umma_commit_w(pv_done);
+      if (c > 0 && c + 1 < kt.n) load(sV, mv, &v_full[(c + 1) & 1], c + 1);       // (P V(c - 1) had read its V at p_full)
+    }
   } else if (rows > 0) {
     const int row = 32 * warp + lane, i = r0 + row, p = plo + row;
     const uint32_t tS = tbase + ((uint32_t)(32 * warp) << 16), tO = tS + 64;
-    auto load_kv = [&](int c) {      // (one thread)
-      uint8_t* st = sKV + (c & 1) * 2 * kTile;
-      mbar_arrive_expect_tx(&kv_full[c & 1], 2 * kTile);
-      load_tile(st, mk, &kv_full[c & 1], b, h / a.group, kt.tile(c) * 64);
-      load_tile(st + kTile, mv, &kv_full[c & 1], b, h / a.group, kt.tile(c) * 64);
-    };
-    if (threadIdx.x == 0 && kt.n > 0) {
-      mbar_arrive_expect_tx(q_full, 2 * kTile);
-      load_tile(sQ, mq, q_full, b, h, r0);
-      load_tile(sQ + kTile, mq, q_full, b, h, r0 + 64);
-      load_kv(0);
-      if (kt.n > 1) load_kv(1);
-    }
+    uint8_t* prow = sP + row * 128;
     // tiles that every row sees whole: sink tiles below fs, window tiles of [f0, f1)
     const int top = min(plo + a.right + 1, s.kn);
     const int fs = max(0, min(a.sinks, top)) >> 6, f0 = (max(0, phi - a.left) + 63) >> 6, f1 = max(f0, top >> 6);
@@ -230,59 +281,43 @@ __global__ void __launch_bounds__(kFwdThreads, 4)
       const int t = kt.tile(c);
       if (!waitw(s_full, (uint32_t)(c & 1), kErrTimeoutAccum)) { ok = false; break; }
       tc_fence_after();
-      if (threadIdx.x == 0 && c > 0 && c + 1 < kt.n) load_kv(c + 1);
-      uint32_t ml = 0xffffffffu, mh = 0xffffffffu;
-      const bool edge = !(t < fs || (t >= f0 && t < f1));
-      if (edge) {
+      uint32_t v[64];
+      tmem_ld32(tS, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
+      tmem_ld32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
+      tmem_ld_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(s_read);
+      if (!(t < fs || (t >= f0 && t < f1))) {
         const uint64_t mask = seen_mask(a, s, p, t * 64);
-        ml = (uint32_t)mask;
-        mh = (uint32_t)(mask >> 32);
-      }
-      // P = 2^(x - m) in one pass with the base m of the tiles before, while the row's maximum is
-      // taken; the base stays unless the maximum is more than 2^8 above it (P then stays below 2^8,
-      // and O is rescaled rarely).  Otherwise, as in the first tile, the pass is made again.
-      uint32_t pk[32];
-      float lt;
-      while (true) {
-        const float mb = m_used == -INFINITY ? 0.f : m_used;
-        const uint64_t nb2 = f2(-mb, -mb);
-        uint64_t ls[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        const uint32_t ml = (uint32_t)mask, mh = (uint32_t)(mask >> 32);
+        if (__any_sync(0xffffffffu, ml != 0xffffffffu)) {      // (32 rows' edge often lies in one half)
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          uint32_t v[32];
-          tmem_ld32(tS + 32 * q, v);
-          tmem_ld_wait();
-          if (edge) {
-            const uint32_t mm = q ? mh : ml;
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!((mm >> e) & 1u)) v[e] = 0xff800000u;
-          }
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            mx[e & 3] = max3(mx[e & 3], __uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
-            float x0, x1;
-            f2split(ffma2(f2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), sc2, nb2), x0, x1);
-            const float p0 = ex2(x0), p1 = ex2(x1);
-            ls[e & 1] = fadd2(ls[e & 1], f2(p0, p1));
-            pk[16 * q + e] = pack2<BF>(p0, p1);
-          }
+          for (int e = 0; e < 32; ++e)
+            if (!((ml >> e) & 1u)) v[e] = 0xff800000u;
         }
-        const float top_x = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.sl2;
-        float l0, l1, l2, l3;
-        f2split(ls[0], l0, l1);
-        f2split(ls[1], l2, l3);
-        lt = (l0 + l1) + (l2 + l3);
-        const bool grow = top_x > m_used + 8.f;
-        if (!__any_sync(0xffffffffu, grow)) break;
+        if (__any_sync(0xffffffffu, mh != 0xffffffffu)) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (!((mh >> e) & 1u)) v[32 + e] = 0xff800000u;
+        }
+      }
+      const float mx = rowmax64(v) * a.sl2;
+      // the exponent's base stays unless the row's maximum grew by more than 2^8: P then stays below
+      // 2^8, and O is rescaled rarely
+      const bool grow = mx > m_used + 8.f;
+      bool waited = c == 0;
+      if (__any_sync(0xffffffffu, grow)) {
         float alpha = 1.f;
         if (grow) {
-          alpha = m_used == -INFINITY ? 0.f : ex2(m_used - top_x);
-          m_used = top_x;
+          alpha = m_used == -INFINITY ? 0.f : ex2(m_used - mx);
+          m_used = mx;
         }
         l *= alpha;
         if (c > 0) {
+          if (!waitw(pv_done, (uint32_t)((c - 1) & 1), kErrTimeoutAccum)) { ok = false; break; }
+          waited = true;
+          tc_fence_after();
 #pragma unroll 1
           for (int q = 0; q < 4; ++q) {
             uint32_t o[16];
@@ -292,22 +327,40 @@ __global__ void __launch_bounds__(kFwdThreads, 4)
             for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
             tmem_st16(tO + 16 * q, o);
           }
+          tmem_st_wait();
         }
       }
-      l += lt;
-      tmem_st16(tS, *reinterpret_cast<uint32_t(*)[16]>(&pk[0]));
-      tmem_st16(tS + 16, *reinterpret_cast<uint32_t(*)[16]>(&pk[16]));
-      if (t * 64 + 64 > s.kn && s.kn < a.Sk) {   // values behind the sequence's end (its last tile)
-        if (!waitw(&kv_full[c & 1], (uint32_t)((c >> 1) & 1), kErrTimeoutFull)) { ok = false; break; }
-        zero_rows(sKV + (c & 1) * 2 * kTile + kTile, max(0, s.kn - t * 64), row, 128);
-        fence_proxy_async_smem();
+      const float mb = m_used == -INFINITY ? 0.f : m_used;
+      const uint64_t nb2 = f2(-mb, -mb);
+      uint64_t ls[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {
+        float x0, x1;
+        f2split(ffma2(f2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), sc2, nb2), x0, x1);
+        float p0, p1;
+        ex2_at(e, x0, x1, p0, p1);
+        ls[e & 1] = fadd2(ls[e & 1], f2(p0, p1));
+        v[e] = pack2<BF>(p0, p1);
       }
-      tmem_st_wait();
+      float l0, l1, l2, l3;
+      f2split(ls[0], l0, l1);
+      f2split(ls[1], l2, l3);
+      l += (l0 + l1) + (l2 + l3);
+      // P's buffer is free once the tile before's P V is done
+      if (!waited && !waitw(pv_done, (uint32_t)((c - 1) & 1), kErrTimeoutAccum)) { ok = false; break; }
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        *reinterpret_cast<uint4*>(prow + ((q ^ (row & 7)) << 4)) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+      if (t * 64 + 64 > s.kn && s.kn < a.Sk) {   // values behind the sequence's end (its last tile)
+        if (!waitw(&v_full[c & 1], (uint32_t)((c >> 1) & 1), kErrTimeoutFull)) { ok = false; break; }
+        zero_rows(sV + (c & 1) * kTile, max(0, s.kn - t * 64), row, 128);
+      }
+      fence_proxy_async_smem();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(p_full);
     }
-    const bool have = ok && kt.n > 0 && waitw(o_full, 0, kErrTimeoutAccum);
+    const bool have = ok && kt.n > 0 && waitw(pv_done, (uint32_t)((kt.n - 1) & 1), kErrTimeoutAccum);
     tc_fence_after();
     const bool empty = m_used == -INFINITY && l == l;   // no visible key (a NaN score stays a NaN)
     const float inv = 1.f / l;
