@@ -92,7 +92,7 @@ static int plan_tail(Ctx* c, const GemmDesc& d, GemmArgs& a, long tiles, long sl
   a.tail_t0 = (int)tiles;
   a.tail_parts = 1;
   a.tail_kbps = nkb;
-  if (a.splits != 1 || !d.out || d.out_h || d.out_h_t || tiles <= slots) return 0;
+  if (a.splits != 1 || !d.out || d.out_h || d.out_h_t || d.epi || tiles <= slots) return 0;
   const long rem = tiles % slots;
   if (rem == 0) return 0;
   int parts = (int)(slots / rem);
@@ -116,17 +116,37 @@ static int plan_tail(Ctx* c, const GemmDesc& d, GemmArgs& a, long tiles, long sl
   return 0;
 }
 
-template <int BN, int STAGES, int BMODE, bool A_MN>
+// The maps of z and the residual, like the output's own (tma_out says whether there is one).
+static int act_maps(const GemmDesc&, GemmArgs&, std::string&) { return 0; }
+static int act_maps(const GemmDesc& d, GemmActArgs& a, std::string& err) {
+  a.e = *d.epi;
+  if (!a.tma_out) return 0;
+  auto map = [&](CUtensorMap* m, const void* p, const char* what) {
+    return a.tma_out == 1
+               ? make_map(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, p, d.N, d.M, d.ldo * 4, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B, what, err)
+               : make_map(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, p, d.N, d.M, d.ldo_h * 2, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B, what, err);
+  };
+  return (a.e.z && map(&a.tm_z, a.e.z, "z")) || (a.e.residual && map(&a.tm_res, a.e.residual, "residual"));
+}
+// z and the residual allow the vector accesses of the TMA epilogue
+static bool act_aligned(const GemmDesc& d) {
+  return !d.epi || ((reinterpret_cast<uintptr_t>(d.epi->z) | reinterpret_cast<uintptr_t>(d.epi->residual)) & 15) == 0;
+}
+
+template <int BN, int STAGES, int BMODE, bool A_MN, class Args = GemmArgs>
 static int launch(Ctx* c, const GemmDesc& d, const CUtensorMap& ta, const CUtensorMap& tb,
                   const CUtensorMap& tbs, const CUtensorMap& tea, const CUtensorMap& teb,
                   const GemmArgs& args, std::string& err) {
   using L = GemmSmem<BN, STAGES, BMODE>;
   const auto SW = CU_TENSOR_MAP_SWIZZLE_128B;
   using R = GemmRoles<BMODE>;
-  auto kern = gemm_tc_kernel<BN, STAGES, BMODE, A_MN>;
-  if (smem_attr(reinterpret_cast<const void*>(kern), L::DYN, c->device, "gemm smem attribute", err)) return 1;
+  auto kern = gemm_tc_kernel<BN, STAGES, BMODE, A_MN, Args>;
+  constexpr int dyn = L::DYN + (kHasAct<Args> ? kActBarBytes : 0);
+  static_assert(dyn <= 232448, "shared memory budget (227 KB)");
+  if (smem_attr(reinterpret_cast<const void*>(kern), dyn, c->device, "gemm smem attribute", err)) return 1;
   const long tiles = (long)((d.M + kBM - 1) / kBM) * ((d.N + BN - 1) / BN);
-  GemmArgs a = args;
+  Args a{};
+  static_cast<GemmArgs&>(a) = args;
   // split-K when the output has too few tiles to fill the GPU and K is long
   const int nkb = (d.K + kBK - 1) / kBK;
   a.splits = 1;
@@ -166,7 +186,7 @@ static int launch(Ctx* c, const GemmDesc& d, const CUtensorMap& ta, const CUtens
   // epilogue through TMA stores when the output is a single row-major tensor
   CUtensorMap tout = ta;
   a.tma_out = 0;
-  if (a.splits == 1) {
+  if (a.splits == 1 && act_aligned(d)) {
     std::string e2;
     if (d.out && !d.out_h && !d.out_h_t && !d.out_trans && (d.ldo % 4) == 0 &&
         (reinterpret_cast<uintptr_t>(d.out) & 15) == 0 &&
@@ -177,24 +197,27 @@ static int launch(Ctx* c, const GemmDesc& d, const CUtensorMap& ta, const CUtens
              !make_map(&tout, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, d.out_h, d.N, d.M, d.ldo_h * 2, 64, 32, SW, "out_h", e2))
       a.tma_out = 2;
   }
+  if (act_maps(d, a, err)) return 1;
   const long items = a.tail_parts > 1 ? a.tail_t0 + (tiles - a.tail_t0) * a.tail_parts : tiles * a.splits;
   const unsigned grid = (unsigned)(items < (long)c->sm_count ? items : (long)c->sm_count);
   {
     ProfScope prof_(c, d.name);
-    launch_pdl(c, kern, grid, R::THREADS, L::DYN, ta, tb, tbs, tea, teb, tout, a);
+    launch_pdl(c, kern, grid, R::THREADS, dyn, ta, tb, tbs, tea, teb, tout, a);
     if (check_launch("gemm_tc", err)) return 1;
   }
   return 0;
 }
 
 // CTA-pair launch (cta_group::2, clusters of 2): f16 operands, no split-K.
-template <int BN, int STAGES, int BMODE>
+template <int BN, int STAGES, int BMODE, class Args = GemmArgs>
 static int launch_pair(Ctx* c, const GemmDesc& d, const CUtensorMap& ta, const CUtensorMap& tb,
                        const CUtensorMap& tea, const CUtensorMap& teb, const GemmArgs& args, std::string& err) {
   using L = Gemm2Smem<BN, STAGES>;
   const auto SW = CU_TENSOR_MAP_SWIZZLE_128B;
-  auto kern = gemm_tc2_kernel<BN, STAGES, BMODE>;
-  if (smem_attr(reinterpret_cast<const void*>(kern), L::DYN, c->device, "gemm pair smem attribute", err)) return 1;
+  auto kern = gemm_tc2_kernel<BN, STAGES, BMODE, Args>;
+  constexpr int dyn = L::DYN + (kHasAct<Args> ? kActBarBytes : 0);
+  static_assert(dyn <= 232448, "shared memory budget (227 KB)");
+  if (smem_attr(reinterpret_cast<const void*>(kern), dyn, c->device, "gemm pair smem attribute", err)) return 1;
   // (the cluster occupancy is a property of the kernel and the sm_100 part, the same on every device)
   static std::atomic<int> max_clusters{0};
   if (!max_clusters.load()) {
@@ -204,7 +227,7 @@ static int launch_pair(Ctx* c, const GemmDesc& d, const CUtensorMap& ta, const C
     at[0].val.clusterDim.x = 2; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
     q.gridDim = dim3(2 * (unsigned)(c->sm_count / 2));
     q.blockDim = dim3(kPairThreads);
-    q.dynamicSmemBytes = L::DYN;
+    q.dynamicSmemBytes = dyn;
     q.attrs = at;
     q.numAttrs = 1;
     int n = 0;
@@ -214,13 +237,14 @@ static int launch_pair(Ctx* c, const GemmDesc& d, const CUtensorMap& ta, const C
     }
     max_clusters.store(n);
   }
-  GemmArgs a = args;
+  Args a{};
+  static_cast<GemmArgs&>(a) = args;
   a.splits = 1;
   a.kb_per_split = (d.K + kBK - 1) / kBK;
   a.partial = nullptr;
   CUtensorMap tout = ta;
   a.tma_out = 0;
-  {
+  if (act_aligned(d)) {
     std::string e2;
     if (d.out && !d.out_h && !d.out_trans && (d.ldo % 4) == 0 && (reinterpret_cast<uintptr_t>(d.out) & 15) == 0 &&
         !make_map(&tout, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, d.out, d.N, d.M, d.ldo * 4, 32, 32, SW, "out", e2))
@@ -236,6 +260,7 @@ static int launch_pair(Ctx* c, const GemmDesc& d, const CUtensorMap& ta, const C
   }
   const long tiles = (long)((d.M + 2 * kBM - 1) / (2 * kBM)) * ((d.N + BN - 1) / BN);
   if (plan_tail(c, d, a, tiles, (long)max_clusters, (d.M + 2 * kBM - 1) / (2 * kBM), BN, err)) return 1;
+  if (act_maps(d, a, err)) return 1;
   const long items = a.tail_parts > 1 ? a.tail_t0 + (tiles - a.tail_t0) * a.tail_parts : tiles;
   const long clusters = items < (long)max_clusters ? items : (long)max_clusters;
   cudaLaunchConfig_t cfg = {};
@@ -246,7 +271,7 @@ static int launch_pair(Ctx* c, const GemmDesc& d, const CUtensorMap& ta, const C
   at[1].val.programmaticStreamSerializationAllowed = use_pdl(c) ? 1 : 0;
   cfg.gridDim = dim3((unsigned)(2 * clusters));
   cfg.blockDim = dim3(kPairThreads);
-  cfg.dynamicSmemBytes = L::DYN;
+  cfg.dynamicSmemBytes = dyn;
   cfg.stream = c->stream;
   cfg.attrs = at;
   cfg.numAttrs = 2;
@@ -355,6 +380,11 @@ int gemm(Ctx* c, const GemmDesc& d, std::string& err) {
   // and the context has not asked for the in-smem path explicitly
   const bool quant = weight_b && d.w && (d.w->type == kTypeQ8_0 || d.w->type == kTypeQ4_K) &&
                      !(d.w->f16 && !c->smem_dequant);
+  if (d.epi && (quant || d.bsrc != kB_WEIGHT_NT || d.a_mn || d.out_trans || d.out_h_trans || d.out_h_t || d.accumulate ||
+                (d.out != nullptr) == (d.out_h != nullptr) || (d.out ? d.ldo : d.ldo_h) != d.N)) {
+    err = "gemm: the activation epilogue needs an f16 weight operand and one dense row-major output";
+    return 1;
+  }
   if (d.hp && quant) { err = "gemm: the fused head preparation needs an f16 weight operand"; return 1; }
   if (quant && c->dequant_tmem && wq_fits(d)) {
     // (inside a stream capture the transposed codes of an input-gradient GEMM cannot be made: such
@@ -498,12 +528,20 @@ int gemm(Ctx* c, const GemmDesc& d, std::string& err) {
         if (make_map(&teb2, BF, d.ext_b, 64, d.N, 128, 64, bp / 2, SW, "ext B half", err)) return 1;
       }
       if (d.hp && bmode != 0) { err = "gemm: the fused head preparation needs a K-major B operand"; return 1; }
+      if (d.epi)
+        return bp == 192 ? launch_pair<192, 5, 0, GemmActArgs>(c, d, ta, tb2, tea2, teb2, a, err)
+                         : launch_pair<256, 5, 0, GemmActArgs>(c, d, ta, tb2, tea2, teb2, a, err);
       if (bp == 192) return launch_pair<192, 6, 0>(c, d, ta, tb2, tea2, teb2, a, err);
       return bmode == 0 ? launch_pair<256, 6, 0>(c, d, ta, tb2, tea2, teb2, a, err)
                         : launch_pair<256, 6, 1>(c, d, ta, tb2, tea2, teb2, a, err);
     }
   }
   if (d.hp) { err = "gemm: the fused head preparation runs on the CTA-pair kernel only"; return 1; }
+  if (d.epi) {
+    if (bn == 256) return launch<256, 4, 0, false, GemmActArgs>(c, d, ta, tb, tbs, tea, teb, a, err);
+    if (bn == 192) return launch<192, 4, 0, false, GemmActArgs>(c, d, ta, tb, tbs, tea, teb, a, err);
+    return launch<128, 6, 0, false, GemmActArgs>(c, d, ta, tb, tbs, tea, teb, a, err);
+  }
   if (bn == 256) {
     switch (bmode) {
       case 0: return launch<256, 4, 0, false>(c, d, ta, tb, tbs, tea, teb, a, err);

@@ -29,6 +29,9 @@
 // values are bit-identical to ggml's to_float (then rounded once to f16 for the tensor core).
 #pragma once
 
+#include <type_traits>
+
+#include "activation.cuh"
 #include "sa3k_common.cuh"
 #include "sa3k_internal.h"
 
@@ -67,6 +70,107 @@ struct GemmArgs {
 };
 
 constexpr int kBM = 128, kBK = 64;
+
+// Arguments of the kernels with an activation epilogue (ActEpi): a template argument of its own, so
+// that the kernels without one stay as they are.
+struct GemmActArgs : GemmArgs {
+  ActEpi e;
+  CUtensorMap tm_z;         // TMA store of z (tma_out != 0 and e.z)
+  CUtensorMap tm_res;       // TMA load of the residual (tma_out != 0 and e.residual)
+};
+constexpr int kActBarBytes = 128;   // residual barriers: 8 epilogue warps x 2, behind the kernel's own shared memory
+template <class Args>
+constexpr bool kHasAct = std::is_same<Args, GemmActArgs>::value;
+
+// One value of the direct and split-K paths: z kept, activation and residual applied.
+template <class Args>
+__device__ __forceinline__ float act_element(const Args& args, float v, long row, int col) {
+  if constexpr (kHasAct<Args>) {
+    const long i = row * args.N + col;
+    const bool h = args.out_h != nullptr;
+    if (args.e.z) {
+      if (h) static_cast<__half*>(args.e.z)[i] = __float2half_rn(v);
+      else static_cast<float*>(args.e.z)[i] = v;
+    }
+    v = act_value(args.e.act, v);
+    if (args.e.residual)
+      v += h ? __half2float(static_cast<const __half*>(args.e.residual)[i]) : static_cast<const float*>(args.e.residual)[i];
+  }
+  return v;
+}
+
+// The residual's chunks (32 rows x 128 bytes, like the output's) of one epilogue warp: TMA brings a
+// chunk into the staging buffer that its output will leave from (direct loads, 16 bytes of 32 rows at
+// a time, thrashed the few KB of L1 that are left and cost 30 us on a 4352 x 6144 x 1536 product).
+// With two buffers a chunk is fetched while the one before it is worked on.
+template <int BUFS>
+struct ResidualPipe {
+  uint8_t* stg;
+  uint64_t* bar;       // [BUFS]
+  int issued = 0, taken = 0;
+  __device__ __forceinline__ uint8_t* buf(int i) const { return stg + (BUFS == 2 ? (i & 1) : 0) * 4096; }
+  __device__ __forceinline__ void issue(const GemmActArgs& args, int lane, int nb, int rbase) {
+    if (lane == 0) {
+      // the stores from this buffer have read it (of two, the last one is the other's)
+      if (BUFS == 2) bulk_wait_read<1>();
+      else bulk_wait_read<0>();
+      uint64_t* b = bar + (BUFS == 2 ? (issued & 1) : 0);
+      mbar_arrive_expect_tx(b, 4096);
+      tma_load_2d(buf(issued), &args.tm_res, b, nb, rbase);
+    }
+    __syncwarp();
+    ++issued;
+  }
+  // the lane's row of the chunk that was issued first; false on a timeout
+  __device__ __forceinline__ bool take(uint4 (&v)[8], int lane, int* err) {
+    const uint32_t use = (uint32_t)(BUFS == 2 ? taken >> 1 : taken);
+    const bool ok = mbar_wait(bar + (BUFS == 2 ? (taken & 1) : 0), use & 1u, err, kErrTimeoutOther);
+    const uint8_t* p = buf(taken);
+    ++taken;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) v[c] = *reinterpret_cast<const uint4*>(p + lane * 128 + ((c ^ (lane & 7)) << 4));
+    __syncwarp();
+    return ok;
+  }
+};
+
+struct ResidualChunk {
+  uint4 v[8];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int c = 0; c < 8; ++c) v[c] = make_uint4(0u, 0u, 0u, 0u);
+  }
+  __device__ __forceinline__ float half_at(int j) const {
+    const uint32_t w[4] = {v[j >> 3].x, v[j >> 3].y, v[j >> 3].z, v[j >> 3].w};
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[(j & 7) >> 1]));
+    return (j & 1) ? f.y : f.x;
+  }
+  __device__ __forceinline__ float float_at(int j) const {
+    const uint32_t w[4] = {v[j >> 2].x, v[j >> 2].y, v[j >> 2].z, v[j >> 2].w};
+    return __uint_as_float(w[j & 3]);
+  }
+};
+
+// act(f) + residual over a chunk; one activation per code path, so that the loop holds no branch
+template <int ACT>
+__device__ __forceinline__ void act_chunk_as(const GemmActArgs& args, float (&f)[64], const ResidualChunk& r) {
+  if (args.out_h) {
+#pragma unroll
+    for (int j = 0; j < 64; ++j) f[j] = act_value(ACT, f[j]) + r.half_at(j);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) f[j] = act_value(ACT, f[j]) + r.float_at(j);
+  }
+}
+__device__ __forceinline__ void act_chunk(const GemmActArgs& args, float (&f)[64], const ResidualChunk& r) {
+  switch (args.e.act) {
+    case kActSilu: act_chunk_as<kActSilu>(args, f, r); break;
+    case kActGelu: act_chunk_as<kActGelu>(args, f, r); break;
+    case kActGeluTanh: act_chunk_as<kActGeluTanh>(args, f, r); break;
+    default: act_chunk_as<kActNone>(args, f, r);
+  }
+}
+
 
 // A work item of the persistent GEMM kernels: tile t and its K range [kb0, kb0 + nkb) of 64-wide
 // k-blocks; total adds the K = 16 extension stage to the last range.  Items [0, tail_t0) are
@@ -290,7 +394,8 @@ __device__ __forceinline__ void epi_columns(const uint32_t (&v)[32], float* f, i
 // (__ldcg: other CTAs wrote them).  Four columns per thread when N % 4 == 0 (n0 is a multiple of
 // the N tile); the mapping is column-fastest for row-major outputs (coalesced partial reads and
 // output writes) and row-fastest when an output is transposed.
-__device__ __forceinline__ void splitk_finish(const GemmArgs& args, int m0, int n0, int rows, int cols, int tid,
+template <class Args>
+__device__ __forceinline__ void splitk_finish(const Args& args, int m0, int n0, int rows, int cols, int tid,
                                               int nt) {
   const long mn = (long)args.M * args.N;
   const bool trans = args.out_trans || args.out_h_trans || args.out_h_t;
@@ -318,6 +423,7 @@ __device__ __forceinline__ void splitk_finish(const GemmArgs& args, int m0, int 
       float v = x[u] * args.alpha;
       if (args.col_scale) v *= args.col_scale[col];
       if (args.col_bias) v += args.col_bias[col];
+      v = act_element(args, v, row, col);
       if (args.out) {
         float* dst = args.out_trans ? args.out + (long)col * args.ldo + row : args.out + (long)row * args.ldo + col;
         *dst = args.accumulate ? *dst + v : v;
@@ -377,12 +483,12 @@ __device__ __forceinline__ void splitk_finish_rows16(const GemmArgs& args, int m
 // columns) and, with split-K, one K-range of it.
 // The accumulator is double-buffered in TMEM: the epilogue drains tile i while the MMA warp
 // accumulates tile i + 1.
-template <int BN, int STAGES, int BMODE, bool A_MN>
+template <int BN, int STAGES, int BMODE, bool A_MN, class Args>
 __global__ void __launch_bounds__(GemmRoles<BMODE>::THREADS, 1)
     gemm_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                    const __grid_constant__ CUtensorMap tm_bs, const __grid_constant__ CUtensorMap tm_ea,
                    const __grid_constant__ CUtensorMap tm_eb, const __grid_constant__ CUtensorMap tm_out,
-                   const __grid_constant__ GemmArgs args) {
+                   const __grid_constant__ Args args) {
   using T = BModeTraits<BMODE>;
   using L = GemmSmem<BN, STAGES, BMODE>;
   using R = GemmRoles<BMODE>;
@@ -417,6 +523,10 @@ __global__ void __launch_bounds__(GemmRoles<BMODE>::THREADS, 1)
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tfull[a], 1);
       mbar_init(&tempty[a], 32 * R::EPI_WARPS);
+    }
+    if constexpr (kHasAct<Args>) {
+      uint64_t* rb = reinterpret_cast<uint64_t*>(smem + L::TOTAL);
+      for (int w = 0; w < 16; ++w) mbar_init(&rb[w], 1);
     }
     *abort_flag = 0;
     fence_barrier_init();
@@ -570,6 +680,30 @@ __global__ void __launch_bounds__(GemmRoles<BMODE>::THREADS, 1)
     volatile int* last_split = reinterpret_cast<volatile int*>(tmem_slot + 2);
     int nstore = 0;
     int ti = 0;
+    // the residual's next chunk for this warp at or after column step c of work item `it`
+    ResidualPipe<L::STAGE_BUFS> rp{stg, reinterpret_cast<uint64_t*>(smem + L::TOTAL) + 2 * (warp - 2)};
+    int r_item = (int)blockIdx.x, r_c = half * cstep;
+    auto residual_next = [&]() {
+      if constexpr (kHasAct<Args>) {
+        while (r_item < nitems) {
+          const int rt = decode_item(args, r_item, ntiles, nkb_all).t;
+          const int rn = (rt / tiles_m) * BN + r_c, rr = (rt % tiles_m) * kBM + 32 * q;
+          const bool in = r_c < BN && rn < args.N;
+          r_c += NH * cstep;
+          if (!in || r_c >= BN) {
+            r_c = half * cstep;
+            r_item += (int)gridDim.x;
+          }
+          if (in) {
+            rp.issue(args, lane, rn, rr);
+            return;
+          }
+        }
+      }
+    };
+    bool use_res = false;
+    if constexpr (kHasAct<Args>) use_res = args.tma_out && args.e.residual;
+    if (use_res && L::STAGE_BUFS == 2) residual_next();
     for (int item = blockIdx.x; item < nitems; item += gridDim.x, ++ti) {
       const WorkItem w = decode_item(args, item, ntiles, nkb_all);
       const int t = w.t;
@@ -587,6 +721,7 @@ __global__ void __launch_bounds__(GemmRoles<BMODE>::THREADS, 1)
       for (int c0 = half * cstep; c0 < BN; c0 += NH * cstep) {
         float f[64];
         const int nb = n0 + c0;
+        if (use_res && L::STAGE_BUFS == 1 && nb < args.N) residual_next();
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           if (h == 1 && cstep == 32) break;
@@ -600,42 +735,75 @@ __global__ void __launch_bounds__(GemmRoles<BMODE>::THREADS, 1)
           tmem_ld_wait();
           epi_columns(v, f + 32 * h, nb + 32 * h, args, split_out, bias);
         }
-        if (!have || nb >= args.N) continue;
+        if (!have || nb >= args.N) {
+          if (use_res && nb < args.N) {      // (a wait ran out: the copy in flight still lands)
+            uint4 drop[8];
+            rp.take(drop, lane, args.err);
+            if (L::STAGE_BUFS == 2) residual_next();
+          }
+          continue;
+        }
         if (args.tma_out) {
           // ---- TMA store path: swizzled staging (16-byte chunk c of row r at c ^ (r & 7))
-          uint8_t* buf = stg + (L::STAGE_BUFS == 2 ? (nstore & 1) : 0) * L::STAGE_BYTES;
-          if (nstore >= L::STAGE_BUFS) {
-            // the store that last used this buffer must have read it
-            if (lane == 0) {
-              if (L::STAGE_BUFS == 2) bulk_wait_read<1>();
-              else bulk_wait_read<0>();
+          // the chunk through staging buffer b (16-byte chunk c of row r at c ^ (r & 7)) and out
+          auto put = [&](uint8_t* b, const CUtensorMap& map) {
+            if (args.tma_out == 1) {
+#pragma unroll
+              for (int c = 0; c < 8; ++c)
+                *reinterpret_cast<float4*>(b + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+                    make_float4(f[4 * c], f[4 * c + 1], f[4 * c + 2], f[4 * c + 3]);
+            } else {
+#pragma unroll
+              for (int c = 0; c < 8; ++c) {
+                uint4 o;
+                o.x = pack_f16x2(f[8 * c], f[8 * c + 1]);
+                o.y = pack_f16x2(f[8 * c + 2], f[8 * c + 3]);
+                o.z = pack_f16x2(f[8 * c + 4], f[8 * c + 5]);
+                o.w = pack_f16x2(f[8 * c + 6], f[8 * c + 7]);
+                *reinterpret_cast<uint4*>(b + lane * 128 + ((c ^ (lane & 7)) << 4)) = o;
+              }
             }
+            fence_proxy_async_smem();
             __syncwarp();
-          }
-          if (args.tma_out == 1) {
-#pragma unroll
-            for (int c = 0; c < 8; ++c)
-              *reinterpret_cast<float4*>(buf + lane * 128 + ((c ^ (lane & 7)) << 4)) =
-                  make_float4(f[4 * c], f[4 * c + 1], f[4 * c + 2], f[4 * c + 3]);
-          } else {
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              uint4 o;
-              o.x = pack_f16x2(f[8 * c], f[8 * c + 1]);
-              o.y = pack_f16x2(f[8 * c + 2], f[8 * c + 3]);
-              o.z = pack_f16x2(f[8 * c + 4], f[8 * c + 5]);
-              o.w = pack_f16x2(f[8 * c + 6], f[8 * c + 7]);
-              *reinterpret_cast<uint4*>(buf + lane * 128 + ((c ^ (lane & 7)) << 4)) = o;
+            if (lane == 0) {
+              if (args.accumulate || w.add) tma_reduce_add_2d(&map, b, nb, rbase);
+              else tma_store_2d(&map, b, nb, rbase);
+              bulk_commit();
             }
+          };
+          auto stage_out = [&](const CUtensorMap& map) {
+            uint8_t* b = stg + (L::STAGE_BUFS == 2 ? (nstore & 1) : 0) * L::STAGE_BYTES;
+            if (nstore >= L::STAGE_BUFS) {
+              // the store that last used this buffer must have read it
+              if (lane == 0) {
+                if (L::STAGE_BUFS == 2) bulk_wait_read<1>();
+                else bulk_wait_read<0>();
+              }
+              __syncwarp();
+            }
+            put(b, map);
+            ++nstore;
+          };
+          if constexpr (kHasAct<Args>) {
+            ResidualChunk res;
+            if (use_res) {       // z and the output leave from the buffer that the residual came into
+              uint8_t* b = rp.buf(rp.taken);
+              rp.take(res.v, lane, args.err);
+              if (args.e.z) {
+                put(b, args.tm_z);
+                if (lane == 0) bulk_wait_read<0>();
+                __syncwarp();
+              }
+              act_chunk(args, f, res);
+              put(b, tm_out);
+              if (L::STAGE_BUFS == 2) residual_next();
+              continue;
+            }
+            res.clear();
+            if (args.e.z) stage_out(args.tm_z);
+            act_chunk(args, f, res);
           }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            if (args.accumulate || w.add) tma_reduce_add_2d(&tm_out, buf, nb, rbase);
-            else tma_store_2d(&tm_out, buf, nb, rbase);
-            bulk_commit();
-          }
-          ++nstore;
+          stage_out(tm_out);
           continue;
         }
         // ---- direct path
@@ -674,11 +842,12 @@ __global__ void __launch_bounds__(GemmRoles<BMODE>::THREADS, 1)
           for (int r = 0; r < 32; ++r) {
             const int row = rbase + r;
             if (row >= args.M || lane >= ncols) continue;
-            const float x = st32[r * 32 + (lane ^ r)];
+            float x = st32[r * 32 + (lane ^ r)];
             if (split_out) {
               pbase[(long)row * args.N + nb + lane] = x;
               continue;
             }
+            x = act_element(args, x, row, nb + lane);
             if (args.out && !args.out_trans) {
               float* dst = args.out + (long)row * args.ldo + nb + lane;
               if (add) atomicAdd(dst, x);

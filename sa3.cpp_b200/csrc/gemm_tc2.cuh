@@ -163,11 +163,11 @@ struct Gemm2Smem {
 };
 
 // BMODE 0: B is [N][K] row-major (K-major); 1: B is [K][N] row-major (MN-major).  A is [M][K].
-template <int BN, int STAGES, int BMODE>
+template <int BN, int STAGES, int BMODE, class Args>
 __global__ void __launch_bounds__(kPairThreads, 1)
     gemm_tc2_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                     const __grid_constant__ CUtensorMap tm_ea, const __grid_constant__ CUtensorMap tm_eb,
-                    const __grid_constant__ CUtensorMap tm_out, const __grid_constant__ GemmArgs args) {
+                    const __grid_constant__ CUtensorMap tm_out, const __grid_constant__ Args args) {
   using L = Gemm2Smem<BN, STAGES>;
   constexpr bool BMN = BMODE == 1;
   constexpr int EPI_WARPS = kPairEpiWarps;
@@ -203,6 +203,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tfull[a], 1);
       mbar_init(&tempty[a], 2 * EPI_WARPS);
+    }
+    if constexpr (kHasAct<Args>) {
+      uint64_t* rb = reinterpret_cast<uint64_t*>(smem + L::TOTAL);
+      for (int w = 0; w < 16; ++w) mbar_init(&rb[w], 1);
     }
     *abort_flag = 0;
     fence_barrier_init();
@@ -327,6 +331,30 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     const int cstep = args.tma_out == 2 ? 64 : 32;
     const uint32_t tempty0 = mapa_shared(smem_u32(tempty), 0);
     int nstore = 0, ti = 0;
+    // the residual's next chunk for this warp at or after column step c of work item `it`
+    ResidualPipe<L::STAGE_BUFS> rp{stg, reinterpret_cast<uint64_t*>(smem + L::TOTAL) + 2 * (warp - 2)};
+    int r_item = (int)cluster, r_c = half * cstep;
+    auto residual_next = [&]() {
+      if constexpr (kHasAct<Args>) {
+        while (r_item < nitems) {
+          const int rt = decode_item(args, r_item, ntiles, nkb_all).t;
+          const int rn = (rt / tiles_m) * BN + r_c, rr = (rt % tiles_m) * PM + (int)rank * kBM + 32 * q;
+          const bool in = r_c < BN && rn < args.N;
+          r_c += NH * cstep;
+          if (!in || r_c >= BN) {
+            r_c = half * cstep;
+            r_item += (int)nclusters;
+          }
+          if (in) {
+            rp.issue(args, lane, rn, rr);
+            return;
+          }
+        }
+      }
+    };
+    bool use_res = false;
+    if constexpr (kHasAct<Args>) use_res = args.tma_out && args.e.residual;
+    if (use_res && L::STAGE_BUFS == 2) residual_next();
     for (int item = cluster; item < nitems; item += nclusters, ++ti) {
       const WorkItem w = decode_item(args, item, ntiles, nkb_all);
       const int t = w.t;
@@ -342,6 +370,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       for (int c0 = half * cstep; c0 < BN; c0 += NH * cstep) {
         float f[64];
         const int nb = n0 + c0;
+        if (use_res && L::STAGE_BUFS == 1 && nb < args.N) residual_next();
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           if (h == 1 && cstep == 32) break;
@@ -350,41 +379,75 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           tmem_ld_wait();
           epi_columns(v, f + 32 * h, nb + 32 * h, args, false, bias);
         }
-        if (!have || nb >= args.N) continue;
+        if (!have || nb >= args.N) {
+          if (use_res && nb < args.N) {      // (a wait ran out: the copy in flight still lands)
+            uint4 drop[8];
+            rp.take(drop, lane, args.err);
+            if (L::STAGE_BUFS == 2) residual_next();
+          }
+          continue;
+        }
         if (args.has_hp && rbase + lane < args.M) head_prep_epi(args.hp, f, nb, rbase + lane);   // (cstep is 64)
         if (args.tma_out) {
-          uint8_t* buf = stg + (L::STAGE_BUFS == 2 ? (nstore & 1) : 0) * L::STAGE_BYTES;
-          if (nstore >= L::STAGE_BUFS) {
-            if (lane == 0) {
-              if (L::STAGE_BUFS == 2) bulk_wait_read<1>();
-              else bulk_wait_read<0>();
+          // the chunk through staging buffer b (16-byte chunk c of row r at c ^ (r & 7)) and out
+          auto put = [&](uint8_t* b, const CUtensorMap& map) {
+            if (args.tma_out == 1) {
+#pragma unroll
+              for (int c = 0; c < 8; ++c)
+                *reinterpret_cast<float4*>(b + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+                    make_float4(f[4 * c], f[4 * c + 1], f[4 * c + 2], f[4 * c + 3]);
+            } else {
+#pragma unroll
+              for (int c = 0; c < 8; ++c) {
+                uint4 o;
+                o.x = pack_f16x2(f[8 * c], f[8 * c + 1]);
+                o.y = pack_f16x2(f[8 * c + 2], f[8 * c + 3]);
+                o.z = pack_f16x2(f[8 * c + 4], f[8 * c + 5]);
+                o.w = pack_f16x2(f[8 * c + 6], f[8 * c + 7]);
+                *reinterpret_cast<uint4*>(b + lane * 128 + ((c ^ (lane & 7)) << 4)) = o;
+              }
             }
+            fence_proxy_async_smem();
             __syncwarp();
-          }
-          if (args.tma_out == 1) {
-#pragma unroll
-            for (int c = 0; c < 8; ++c)
-              *reinterpret_cast<float4*>(buf + lane * 128 + ((c ^ (lane & 7)) << 4)) =
-                  make_float4(f[4 * c], f[4 * c + 1], f[4 * c + 2], f[4 * c + 3]);
-          } else {
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              uint4 o;
-              o.x = pack_f16x2(f[8 * c], f[8 * c + 1]);
-              o.y = pack_f16x2(f[8 * c + 2], f[8 * c + 3]);
-              o.z = pack_f16x2(f[8 * c + 4], f[8 * c + 5]);
-              o.w = pack_f16x2(f[8 * c + 6], f[8 * c + 7]);
-              *reinterpret_cast<uint4*>(buf + lane * 128 + ((c ^ (lane & 7)) << 4)) = o;
+            if (lane == 0) {
+              if (args.accumulate || w.add) tma_reduce_add_2d(&map, b, nb, rbase);
+              else tma_store_2d(&map, b, nb, rbase);
+              bulk_commit();
             }
+          };
+          auto stage_out = [&](const CUtensorMap& map) {
+            uint8_t* b = stg + (L::STAGE_BUFS == 2 ? (nstore & 1) : 0) * L::STAGE_BYTES;
+            if (nstore >= L::STAGE_BUFS) {
+              // the store that last used this buffer must have read it
+              if (lane == 0) {
+                if (L::STAGE_BUFS == 2) bulk_wait_read<1>();
+                else bulk_wait_read<0>();
+              }
+              __syncwarp();
+            }
+            put(b, map);
+            ++nstore;
+          };
+          if constexpr (kHasAct<Args>) {
+            ResidualChunk res;
+            if (use_res) {       // z and the output leave from the buffer that the residual came into
+              uint8_t* b = rp.buf(rp.taken);
+              rp.take(res.v, lane, args.err);
+              if (args.e.z) {
+                put(b, args.tm_z);
+                if (lane == 0) bulk_wait_read<0>();
+                __syncwarp();
+              }
+              act_chunk(args, f, res);
+              put(b, tm_out);
+              if (L::STAGE_BUFS == 2) residual_next();
+              continue;
+            }
+            res.clear();
+            if (args.e.z) stage_out(args.tm_z);
+            act_chunk(args, f, res);
           }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            if (args.accumulate || w.add) tma_reduce_add_2d(&tm_out, buf, nb, rbase);
-            else tma_store_2d(&tm_out, buf, nb, rbase);
-            bulk_commit();
-          }
-          ++nstore;
+          stage_out(tm_out);
           continue;
         }
         // direct path (row-major f32 and / or f16, or transposed outputs)
@@ -418,7 +481,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           for (int r = 0; r < 32; ++r) {
             const int row = rbase + r;
             if (row >= args.M || lane >= ncols) continue;
-            const float x = st32[r * 32 + (lane ^ r)];
+            const float x = act_element(args, st32[r * 32 + (lane ^ r)], row, nb + lane);
             if (args.out && !args.out_trans) {
               float* dst = args.out + (long)row * args.ldo + nb + lane;
               if (w.add) atomicAdd(dst, x);

@@ -93,6 +93,7 @@ int linear_forward(Ctx* c, const LinearFwd& f, std::string& err) {
   g.out = f.y; g.ldo = w->out;
   g.out_h = f.y_h; g.ldo_h = w->out;
   g.hp = f.hp;
+  g.epi = f.epi;
   g.name = "linear.fwd";
   return gemm(c, g, err);
 }

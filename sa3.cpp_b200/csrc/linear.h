@@ -47,11 +47,18 @@ struct LinearFwd {
   __half* ut = nullptr;
   int64_t ut_ld = 0;
   const HeadPrepEpi* hp = nullptr;     // fused head preparation of a qkv projection (see gemm())
+  const ActEpi* epi = nullptr;         // activation and residual (see gemm())
 };
 int linear_forward(Ctx* c, const LinearFwd& f, std::string& err);
 // u = x A^T of an adapter, written as ut = f16(u)^T [16][ut_ld]
 int lora_u(Ctx* c, const __half* x_h, int64_t M, int64_t in, const AdapterPrep& ad, __half* ut,
            int64_t ut_ld, std::string& err);
+
+// y = act(x W^T + bias) + residual for a few rows, read straight from the weight's stored form
+// (linear_rows.cu); x, residual, z, y of `type` (F16 or F32), S rows for which linear_rows_applies
+bool linear_rows_applies(int64_t S);
+int linear_rows(Ctx* c, const Weight* w, const float* bias, int act, int type, const void* x, int64_t S,
+                const void* residual, void* z, void* y, std::string& err);
 
 struct LinearBwd {
   const Weight* w = nullptr;

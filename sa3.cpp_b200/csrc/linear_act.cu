@@ -26,28 +26,67 @@ __global__ void __launch_bounds__(256) act_residual_kernel(const float* zf, long
   }
 }
 
-// dz = f16(g dy act'(z)); partial column sums of dy act'(z) and of dy act'(z) (z - bias) / g over
-// the block's rows: part[blockIdx.y][2][out].  Column per thread, kActRows rows per block.
-constexpr int kActRows = 32;
-template <class T>
-__global__ void __launch_bounds__(128) act_bwd_kernel(const T* dy, const T* z, const float* bias, const float* g, int act,
-                                                      long S, long out, __half* dz, long dz_ld, float* part) {
+// dz = f16(g dy act'(z)), and with part the partial column sums over the block's kActRows rows:
+// part[blockIdx.y][0] of dy act'(z) (the bias gradient), [1] of dy act'(z) (z - bias) / g (dora's dg).
+// One pass: dy and z are read and dz is written once, in 16-byte accesses of 8 columns a thread (VEC)
+// or one column a thread (widths and bases that allow none).  Bound by memory: 2047 x 6144 f16 moves
+// 75 MB.
+constexpr int kActRows = 16;
+template <class T, int ACT, bool VEC, bool DORA>
+__global__ void __launch_bounds__(128) act_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ z, const float* __restrict__ bias,
+                                                      const float* __restrict__ g, long S,
+                                                      long out, __half* __restrict__ dz, long dz_ld, float* __restrict__ part) {
   pdl_prologue();
-  const long o = (long)blockIdx.x * 128 + threadIdx.x;
+  constexpr int W = VEC ? 8 : 1;
+  const long o = ((long)blockIdx.x * 128 + threadIdx.x) * W;
   if (o >= out) return;
   const long t0 = (long)blockIdx.y * kActRows, t1 = min(S, t0 + kActRows);
-  const float go = g ? g[o] : 1.f, bo = bias ? bias[o] : 0.f, inv = 1.f / go;
-  float sb = 0.f, sg = 0.f;
-  for (long t = t0; t < t1; ++t) {
-    const float zv = z ? to_f32(z[t * out + o]) : 0.f;
-    const float d = to_f32(dy[t * out + o]) * act_slope(act, zv);
-    dz[t * dz_ld + o] = __float2half_rn(d * go);
-    sb += d;
-    sg = fmaf(d, (zv - bo) * inv, sg);
+  float go[W], bo[W], inv[W], sb[W], sg[W];
+#pragma unroll
+  for (int e = 0; e < W; ++e) {
+    if (DORA) {
+      go[e] = g[o + e];
+      bo[e] = bias ? bias[o + e] : 0.f;
+      inv[e] = 1.f / go[e];
+    }
+    sb[e] = sg[e] = 0.f;
   }
-  if (part) {
-    part[(long)blockIdx.y * 2 * out + o] = sb;
-    part[(long)blockIdx.y * 2 * out + out + o] = sg;
+  constexpr int U = 2;        // rows whose loads are in flight together
+  for (long t = t0; t < t1; t += U) {
+    float d[U][8], v[U][8];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (t + u >= t1) continue;
+      if constexpr (VEC) {
+        load8(dy + (t + u) * out + o, d[u]);
+        if (z) load8(z + (t + u) * out + o, v[u]);
+      } else {
+        d[u][0] = to_f32(dy[(t + u) * out + o]);
+        if (z) v[u][0] = to_f32(z[(t + u) * out + o]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (t + u >= t1) continue;
+      float q[8];
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        if (!z) v[u][e] = 0.f;
+        const float x = d[u][e] * act_slope(ACT, v[u][e]);
+        q[e] = DORA ? x * go[e] : x;
+        sb[e] += x;
+        if (DORA) sg[e] = fmaf(x, (v[u][e] - bo[e]) * inv[e], sg[e]);
+      }
+      if constexpr (VEC) store8(dz + (t + u) * dz_ld + o, q);
+      else dz[(t + u) * dz_ld + o] = __float2half_rn(q[0]);
+    }
+  }
+  if (!part) return;
+  float* p = part + (long)blockIdx.y * 2 * out + o;
+#pragma unroll
+  for (int e = 0; e < W; ++e) {
+    p[e] = sb[e];
+    if (DORA) p[out + e] = sg[e];
   }
 }
 
@@ -59,7 +98,7 @@ int check_args(const Ctx* c, const Weight* w, const sa3k_adapter* ad, int act, i
   if (w->device != c->device) { err = "linear_act: the weight is on another device than the context"; return 1; }
   if (act < kActNone || act > kActGeluTanh) { err = "linear_act: unknown activation"; return 1; }
   if (type != kTypeF32 && type != kTypeF16) { err = "linear_act: the type must be F32 or F16"; return 1; }
-  if (S < 0 || S > (1 << 30)) { err = "linear_act: S must be from 0 to 2^30"; return 1; }
+  if (S < 0 || S > (1 << 20) - 16) { err = "linear_act: S must be from 0 to 2^20 - 16"; return 1; }
   if (S > 0 && (!x || !aligned16(x))) { err = "linear_act: x must be given and start on 16 bytes"; return 1; }
   if (ad && (ad->rank < 1 || ad->rank > 16 || !ad->A || !ad->B)) { err = "adapter rank must be 1..16 with A and B"; return 1; }
   if (ad && ad->magnitude && !ad->base_norm_sq) { err = "dora adapter needs base_norm_sq"; return 1; }
@@ -102,28 +141,57 @@ int act_residual(Ctx* c, const float* zf, int64_t n, int act, const void* residu
 
 int linear_act_forward(Ctx* c, const Weight* w, const sa3k_adapter* ad, const float* bias, int act, int type,
                        const void* x, int64_t S, const void* residual, void* z, void* y, std::string& err) {
+  if (!ad && linear_rows_applies(S)) return linear_rows(c, w, bias, act, type, x, S, residual, z, y, err);
   const __half* x_h;
   if (operand(c, type, x, S * w->in, x_h, err)) return 1;
   AdapterPrep prep;
   __half* ut = nullptr;
   if (ad && prepare_adapter(c, w, ad, x_h, S, prep, ut, err)) return 1;
-  float* zf = static_cast<float*>(scratch_get(c, kSlotActZ, (size_t)(S * w->out) * sizeof(float), err));
-  if (!zf) return 1;
   LinearFwd f;
   f.w = w; f.ad = ad ? &prep : nullptr; f.bias = bias; f.x_h = x_h; f.M = S;
-  f.y = zf; f.ut = ut; f.ut_ld = pad64(S);
+  f.ut = ut; f.ut_ld = pad64(S);
+  const bool half_copy = w->f16 && !(c->smem_dequant && (w->type == kTypeQ8_0 || w->type == kTypeQ4_K));
+  if (half_copy) {     // activation and residual in the GEMM's epilogue
+    ActEpi e;
+    e.act = act; e.residual = residual; e.z = z;
+    f.epi = &e;
+    if (type == kTypeF16) f.y_h = static_cast<__half*>(y);
+    else f.y = static_cast<float*>(y);
+    return linear_forward(c, f, err);
+  }
+  // a base that is dequantized inside the GEMM: the f32 product, then one pass
+  float* zf = static_cast<float*>(scratch_get(c, kSlotActZ, (size_t)(S * w->out) * sizeof(float), err));
+  if (!zf) return 1;
+  f.y = zf;
   if (linear_forward(c, f, err)) return 1;
   return type == kTypeF16 ? act_residual<__half>(c, zf, S * w->out, act, residual, z, y, err)
                           : act_residual<float>(c, zf, S * w->out, act, residual, z, y, err);
 }
 
-template <class T>
-int act_bwd(Ctx* c, const void* dy, const void* z, const float* bias, const float* g, int act, int64_t S, int64_t out,
-            __half* dz, int64_t dz_ld, float* part, std::string& err) {
+template <class T, int ACT>
+int act_bwd_as(Ctx* c, const T* dy, const T* z, const float* bias, const float* g, int64_t S, int64_t out, __half* dz,
+               int64_t dz_ld, float* part, std::string& err) {
+  const bool vec = out % 8 == 0 && aligned16(dy) && aligned16(z);
+  const int64_t per = vec ? 1024 : 128;
+  const dim3 grid((unsigned)((out + per - 1) / per), (unsigned)((S + kActRows - 1) / kActRows));
   ProfScope prof_(c, "linear_act.dz");
-  launch_pdl(c, act_bwd_kernel<T>, dim3((unsigned)((out + 127) / 128), (unsigned)((S + kActRows - 1) / kActRows)),
-             dim3(128), 0, static_cast<const T*>(dy), static_cast<const T*>(z), bias, g, act, (long)S, (long)out, dz, (long)dz_ld, part);
+  auto kern = g ? (vec ? act_bwd_kernel<T, ACT, true, true> : act_bwd_kernel<T, ACT, false, true>)
+                : (vec ? act_bwd_kernel<T, ACT, true, false> : act_bwd_kernel<T, ACT, false, false>);
+  launch_pdl(c, kern, grid, dim3(128), 0, dy, z, bias, g, (long)S, (long)out, dz, (long)dz_ld, part);
   return check_launch("linear_act dz", err);
+}
+
+template <class T>
+int act_bwd(Ctx* c, const void* dyv, const void* zv, const float* bias, const float* g, int act, int64_t S, int64_t out,
+            __half* dz, int64_t dz_ld, float* part, std::string& err) {
+  const T* dy = static_cast<const T*>(dyv);
+  const T* z = static_cast<const T*>(zv);
+  switch (act) {
+    case kActSilu: return act_bwd_as<T, kActSilu>(c, dy, z, bias, g, S, out, dz, dz_ld, part, err);
+    case kActGelu: return act_bwd_as<T, kActGelu>(c, dy, z, bias, g, S, out, dz, dz_ld, part, err);
+    case kActGeluTanh: return act_bwd_as<T, kActGeluTanh>(c, dy, z, bias, g, S, out, dz, dz_ld, part, err);
+    default: return act_bwd_as<T, kActNone>(c, dy, z, bias, g, S, out, dz, dz_ld, part, err);
+  }
 }
 
 int linear_act_backward(Ctx* c, const Weight* w, const sa3k_adapter* ad, const float* bias, int act, int type,

@@ -177,6 +177,15 @@ struct HeadPrepEpi {
   float eps = 0.f;
 };
 
+// Activation and residual in a forward GEMM's epilogue (linear_act.cu): with v the value that the
+// GEMM would store (column scale and bias applied), z = v and the output is act(v) + residual.  z and
+// the residual have the output's type (out: f32, out_h: f16) and its row length N.
+struct ActEpi {
+  int act = 0;                   // activation.cuh
+  const void* residual = nullptr;
+  void* z = nullptr;
+};
+
 struct GemmDesc {
   int M = 0, N = 0, K = 0;
   // A: f16, K-major [M][lda] or (a_mn) MN-major [K][lda]
@@ -212,6 +221,7 @@ struct GemmDesc {
   // summation order, and so the last bits, vary from run to run).  f32 `out` only.
   int atomic_split = 0;
   const HeadPrepEpi* hp = nullptr;   // fused head preparation (CTA-pair path, f16 output only)
+  const ActEpi* epi = nullptr;       // (f16 K-major weight operand, row-major out or out_h of ld N)
   const char* name = "gemm";   // launch class for the profiler
 };
 
