@@ -177,8 +177,10 @@ static int launch(Ctx* c, const GemmDesc& d, const CUtensorMap& ta, const CUtens
         float* part = static_cast<float*>(scratch_get(c, kSlotSplitK, (size_t)splits * d.M * d.N * sizeof(float), err));
         if (!part) return 1;
         a.partial = part;
-        a.tile_cnt = split_counters(c, err);
-        if (!a.tile_cnt) return 1;
+        if (!d.epi) {
+          a.tile_cnt = split_counters(c, err);
+          if (!a.tile_cnt) return 1;
+        }
       }
     }
   }
@@ -205,6 +207,7 @@ static int launch(Ctx* c, const GemmDesc& d, const CUtensorMap& ta, const CUtens
     launch_pdl(c, kern, grid, R::THREADS, dyn, ta, tb, tbs, tea, teb, tout, a);
     if (check_launch("gemm_tc", err)) return 1;
   }
+  if (d.epi && a.partial) return k_act_splits(c, d, a.partial, a.splits, err);
   return 0;
 }
 

@@ -82,7 +82,7 @@ constexpr int kActBarBytes = 128;   // residual barriers: 8 epilogue warps x 2, 
 template <class Args>
 constexpr bool kHasAct = std::is_same<Args, GemmActArgs>::value;
 
-// One value of the direct and split-K paths: z kept, activation and residual applied.
+// One value of the direct path: z kept, activation and residual applied.
 template <class Args>
 __device__ __forceinline__ float act_element(const Args& args, float v, long row, int col) {
   if constexpr (kHasAct<Args>) {
@@ -394,8 +394,7 @@ __device__ __forceinline__ void epi_columns(const uint32_t (&v)[32], float* f, i
 // (__ldcg: other CTAs wrote them).  Four columns per thread when N % 4 == 0 (n0 is a multiple of
 // the N tile); the mapping is column-fastest for row-major outputs (coalesced partial reads and
 // output writes) and row-fastest when an output is transposed.
-template <class Args>
-__device__ __forceinline__ void splitk_finish(const Args& args, int m0, int n0, int rows, int cols, int tid,
+__device__ __forceinline__ void splitk_finish(const GemmArgs& args, int m0, int n0, int rows, int cols, int tid,
                                               int nt) {
   const long mn = (long)args.M * args.N;
   const bool trans = args.out_trans || args.out_h_trans || args.out_h_t;
@@ -423,7 +422,6 @@ __device__ __forceinline__ void splitk_finish(const Args& args, int m0, int n0, 
       float v = x[u] * args.alpha;
       if (args.col_scale) v *= args.col_scale[col];
       if (args.col_bias) v += args.col_bias[col];
-      v = act_element(args, v, row, col);
       if (args.out) {
         float* dst = args.out_trans ? args.out + (long)col * args.ldo + row : args.out + (long)row * args.ldo + col;
         *dst = args.accumulate ? *dst + v : v;
@@ -859,7 +857,7 @@ __global__ void __launch_bounds__(GemmRoles<BMODE>::THREADS, 1)
           __syncwarp();
         }
       }
-      if (split_out) {
+      if (!kHasAct<Args> && split_out) {      // (with an activation a pass of its own adds the splits)
         // ---- split-K: the CTA that completes the tile's last split reduces it.  Every thread
         // makes its partial stores visible, one thread counts the split in, and the last one
         // sums the splits in order 0, 1, ... (deterministic) from L2 and runs the epilogue.

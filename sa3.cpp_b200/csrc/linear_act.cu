@@ -26,6 +26,55 @@ __global__ void __launch_bounds__(256) act_residual_kernel(const float* zf, long
   }
 }
 
+// Output of a split-K product: partial sums added in split order, column scale, bias, activation and
+// residual; W columns per thread.  A pass of its own over all SMs: the last CTA of each tile adding its
+// own splits took most of the time (33 x 6144 x 1536: 32 us, with this pass 19).
+template <class T, int W>
+__global__ void __launch_bounds__(128) act_splits_kernel(const float* __restrict__ partial, int splits, long n, int N,
+                                                         const float* __restrict__ scale, const float* __restrict__ bias, int act,
+                                                         const T* __restrict__ residual, T* __restrict__ z, T* __restrict__ y) {
+  pdl_prologue();
+  const long i = ((long)blockIdx.x * 128 + threadIdx.x) * W;
+  if (i >= n) return;
+  float v[W];
+#pragma unroll
+  for (int e = 0; e < W; ++e) v[e] = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) {
+    if constexpr (W == 4) {
+      const float4 p = *reinterpret_cast<const float4*>(partial + (long)s * n + i);
+      v[0] += p.x; v[1] += p.y; v[2] += p.z; v[3] += p.w;
+    } else {
+      v[0] += partial[(long)s * n + i];
+    }
+  }
+  const int col = (int)(i % N);
+#pragma unroll
+  for (int e = 0; e < W; ++e) {
+    if (scale) v[e] *= scale[col + e];
+    if (bias) v[e] += bias[col + e];
+    if (z) z[i + e] = from_f32<T>(v[e]);
+    v[e] = act_value(act, v[e]);
+    if (residual) v[e] += to_f32(residual[i + e]);
+    y[i + e] = from_f32<T>(v[e]);
+  }
+}
+
+template <class T>
+int act_splits(Ctx* c, const GemmDesc& d, const float* partial, int splits, T* y, std::string& err) {
+  const long n = (long)d.M * d.N;
+  const T* res = static_cast<const T*>(d.epi->residual);
+  T* z = static_cast<T*>(d.epi->z);
+  ProfScope prof_(c, "linear_act.splits");
+  if (d.N % 4 == 0)
+    launch_pdl(c, act_splits_kernel<T, 4>, dim3((unsigned)((n / 4 + 127) / 128)), dim3(128), 0, partial, splits, n, d.N, d.col_scale,
+               d.col_bias, d.epi->act, res, z, y);
+  else
+    launch_pdl(c, act_splits_kernel<T, 1>, dim3((unsigned)((n + 127) / 128)), dim3(128), 0, partial, splits, n, d.N, d.col_scale,
+               d.col_bias, d.epi->act, res, z, y);
+  return check_launch("linear_act splits", err);
+}
+
 // dz = f16(g dy act'(z)), and with part the partial column sums over the block's kActRows rows:
 // part[blockIdx.y][0] of dy act'(z) (the bias gradient), [1] of dy act'(z) (z - bias) / g (dora's dg).
 // One pass: dy and z are read and dz is written once, in 16-byte accesses of 8 columns a thread (VEC)
@@ -237,6 +286,11 @@ int linear_act_backward(Ctx* c, const Weight* w, const sa3k_adapter* ad, const f
 }
 
 }  // namespace
+
+int k_act_splits(Ctx* c, const GemmDesc& d, const float* partial, int splits, std::string& err) {
+  return d.out_h ? act_splits<__half>(c, d, partial, splits, d.out_h, err) : act_splits<float>(c, d, partial, splits, d.out, err);
+}
+
 }  // namespace sa3k
 
 using namespace sa3k;

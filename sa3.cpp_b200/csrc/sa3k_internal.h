@@ -226,6 +226,9 @@ struct GemmDesc {
 };
 
 int gemm(Ctx* c, const GemmDesc& d, std::string& err);
+// the output of a split-K GEMM with an activation epilogue from its partial sums [splits][M][N]
+// (linear_act.cu)
+int k_act_splits(Ctx* c, const GemmDesc& d, const float* partial, int splits, std::string& err);
 // true when gemm() runs an M x N GEMM with an f16 B operand (f16_b) on the CTA-pair kernel
 bool gemm_pair_applies(const Ctx* c, int M, int N, bool f16_b);
 
