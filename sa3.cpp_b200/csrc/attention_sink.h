@@ -43,4 +43,8 @@ __device__ __forceinline__ bool sink_sees(const SinkArgs& a, const SinkSeq& s, i
   return j < s.kn && j <= p + a.right && (j < a.sinks || j >= p - a.left);
 }
 
+// the forward for a few query rows per key / value head (attention_rows.cu)
+bool sink_rows_applies(const SinkArgs& a);
+int sink_rows_forward(Ctx* c, const SinkArgs& a, bool bf16, std::string& err);
+
 }  // namespace sa3k
