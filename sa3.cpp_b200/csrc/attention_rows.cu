@@ -5,7 +5,7 @@
 // values once, at the rate of memory, and to have enough loads in flight.  The query rows of all heads
 // that share a key / value head form one 16-row operand of mma.sync m16n8k16, so a shared head's cache
 // is read once for its group.  Work is split along the keys twice: the warps of a CTA take the 32-key
-// steps that the window and the sinks cover in turn, and the CTAs of a cluster (1 to 8) take turns
+// steps that the window and the sinks cover in turn, and the CTAs of a cluster (1 to 16) take turns
 // before that, so that a batch of one still reaches most SMs.  Every warp keeps its own running
 // maximum, sum and output (f32, registers) and three steps of K and V (8 KB each, cp.async) in
 // flight; warps are joined through shared memory and CTAs through their cluster's, in rank order, so
@@ -71,11 +71,20 @@ __device__ __forceinline__ float exp2_of(float x) {
   return y;
 }
 
-__device__ __forceinline__ float ld_cluster(const float* p, uint32_t rank) {
+// shared memory of CTA `rank` of the cluster, at this CTA's address p
+__device__ __forceinline__ uint32_t peer(const float* p, uint32_t rank) {
   uint32_t a;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ float ld_peer(uint32_t a) {
   float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ float4 ld_peer4(uint32_t a) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a));
   return v;
 }
 __device__ __forceinline__ void cluster_barrier() {
@@ -92,27 +101,6 @@ __global__ void __launch_bounds__(32 * kRowsWarps, 2) sink_rows_kernel(const __g
   const int b = blockIdx.y / a.Hkv, hk = blockIdx.y % a.Hkv;
   const SinkSeq s = sink_seq(a, b);
   const int row0 = blockIdx.z * 16, rows = min(16, s.qn * a.group - row0);
-  // this thread's rows g and g + 8
-  int p[2];
-  uint32_t q[4][4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) q[k][i] = 0u;
-#pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int r = row0 + g + 8 * u, i = r / a.group, h = hk * a.group + r % a.group;
-    p[u] = s.pos0 + i;
-    if (g + 8 * u < rows) {
-      const uint32_t* src = reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(a.q.p) + (long)b * a.q.sb +
-                                                             (long)h * a.q.sh + (long)i * a.q.ld);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {        // dims 16 k + 2 t (, + 1) and 16 k + 8 + 2 t
-        q[k][u] = src[8 * k + t];
-        q[k][2 + u] = src[8 * k + 4 + t];
-      }
-    }
-  }
   // 32-key steps that some row of the tile sees: sink steps [0, ns), window steps from w0
   const int plo = s.pos0 + row0 / a.group, phi = s.pos0 + (row0 + max(rows, 1) - 1) / a.group;
   int ns = 0, w0 = 0, n = 0;
@@ -151,6 +139,27 @@ __global__ void __launch_bounds__(32 * kRowsWarps, 2) sink_rows_kernel(const __g
     for (int i = 0; i < 4; ++i) o[d][i] = 0.f;
   const int mine = first < n ? (n - first + stride - 1) / stride : 0;
   for (int c = 0; c < kRowsStages - 1; ++c) load(c);
+  // this thread's rows g and g + 8
+  int p[2];
+  uint32_t q[4][4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[k][i] = 0u;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int r = row0 + g + 8 * u, i = r / a.group, h = hk * a.group + r % a.group;
+    p[u] = s.pos0 + i;
+    if (g + 8 * u < rows) {
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(a.q.p) + (long)b * a.q.sb +
+                                                             (long)h * a.q.sh + (long)i * a.q.ld);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {        // dims 16 k + 2 t (, + 1) and 16 k + 8 + 2 t
+        q[k][u] = src[8 * k + t];
+        q[k][2 + u] = src[8 * k + 4 + t];
+      }
+    }
+  }
   for (int c = 0; c < mine; ++c) {
     cp_wait<kRowsStages - 2>();
     __syncwarp();
@@ -262,17 +271,39 @@ __global__ void __launch_bounds__(32 * kRowsWarps, 2) sink_rows_kernel(const __g
     }
     cluster_barrier();
     if (rank == 0) {
-      const float* own0 = own;
       M = -INFINITY;
-      for (int c = 0; c < nrank; ++c) M = fmaxf(M, ld_cluster(own0 + 1024 + r, c));
       L = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = 0.f;
-      for (int c = 0; c < nrank; ++c) {
-        const float f = M == -INFINITY ? 1.f : exp2_of(ld_cluster(own0 + 1024 + r, c) - M);
-        L = fmaf(f, ld_cluster(own0 + 1040 + r, c), L);
+      for (int c0 = 0; c0 < nrank; c0 += 8) {      // eight peers' values are requested before the first is used
+        float mc[8], lc[8], top = M;
+        float4 x0[8], x1[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = fmaf(f, ld_cluster(own0 + r * 64 + d0 + e, c), v[e]);
+        for (int c = 0; c < 8; ++c) {
+          mc[c] = -INFINITY;
+          if (c0 + c >= nrank) continue;
+          const uint32_t base = peer(own, c0 + c);
+          mc[c] = ld_peer(base + 4 * (1024 + r));
+          lc[c] = ld_peer(base + 4 * (1040 + r));
+          x0[c] = ld_peer4(base + 4 * (r * 64 + d0));
+          x1[c] = ld_peer4(base + 4 * (r * 64 + d0 + 4));
+        }
+#pragma unroll
+        for (int c = 0; c < 8; ++c) top = fmaxf(top, mc[c]);
+        const float f0 = top == -INFINITY ? 1.f : exp2_of(M - top);
+        M = top;
+        L *= f0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= f0;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          if (c0 + c >= nrank) continue;
+          const float f = M == -INFINITY ? 1.f : exp2_of(mc[c] - M);
+          const float x[8] = {x0[c].x, x0[c].y, x0[c].z, x0[c].w, x1[c].x, x1[c].y, x1[c].z, x1[c].w};
+          L = fmaf(f, lc[c], L);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = fmaf(f, x[e], v[e]);
+        }
       }
     }
     cluster_barrier();       // (no CTA leaves while its shared memory is read)
@@ -295,11 +326,17 @@ int launch(Ctx* c, const SinkArgs& a, std::string& err) {
   auto kern = sink_rows_kernel<BF>;
   if (smem_attr(reinterpret_cast<const void*>(kern), kRowsSmem, c->device, "attention_sink smem attribute", err)) return 1;
   const int tiles = (a.Sq * a.group + 15) / 16;
-  // CTAs per (batch entry, head): a power of two up to 8, until there are two per SM or every warp
-  // would be left with less than two of the steps that a full window has
+  // CTAs per (batch entry, head): a power of two up to 16, until there are two per SM.  Up to 4 pay when
+  // every warp keeps two of its 32-key steps (1 x 24 heads, 576 keys: 6.6 us with one, 6.1 with four),
+  // more when it keeps five (4 x 8 heads, 2051 keys: 8.1 us with four, 9.0 with eight; 1 x 8 heads,
+  // 65536 keys: 92 us with four, 49 with eight).
   const long span = std::min<long>(a.Sk, (long)a.sinks + std::min<long>((long)a.left + a.right + a.Sq, a.Sk));
   int nrank = 1;
-  while (nrank < 8 && (long)a.B * a.Hkv * tiles * nrank < 2 * (long)c->sm_count && span > (long)nrank * kRowsWarps * 64) nrank *= 2;
+  while (nrank < 16 && (long)a.B * a.Hkv * tiles * nrank < 2 * (long)c->sm_count &&
+         span > (long)nrank * kRowsWarps * (nrank < 4 ? 64 : 160))
+    nrank *= 2;
+  if (nrank > 8 && cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+    return check_launch("attention_sink cluster attribute", err);
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;

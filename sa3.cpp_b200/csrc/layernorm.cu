@@ -22,24 +22,27 @@
 namespace sa3k {
 namespace {
 
-// out[i] (+)= sum over blocks of part[block][which][i]: 32 columns x 32 slices of the blocks per
-// thread block, the slices added in order.
-__global__ void __launch_bounds__(1024) fold_partials_kernel(const float* part, int nblocks, int cols, float* out0,
-                                                             float* out1, int acc0, int acc1) {
-  __shared__ float s[32][33];
+// out[i] (+)= sum over b of part[b][which][i]: a block takes 8 columns (a 32-byte sector) in 64 slices of
+// the partial rows, which are then added in order.
+__global__ void __launch_bounds__(512) fold_partials_kernel(const float* part, int nblocks, int cols, float* out0,
+                                                            float* out1, int acc0, int acc1) {
+  __shared__ float s[8][65];
   pdl_prologue();
-  const int i = blockIdx.x * 32 + (threadIdx.x & 31), w = threadIdx.x >> 5;
+  const int e = threadIdx.x & 7, w = threadIdx.x >> 3, i = blockIdx.x * 8 + e;
   float* out = blockIdx.y == 0 ? out0 : out1;
   if (!out) return;
   const float* p = part + (long)blockIdx.y * cols + i;
   float v = 0.f;
-  if (i < cols)
-    for (int b = w; b < nblocks; b += 32) v += p[(long)b * 2 * cols];
-  s[w][threadIdx.x & 31] = v;
+  if (i < cols) {
+#pragma unroll 4
+    for (int b = w; b < nblocks; b += 64) v += p[(long)b * 2 * cols];
+  }
+  s[e][w] = v;
   __syncthreads();
-  // warp w takes column w of the 32: its lanes hold the 32 slices
-  v = warp_sum(s[threadIdx.x & 31][w]);
-  const int o = blockIdx.x * 32 + w;
+  const int c = threadIdx.x >> 5;       // warps 0 .. 7: a column each
+  if (c >= 8) return;
+  v = warp_sum(s[c][threadIdx.x & 31] + s[c][32 + (threadIdx.x & 31)]);
+  const int o = blockIdx.x * 8 + c;
   if ((threadIdx.x & 31) == 0 && o < cols) out[o] = (blockIdx.y == 0 ? acc0 : acc1) ? out[o] + v : v;
 }
 
@@ -48,7 +51,7 @@ __global__ void __launch_bounds__(1024) fold_partials_kernel(const float* part, 
 int k_fold_partials(Ctx* c, const float* part, int nblocks, int cols, float* out0, float* out1, int acc0, int acc1,
                     std::string& err) {
   ProfScope prof_(c, "fold_partials");
-  launch_pdl(c, fold_partials_kernel, dim3((unsigned)((cols + 31) / 32), 2), dim3(1024), 0, part, nblocks, cols, out0, out1,
+  launch_pdl(c, fold_partials_kernel, dim3((unsigned)((cols + 7) / 8), 2), dim3(512), 0, part, nblocks, cols, out0, out1,
              acc0, acc1);
   return check_launch("fold partials", err);
 }
@@ -142,7 +145,7 @@ __device__ __forceinline__ void store_chunk(T* p, int c, int t, int tpr, int col
 
 // Forward with the row in registers: NV chunks of 8 columns per thread.
 template <class TX, class TY, bool BLOCK, int NV, bool VEC>
-__global__ void __launch_bounds__(1024) ln_fwd_kernel(const LnArgs a, int tpr) {
+__global__ void __launch_bounds__(BLOCK ? 1024 : 256) ln_fwd_kernel(const LnArgs a, int tpr) {
   __shared__ float2 red[2][32];
   pdl_prologue();
   const int t = BLOCK ? threadIdx.x : threadIdx.x & (tpr - 1);
@@ -307,6 +310,175 @@ __global__ void __launch_bounds__(1024) ln_bwd_kernel(const LnArgs a, int tpr) {
   }
 }
 
+// Backward of rows of 257 to 8192 columns with vector access.  The block's next rows of x and dy come
+// into a ring in shared memory by bulk copies, pairs of rows ahead, so that memory stays busy through
+// the reductions; and two rows are reduced together: their four sums take 6 shuffles a warp (each step
+// sends away the half that the lane does not keep) and one barrier, where row by row it was 40 and two.
+// Packed f32 pairs halve the instructions, which bounded the kernel (270 a warp and row, 2.4 a clock).
+// A thread takes about 85 registers without spills (they went to L2, the ring having taken L1: 44 us
+// for 16383 x 1536 with the fold instead of 35), so the blocks per SM follow from the threads of a row; rows of more
+// than 5120 columns have 64 registers a thread and read the slot again instead of holding its values.
+constexpr int kLnMaxSlots = 8;
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+// (a0, b0, a1, b1) summed over the block; `red` is alternated by the caller
+__device__ __forceinline__ float4 block_sum4(float a0, float b0, float a1, float b1, float4* red) {
+  const int lane = threadIdx.x & 31, nw = blockDim.x >> 5;
+  const bool hi = lane & 16, sel = lane & 8;
+  float a = (hi ? a1 : a0) + __shfl_xor_sync(0xffffffffu, hi ? a0 : a1, 16);
+  float b = (hi ? b1 : b0) + __shfl_xor_sync(0xffffffffu, hi ? b0 : b1, 16);
+  float v = (sel ? b : a) + __shfl_xor_sync(0xffffffffu, sel ? a : b, 8);
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if ((lane & 7) == 0) reinterpret_cast<float*>(red + (threadIdx.x >> 5))[lane >> 3] = v;
+  __syncthreads();
+  float4 s = red[0];
+#pragma unroll 2
+  for (int w = 1; w < nw; ++w) {
+    const float4 x = red[w];
+    s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+  }
+  return s;
+}
+
+template <class TX, class TY, int MAXT, int MINB>
+__global__ void __launch_bounds__(MAXT, MINB) ln_bwd_ring_kernel(const LnArgs a, int slots, int* err) {
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ float4 red[2][32];
+  __shared__ __align__(8) uint64_t full[kLnMaxSlots];
+  const int t = threadIdx.x, i0 = 8 * t;
+  const uint32_t xb = (uint32_t)a.cols * sizeof(TX), yb = (uint32_t)a.cols * sizeof(TY), row_bytes = xb + yb;
+  if (t == 0) {
+    for (int k = 0; k < slots; ++k) mbar_init(&full[k], 1);
+    fence_barrier_init();
+  }
+  __syncthreads();
+  pdl_prologue();
+  const long first = blockIdx.x, step = gridDim.x;          // a pair: rows r and r + step
+  auto fetch = [&](long r, int slot) {                      // (thread 0)
+    const int n = r + step < a.rows ? 2 : 1;
+    mbar_arrive_expect_tx(&full[slot], n * row_bytes);
+    for (int k = 0; k < n; ++k) {
+      uint8_t* dst = ring + (size_t)(2 * slot + k) * row_bytes;
+      bulk_load(dst, static_cast<const TX*>(a.x) + (r + k * step) * a.x_ld, xb, &full[slot]);
+      bulk_load(dst + xb, static_cast<const TY*>(a.dy) + (r + k * step) * a.dy_ld, yb, &full[slot]);
+    }
+  };
+  if (t == 0)
+    for (int k = 0; k < slots; ++k)
+      if (first + 2 * k * step < a.rows) fetch(first + 2 * k * step, k);
+  const bool in = i0 < a.cols;
+  uint64_t gm[4], sg[4], sb[4];            // pairs of f32 (two lanes of work per instruction)
+#pragma unroll
+  for (int e = 0; e < 4; ++e) gm[e] = f2(1.f, 1.f), sg[e] = sb[e] = f2(0.f, 0.f);
+  if (a.gamma && in) {
+    float v[8];
+    load8(a.gamma + i0, v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) gm[e] = f2(v[2 * e], v[2 * e + 1]);
+  }
+  const float inv = 1.f / (float)a.cols;
+  bool ok = true;
+  int slot = 0, ph = 0;
+  uint32_t phase = 0;
+  float mu[2] = {0.f, 0.f}, rs[2] = {0.f, 0.f};
+  auto stats = [&](long r, float (&m)[2], float (&q)[2]) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (r + k * step < a.rows) {
+        m[k] = a.mean[r + k * step];
+        q[k] = a.rstd[r + k * step];
+      }
+  };
+  float mu_next[2] = {0.f, 0.f}, rs_next[2] = {0.f, 0.f};
+  stats(first, mu_next, rs_next);
+  for (long r = first; r < a.rows; r += 2 * step, ph ^= 1) {
+    const bool two = r + step < a.rows;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      mu[k] = mu_next[k];
+      rs[k] = rs_next[k];
+    }
+    stats(r + 2 * step, mu_next, rs_next);
+    if (ok) ok = mbar_wait(&full[slot], phase, err, kErrTimeoutFull);
+    const uint8_t* src = ring + (size_t)(2 * slot) * row_bytes;
+    float s1[2] = {0.f, 0.f}, s2[2] = {0.f, 0.f};
+    constexpr bool HOLD = MAXT < 1024;
+    uint64_t xh[2][4], g[2][4];
+    auto row_of = [&](int k) {       // xh and g of row k from the slot
+      float xv[8], dv[8];
+      load8(reinterpret_cast<const TX*>(src + k * row_bytes) + i0, xv);
+      load8(reinterpret_cast<const TY*>(src + k * row_bytes + xb) + i0, dv);
+      const uint64_t nmu = f2(-mu[k], -mu[k]), rs2 = f2(rs[k], rs[k]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        xh[k][e] = fmul2(fadd2(f2(xv[2 * e], xv[2 * e + 1]), nmu), rs2);
+        g[k][e] = f2(dv[2 * e], dv[2 * e + 1]);       // (dy; times gamma below)
+      }
+    };
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (!in || (k && !two)) continue;
+      row_of(k);
+      uint64_t p1 = f2(0.f, 0.f), p2 = p1;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        sg[e] = ffma2(g[k][e], xh[k][e], sg[e]);
+        sb[e] = fadd2(sb[e], g[k][e]);
+        g[k][e] = fmul2(g[k][e], gm[e]);
+        p1 = fadd2(p1, g[k][e]);
+        p2 = ffma2(g[k][e], xh[k][e], p2);
+      }
+      float u, v;
+      f2split(p1, u, v);
+      s1[k] = u + v;
+      f2split(p2, u, v);
+      s2[k] = u + v;
+    }
+    const float4 sum = block_sum4(s1[0], s2[0], s1[1], s2[1], red[ph]);
+    // (every thread has read the slot before the sum's barrier, unless it reads it again)
+    if (HOLD && t == 0 && ok && r + 2 * slots * step < a.rows) fetch(r + 2 * slots * step, slot);
+    if (a.out && in && ok) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if (k && !two) continue;
+        if (!HOLD) {
+          row_of(k);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) g[k][e] = fmul2(g[k][e], gm[e]);
+        }
+        const float m1 = (k ? sum.z : sum.x) * inv, m2 = (k ? sum.w : sum.y) * inv, c = -m1 * rs[k];
+        const uint64_t nm2 = f2(-m2, -m2), rs2 = f2(rs[k], rs[k]), c2 = f2(c, c);
+        float o[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f2split(ffma2(ffma2(xh[k][e], nm2, g[k][e]), rs2, c2), o[2 * e], o[2 * e + 1]);
+        store8(static_cast<TX*>(a.out) + (r + k * step) * a.out_ld + i0, o);
+      }
+    }
+    if (!HOLD) {
+      __syncthreads();
+      if (t == 0 && ok && r + 2 * slots * step < a.rows) fetch(r + 2 * slots * step, slot);
+    }
+    if (++slot == slots) {
+      slot = 0;
+      phase ^= 1u;
+    }
+  }
+  if (!in || !a.part) return;
+  float* part = a.part + (long)blockIdx.x * 2 * a.cols;
+  float v[8];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) f2split(sg[e], v[2 * e], v[2 * e + 1]);
+  store8(part + i0, v);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) f2split(sb[e], v[2 * e], v[2 * e + 1]);
+  store8(part + a.cols + i0, v);
+}
+
 // Backward of rows too long for the registers: dx in two passes over the row.
 template <class TX, class TY>
 __global__ void __launch_bounds__(1024) ln_bwd_long_kernel(const LnArgs a) {
@@ -352,19 +524,21 @@ constexpr int kLnMaxRegCols = 32768;   // 1024 threads x 32 values
 
 // Threads per row and chunks per thread.  Rows of up to 256 columns take a part of a warp (the
 // smallest power of two that holds them at 8 columns a thread); longer ones a whole block of at
-// most 1024 threads, at 8, 16 or 32 columns a thread.
+// most 1024 threads, at 8, 16 or 32 columns a thread.  In the forward rows of up to 2048 columns stay
+// with one warp, at up to 64 columns a thread: no barrier, and all of a row's loads in flight (4352 x
+// 1536 f32 -> f16: 12.4 us with blocks, 9.6 with warps).
 struct LnShape {
   bool block;
   int tpr, threads, nv;
 };
-LnShape ln_shape(int cols) {
+LnShape ln_shape(int cols, bool forward) {
   LnShape s;
-  if (cols <= 256) {
+  if (cols <= (forward ? 2048 : 256)) {
     s.block = false;
     s.tpr = 1;
-    while (s.tpr * 8 < cols) s.tpr *= 2;
+    while (s.tpr * 8 < cols && s.tpr < 32) s.tpr *= 2;
     s.threads = 256;
-    s.nv = 1;
+    s.nv = (cols + 255) / 256;
     return s;
   }
   s.block = true;
@@ -391,8 +565,17 @@ int fwd_typed(Ctx* c, const LnArgs& a, bool vec, std::string& err) {
     launch_pdl(c, ln_fwd_long_kernel<TX, TY>, dim3((unsigned)a.rows), dim3(1024), 0, a);
     return check_launch("layernorm forward", err);
   }
-  const LnShape s = ln_shape(a.cols);
-  if (!s.block) return fwd_launch<TX, TY, false, 1>(c, a, s, vec, err);
+  const LnShape s = ln_shape(a.cols, true);
+  if (!s.block) {
+    switch (s.nv) {
+      case 1: return fwd_launch<TX, TY, false, 1>(c, a, s, vec, err);
+      case 2: return fwd_launch<TX, TY, false, 2>(c, a, s, vec, err);
+      case 3: return fwd_launch<TX, TY, false, 3>(c, a, s, vec, err);
+      case 4: return fwd_launch<TX, TY, false, 4>(c, a, s, vec, err);
+      case 5: case 6: return fwd_launch<TX, TY, false, 6>(c, a, s, vec, err);
+      default: return fwd_launch<TX, TY, false, 8>(c, a, s, vec, err);
+    }
+  }
   if (s.nv == 1) return fwd_launch<TX, TY, true, 1>(c, a, s, vec, err);
   if (s.nv == 2) return fwd_launch<TX, TY, true, 2>(c, a, s, vec, err);
   return fwd_launch<TX, TY, true, 4>(c, a, s, vec, err);
@@ -404,6 +587,34 @@ int bwd_blocks(Ctx* c, const LnArgs& a, const LnShape& s) {
   const long need = (a.rows + per - 1) / per;
   const long fit = (long)c->sm_count * std::max(1, 1024 / s.threads);
   return (int)std::max(1L, std::min(need, fit));
+}
+
+// The ring kernel's launch for a row's threads: blocks per SM, and pairs of rows in their share of 200
+// KB (the longest f32 rows, 64 KB of x and dy, have one).
+struct RingShape {
+  int threads, per_sm, slots, blocks;
+};
+RingShape ring_shape(Ctx* c, const LnArgs& a, size_t row_bytes) {
+  RingShape r;
+  r.threads = ((a.cols + 7) / 8 + 31) / 32 * 32;
+  r.per_sm = r.threads <= 96 ? 8 : r.threads <= 192 ? 4 : r.threads <= 320 ? 2 : 1;
+  r.slots = (int)std::max<size_t>(1, std::min<size_t>(kLnMaxSlots, (size_t)200 * 1024 / r.per_sm / (2 * row_bytes)));
+  r.blocks = (int)std::min<long>((long)c->sm_count * r.per_sm, a.rows);
+  return r;
+}
+
+template <class TX, class TY>
+int ring_launch(Ctx* c, const LnArgs& a, const RingShape& r, std::string& err) {
+  const size_t smem = (size_t)r.slots * 2 * a.cols * (sizeof(TX) + sizeof(TY));
+  auto kern = r.threads <= 96    ? ln_bwd_ring_kernel<TX, TY, 96, 8>
+              : r.threads <= 192 ? ln_bwd_ring_kernel<TX, TY, 192, 4>
+              : r.threads <= 320 ? ln_bwd_ring_kernel<TX, TY, 320, 2>
+              : r.threads <= 640 ? ln_bwd_ring_kernel<TX, TY, 640, 1>
+                                 : ln_bwd_ring_kernel<TX, TY, 1024, 1>;
+  if (smem_attr(reinterpret_cast<const void*>(kern), 200 * 1024, c->device, "layernorm smem attribute", err)) return 1;
+  ProfScope prof_(c, "layernorm.bwd");
+  launch_pdl(c, kern, dim3(r.blocks), dim3(r.threads), smem, a, r.slots, c->d_err);
+  return check_launch("layernorm backward", err);
 }
 
 template <class TX, class TY, bool BLOCK, int NV, bool VEC>
@@ -420,12 +631,20 @@ int bwd_typed(Ctx* c, LnArgs a, bool vec, float* dgamma, float* dbeta, int accum
   const bool params = dgamma || dbeta;
   const bool lng = a.cols > kLnMaxRegCols;
   LnShape s{};
+  RingShape ring{};
+  bool use_ring = false;
   int blocks;
   if (lng) {
     blocks = (int)std::min<long>(a.rows, 64);
   } else {
-    s = ln_shape(a.cols);
-    blocks = bwd_blocks(c, a, s);
+    s = ln_shape(a.cols, false);
+    use_ring = vec && s.block && s.nv == 1;
+    if (use_ring) {
+      ring = ring_shape(c, a, (size_t)a.cols * (sizeof(TX) + sizeof(TY)));
+      blocks = ring.blocks;
+    } else {
+      blocks = bwd_blocks(c, a, s);
+    }
   }
   if (params) {
     a.part = static_cast<float*>(scratch_get(c, kSlotLnPart, (size_t)blocks * 2 * a.cols * sizeof(float), err));
@@ -440,8 +659,10 @@ int bwd_typed(Ctx* c, LnArgs a, bool vec, float* dgamma, float* dbeta, int accum
     rc = check_launch("layernorm backward", err);
   } else if (!s.block) {
     rc = vec ? bwd_launch<TX, TY, false, 1, true>(c, a, s, blocks, err) : bwd_launch<TX, TY, false, 1, false>(c, a, s, blocks, err);
+  } else if (use_ring) {
+    rc = ring_launch<TX, TY>(c, a, ring, err);
   } else if (s.nv == 1) {
-    rc = vec ? bwd_launch<TX, TY, true, 1, true>(c, a, s, blocks, err) : bwd_launch<TX, TY, true, 1, false>(c, a, s, blocks, err);
+    rc = bwd_launch<TX, TY, true, 1, false>(c, a, s, blocks, err);
   } else if (s.nv == 2) {
     rc = vec ? bwd_launch<TX, TY, true, 2, true>(c, a, s, blocks, err) : bwd_launch<TX, TY, true, 2, false>(c, a, s, blocks, err);
   } else {
