@@ -138,17 +138,19 @@ __device__ __forceinline__ void zero_rows(uint8_t* tile, int from, int t, int n)
 // A warp's 32 rows of 8 NC values (NC chunks of 16 bytes per lane, its lane's row) to global memory
 // by way of shared memory, so that a store instruction writes whole 128- or 64-byte rows instead of
 // 16 bytes of 32 rows (measured on the forward's 128-row tiles: 6000 cycles a CTA against 1500).
-// `buf`: 32 rows x 128 bytes of this warp's own; `out`: row 0's first value; rows at or past n stay.
-template <int NC>
+// `buf`: 32 rows x PITCH bytes of this warp's own; `out`: row 0's first value; rows at or past n stay.
+template <int NC, int PITCH = 128>
 __device__ __forceinline__ void store_rows(uint8_t* buf, const uint4 (&w)[NC], uint16_t* out, long ld, int n, int lane) {
+  // (chunks are swizzled within a row: by the row in rows of 128 bytes, by half of it in rows of 64)
+  auto at = [](int r, int q) { return r * PITCH + ((PITCH == 128 ? q ^ (r & 7) : q ^ ((r >> 1) & 3)) << 4); };
 #pragma unroll
-  for (int q = 0; q < NC; ++q) *reinterpret_cast<uint4*>(buf + lane * 128 + ((q ^ (lane & 7)) << 4)) = w[q];
+  for (int q = 0; q < NC; ++q) *reinterpret_cast<uint4*>(buf + at(lane, q)) = w[q];
   __syncwarp();
   constexpr int PER = 32 / NC;       // rows per store
 #pragma unroll
   for (int k = 0; k < 32 / PER; ++k) {
     const int r = k * PER + lane / NC, q = lane % NC;
-    const uint4 v = *reinterpret_cast<const uint4*>(buf + r * 128 + ((q ^ (r & 7)) << 4));
+    const uint4 v = *reinterpret_cast<const uint4*>(buf + at(r, q));
     if (r < n) *reinterpret_cast<uint4*>(out + (long)r * ld + 8 * q) = v;
   }
 }
@@ -454,6 +456,7 @@ __global__ void __launch_bounds__(kSinkThreads, 2)
   const uint32_t tbase = *tmem_slot;
   pdl_wait();
 
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.next_item = 0;     // for the dk / dv pass
   const int bh = blockIdx.y, b = bh / a.H, h = bh % a.H, r0 = blockIdx.x * 128;
   const SinkSeq s = sink_seq(a, b);
   const int rows = min(128, s.qn - r0), plo = s.pos0 + r0, phi = plo + rows - 1;
@@ -609,44 +612,70 @@ __global__ void __launch_bounds__(kSinkThreads, 2)
 }
 
 // ==================================================================================== dk, dv
-// CTA: 128 keys of one (batch entry, key / value head); the 64-row query tiles that see them, of
-// every query head of the group, stream past.  Threads own a key row; the warpgroups take 32 of a
-// tile's 64 query columns each.
-// TMEM: S^T [0, 64) and dP^T [64, 128) (P^T, dS^T of columns 32 g .. overwrite the first 16 columns
-// of their own halves), dV [128, 192), dK [192, 256).
-constexpr int kDkvStages = 4;
-constexpr int kDkvSmem = 32768 + kDkvStages * 2 * kTile + 2048 + 256 + 1024;
+// Persistent, one CTA per SM: an item is 128 keys of one (batch entry, key / value head); the 64-row
+// query tiles that see them, of every query head of the group, stream past, and the tiles of one item
+// after the other form one stream of steps.  16 softmax warps in two sets take alternate steps (in a
+// set a thread owns a key row and 32 of the step's 64 query columns), and there are three buffers for
+// S^T and dP^T, so a set finds its next scores ready: with one CTA of 8 warps and one buffer twice per
+// SM every step waited for four products in series (1450 clocks a step and SM; now 700).
+// Items are handed out by a counter, heaviest first (those with sinks are seen by every later query).
+// TMEM: buffer u < 3 at 128 u: S^T [0, 64), dP^T [64, 128) (P^T, dS^T of columns 32 g .. overwrite the
+// first 16 columns of their own halves); dV at 384, dK at 448.
+// smem: 2 x (K 16 KB, V 16 KB) | 6 x (Q 8 KB, dO 8 KB) | 16 x 2 KB output rows | 16 x lse, D | items | barriers
+constexpr int kDkvSets = 2, kDkvStages = 6, kDkvItems = 4;
+constexpr int kDkvWarps = 8 * kDkvSets, kDkvThreads = 32 * (kDkvWarps + 2);
+constexpr int kDkvSmem = 65536 + kDkvStages * 2 * kTile + kDkvWarps * (2048 + 256) + 256 + 512 + 1024;
+
+struct DkvItem {      // n > 0 steps: query tiles [qt0, qt1) of each of the group's heads; n < 0: no more items
+  int b, hk, k0, keys, qt0, qt1, n, pos0, qn, kn;
+};
 
 template <bool BF>
-__global__ void __launch_bounds__(kSinkThreads, 2)
+__global__ void __launch_bounds__(kDkvThreads, 1)
     sink_dkdv_kernel(const __grid_constant__ SeqMap mk, const __grid_constant__ SeqMap mv, const __grid_constant__ SeqMap mq,
                      const __grid_constant__ SeqMap mdo, const __grid_constant__ SinkArgs a) {
   extern __shared__ uint8_t smem_raw[];
   pdl_trigger();
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sK = smem;                   // K 16 KB | V 16 KB
-  uint8_t* sQd = smem + 32768;
-  float* s_ld = reinterpret_cast<float*>(sQd + kDkvStages * 2 * kTile);   // [2 groups][2][16 column pairs][lse 2 | D 2]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sQd + kDkvStages * 2 * kTile + 2048);
-  uint64_t* kv_full = bars;
-  uint64_t* q_full = kv_full + 1;
-  uint64_t* q_empty = q_full + kDkvStages;
-  uint64_t* s_full = q_empty + kDkvStages;
-  uint64_t* ds_full = s_full + 1;
-  uint64_t* acc_full = ds_full + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  uint8_t* sKV = smem;                                  // [2] K | V
+  uint8_t* sQd = smem + 65536;                          // [kDkvStages] Q | dO
+  uint8_t* sOut = sQd + kDkvStages * 2 * kTile;         // [warps][32 rows x 64 bytes]
+  float* s_ld = reinterpret_cast<float*>(sOut + kDkvWarps * 2048);          // [warps][16 column pairs][lse 2 | D 2]
+  DkvItem* items = reinterpret_cast<DkvItem*>(s_ld + 64 * kDkvWarps);       // [kDkvItems]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(items) + 256);
+  uint64_t* kv_full = bars;                             // [2]
+  uint64_t* kv_empty = kv_full + 2;                     // [2] the item's last scores are done
+  uint64_t* q_full = kv_empty + 2;
+  uint64_t* q_empty = q_full + kDkvStages;              // dV and dK of the slot's tile are done
+  uint64_t* s_full = q_empty + kDkvStages;              // [3]
+  uint64_t* ds_full = s_full + 3;                       // [3]
+  uint64_t* acc_full = ds_full + 3;
+  uint64_t* acc_empty = acc_full + 1;
+  uint64_t* item_full = acc_empty + 1;                  // [kDkvItems]
+  uint64_t* item_empty = item_full + kDkvItems;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(item_empty + kDkvItems);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (warp == kSoftWarps && lane == 0) {
-    mbar_init(kv_full, 1);
-    for (int s = 0; s < kDkvStages; ++s) {
-      mbar_init(&q_full[s], 1);
-      mbar_init(&q_empty[s], 1);
+  if (warp == kDkvWarps && lane == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 1);
     }
-    mbar_init(s_full, 1);
-    mbar_init(ds_full, kSoftWarps);
+    for (int i = 0; i < kDkvStages; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
+    }
+    for (int i = 0; i < 3; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&ds_full[i], 8);
+    }
     mbar_init(acc_full, 1);
+    mbar_init(acc_empty, kDkvWarps);
+    for (int i = 0; i < kDkvItems; ++i) {
+      mbar_init(&item_full[i], 1);
+      mbar_init(&item_empty[i], kDkvWarps + 1);
+    }
     *abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&mk.m);
@@ -654,8 +683,8 @@ __global__ void __launch_bounds__(kSinkThreads, 2)
     tma_prefetch_desc(&mq.m);
     tma_prefetch_desc(&mdo.m);
   }
-  if (warp == kSoftWarps + 1) {
-    tmem_alloc(tmem_slot, 256);
+  if (warp == kDkvWarps + 1) {
+    tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
     tc_fence_before();
   }
@@ -663,191 +692,256 @@ __global__ void __launch_bounds__(kSinkThreads, 2)
   tc_fence_after();
   const uint32_t tbase = *tmem_slot;
   pdl_wait();
-
-  // first the tiles with sinks, which the most queries see, of every head
-  const int nbh = a.B * a.Hkv, bh = blockIdx.x % nbh, b = bh / a.Hkv, hk = bh % a.Hkv, k0 = (int)(blockIdx.x / nbh) * 128;
-  const SinkSeq s = sink_seq(a, b);
-  const int keys = min(128, s.kn - k0);
-  int qt0 = 0, nt = 0;                  // query tiles [qt0, qt0 + nt) of each head
-  if (keys > 0) {
-    const int lo = max(0, k0 - a.right - s.pos0);
-    const int hi = k0 < a.sinks ? s.qn : min(s.qn, k0 + keys + a.left - s.pos0);
-    if (lo < hi) {
-      qt0 = lo >> 6;
-      nt = ((hi + 63) >> 6) - qt0;
-    }
-  }
-  const int n = nt * a.group;
-  // step j: query head hk group + j / nt, tile qt0 + j % nt; walked with a cursor
-  struct Step {
-    int h, t;
-    __device__ __forceinline__ void next(int end, int first) {
-      if (++t == end) { t = first; ++h; }
-    }
-  };
-  Step at{hk * a.group, qt0};
-  const int qt1 = qt0 + nt;
   const Waiter wait{abort_flag, a.err};
   const WaiterW<> waitw{abort_flag, a.err};
 
-  if (warp == kSoftWarps) {
-    if (lane == 0 && n > 0) {
-      mbar_arrive_expect_tx(kv_full, 4 * kTile);
-      for (int g = 0; g < 2; ++g) {
-        load_tile(sK + kTile * g, mk, kv_full, b, hk, k0 + 64 * g);
-        load_tile(sK + 2 * kTile + kTile * g, mv, kv_full, b, hk, k0 + 64 * g);
+  if (warp == kDkvWarps) {
+    const int nbh = a.B * a.Hkv, ktiles = (a.Sk + 127) / 128, nitems = nbh * ktiles;
+    int ni = 0, t = 0, L = blockIdx.x;      // items handed on, steps, the item's number
+    bool ok = true;
+    while (ok) {
+      DkvItem it;
+      it.n = -1;
+      if (L < nitems) {
+        const int bh = L % nbh;
+        it.b = bh / a.Hkv;
+        it.hk = bh % a.Hkv;
+        it.k0 = L / nbh * 128;
+        const SinkSeq s = sink_seq(a, it.b);
+        it.pos0 = s.pos0;
+        it.qn = s.qn;
+        it.kn = s.kn;
+        it.keys = min(128, s.kn - it.k0);
+        const int lo = max(0, it.k0 - a.right - s.pos0);
+        const int hi = it.k0 < a.sinks ? s.qn : min(s.qn, it.k0 + it.keys + a.left - s.pos0);
+        it.qt0 = lo >> 6;
+        it.qt1 = lo < hi ? (hi + 63) >> 6 : it.qt0;
+        it.n = it.keys > 0 ? (it.qt1 - it.qt0) * a.group : 0;
+        for (int i = lane; it.n == 0 && i < it.keys * 8; i += 32) {     // keys that no query sees
+          const long r = it.k0 + (i >> 3);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const SinkTensor& out = u ? a.dk : a.dv;
+            uint16_t* p = static_cast<uint16_t*>(out.p) + (long)it.b * out.sb + (long)it.hk * out.sh + r * out.ld + 8 * (i & 7);
+            *reinterpret_cast<uint4*>(p) = make_uint4(0u, 0u, 0u, 0u);
+          }
+        }
       }
-      for (int j = 0; j < n; ++j) {
-        const int st = j % kDkvStages;
-        if (j >= kDkvStages && !wait(&q_empty[st], (uint32_t)((j / kDkvStages) & 1) ^ 1u, kErrTimeoutEmpty)) break;
-        uint8_t* p = sQd + st * 2 * kTile;
-        mbar_arrive_expect_tx(&q_full[st], 2 * kTile);
-        load_tile(p, mq, &q_full[st], b, at.h, at.t * 64);
-        load_tile(p + kTile, mdo, &q_full[st], b, at.h, at.t * 64);
-        at.next(qt1, qt0);
+      if (it.n != 0 && lane == 0) {
+        const int slot = ni % kDkvItems, kb = ni & 1;
+        ok = ni < kDkvItems || wait(&item_empty[slot], (uint32_t)((ni / kDkvItems - 1) & 1), kErrTimeoutEmpty);
+        if (ok) {
+          items[slot] = it;
+          mbar_arrive(&item_full[slot]);
+          if (it.n > 0) ok = ni < 2 || wait(&kv_empty[kb], (uint32_t)((ni / 2 - 1) & 1), kErrTimeoutEmpty);
+        }
+        if (ok && it.n > 0) {
+          uint8_t* kv = sKV + 32768 * kb;
+          mbar_arrive_expect_tx(&kv_full[kb], 4 * kTile);
+          for (int g = 0; g < 2; ++g) {
+            load_tile(kv + kTile * g, mk, &kv_full[kb], it.b, it.hk, it.k0 + 64 * g);
+            load_tile(kv + 2 * kTile + kTile * g, mv, &kv_full[kb], it.b, it.hk, it.k0 + 64 * g);
+          }
+          for (int h = it.hk * a.group; h < (it.hk + 1) * a.group && ok; ++h)
+            for (int q = it.qt0; q < it.qt1; ++q, ++t) {
+              const int st = t % kDkvStages;
+              if (t >= kDkvStages && !wait(&q_empty[st], (uint32_t)((t / kDkvStages - 1) & 1), kErrTimeoutEmpty)) { ok = false; break; }
+              uint8_t* p = sQd + st * 2 * kTile;
+              mbar_arrive_expect_tx(&q_full[st], 2 * kTile);
+              load_tile(p, mq, &q_full[st], it.b, h, q * 64);
+              load_tile(p + kTile, mdo, &q_full[st], it.b, h, q * 64);
+            }
+        }
       }
+      if (it.n < 0) break;
+      if (it.n > 0) ++ni;
+      if (lane == 0) L = (int)gridDim.x + atomicAdd(a.next_item, 1);
+      L = __shfl_sync(0xffffffffu, L, 0);
+      ok = __shfl_sync(0xffffffffu, (int)ok, 0);
     }
-  } else if (warp == kSoftWarps + 1) {
+  } else if (warp == kDkvWarps + 1) {
     constexpr uint32_t id_s = sink_idesc<BF>(0), id_g = sink_idesc<BF>(1);
-    const uint64_t kd = kdesc0(smem_u32(sK)), vd = kdesc0(smem_u32(sK + 2 * kTile));
-    bool ok = n > 0 && waitw(kv_full, 0, kErrTimeoutFull);
-    auto grad = [&](int j) {     // dV += P^T dO, dK += dS^T Q of step j
-      if (!waitw(ds_full, (uint32_t)(j & 1), kErrTimeoutReady)) return false;
+    // Scores run up to three steps ahead of the gradients: `sc` and `gr` walk the same items.
+    struct Cursor {
+      int item = -1, left = 0, t = 0;      // the item (its number), its steps to come, the step
+    } sc, gr;
+    bool ok = true, more = true;
+    // the next item; false when there is none
+    auto advance = [&](Cursor& c) {
+      ++c.item;
+      if (!waitw(&item_full[c.item % kDkvItems], (uint32_t)((c.item / kDkvItems) & 1), kErrTimeoutOther)) { ok = false; return false; }
+      c.left = items[c.item % kDkvItems].n;
+      return c.left > 0;
+    };
+    auto scores = [&]() {        // S^T = K Q^T and dP^T = V dO^T
+      const int st = sc.t % kDkvStages, u = sc.t % 3, kb = sc.item & 1;
+      if (!waitw(&kv_full[kb], (uint32_t)((sc.item >> 1) & 1), kErrTimeoutFull)) return false;
+      if (!waitw(&q_full[st], (uint32_t)((sc.t / kDkvStages) & 1), kErrTimeoutFull)) return false;
       tc_fence_after();
-      const uint32_t qa = smem_u32(sQd + (j % kDkvStages) * 2 * kTile);
-      const uint64_t qmn = mndesc0(qa), dmn = mndesc0(qa + kTile);
+      const uint32_t qa = smem_u32(sQd + st * 2 * kTile), ka = smem_u32(sKV + 32768 * kb), tS = tbase + 128 * u;
+      const uint64_t qd = kdesc0(qa), dd = kdesc0(qa + kTile), kd = kdesc0(ka), vd = kdesc0(ka + 2 * kTile);
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk)
-        umma_ts_w(tbase + 128, tbase + 32 * (kk >> 1) + 8 * (kk & 1), mnstep(dmn, kk), id_g, (j > 0 || kk > 0) ? 1u : 0u);
+      for (int kk = 0; kk < 4; ++kk) umma_f16_w(tS, kstep(kd, kk), kstep(qd, kk), id_s, kk > 0 ? 1u : 0u);
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk)
-        umma_ts_w(tbase + 192, tbase + 64 + 32 * (kk >> 1) + 8 * (kk & 1), mnstep(qmn, kk), id_g, (j > 0 || kk > 0) ? 1u : 0u);
-      umma_commit_w(&q_empty[j % kDkvStages]);
+      for (int kk = 0; kk < 4; ++kk) umma_f16_w(tS + 64, kstep(vd, kk), kstep(dd, kk), id_s, kk > 0 ? 1u : 0u);
+      umma_commit_w(&s_full[u]);
+      ++sc.t;
+      if (--sc.left == 0) umma_commit_w(&kv_empty[kb]);
       return true;
     };
-    for (int j = 0; j < n && ok; ++j) {
-      const int st = j % kDkvStages;
-      if (!waitw(&q_full[st], (uint32_t)((j / kDkvStages) & 1), kErrTimeoutFull)) { ok = false; break; }
-      if (j > 0 && !(ok = grad(j - 1))) break;
+    while (ok) {
+      while (ok && more && sc.t - gr.t < 3) {
+        if (sc.left == 0) more = advance(sc);
+        if (more && ok) ok = scores();
+      }
+      if (!ok || gr.t == sc.t) break;
+      const bool first = gr.left == 0;
+      if (first) {
+        if (gr.item >= 0 && lane == 0) mbar_arrive(&item_empty[gr.item % kDkvItems]);
+        if (!advance(gr)) break;
+      }
+      const int st = gr.t % kDkvStages, u = gr.t % 3;
+      if (!waitw(&ds_full[u], (uint32_t)((gr.t / 3) & 1), kErrTimeoutReady)) break;
+      if (first && gr.item > 0 && !waitw(acc_empty, (uint32_t)((gr.item - 1) & 1), kErrTimeoutOther)) break;
       tc_fence_after();
-      const uint32_t qa = smem_u32(sQd + st * 2 * kTile);
-      const uint64_t qd = kdesc0(qa), dd = kdesc0(qa + kTile);
+      const uint32_t qa = smem_u32(sQd + st * 2 * kTile), tS = tbase + 128 * u;
+      const uint64_t qmn = mndesc0(qa), dmn = mndesc0(qa + kTile);
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk) umma_f16_w(tbase, kstep(kd, kk), kstep(qd, kk), id_s, kk > 0 ? 1u : 0u);
+      for (int kk = 0; kk < 4; ++kk)     // dV += P^T dO
+        umma_ts_w(tbase + 384, tS + 32 * (kk >> 1) + 8 * (kk & 1), mnstep(dmn, kk), id_g, (!first || kk > 0) ? 1u : 0u);
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk) umma_f16_w(tbase + 64, kstep(vd, kk), kstep(dd, kk), id_s, kk > 0 ? 1u : 0u);
-      umma_commit_w(s_full);
+      for (int kk = 0; kk < 4; ++kk)     // dK += dS^T Q
+        umma_ts_w(tbase + 448, tS + 64 + 32 * (kk >> 1) + 8 * (kk & 1), mnstep(qmn, kk), id_g, (!first || kk > 0) ? 1u : 0u);
+      umma_commit_w(&q_empty[st]);
+      ++gr.t;
+      if (--gr.left == 0) umma_commit_w(acc_full);
     }
-    if (ok) ok = grad(n - 1);
-    if (ok) umma_commit_w(acc_full);
-  } else if (keys > 0) {
-    const int g = warp >> 2, quarter = warp & 3, row = 32 * quarter + lane, kj = k0 + row;
-    const int t = (int)threadIdx.x & 127;       // within the warpgroup
+  } else {
+    const int set = warp >> 3, g = (warp >> 2) & 1, wg = warp >> 2, quarter = warp & 3, row = 32 * quarter + lane;
     const uint32_t lane_off = (uint32_t)(32 * quarter) << 16;
-    const uint32_t tS = tbase + lane_off + 32 * g, tP = tS + 64;
-    // thread t < 32 fetches the lse of the group's column t one step ahead, 32 <= t < 64 the D
-    auto fetch = [&](const Step& x) -> float {
-      const int i = x.t * 64 + 32 * g + (t & 31);
-      if (i >= s.qn) return t < 32 ? INFINITY : 0.f;
-      const long r = ((long)b * a.H + x.h) * a.Sq + i;
-      if (t >= 32) return a.D[r];
-      const float v = a.lse[r];
-      return v == -INFINITY ? INFINITY : v;
-    };
     const uint64_t sc2 = f2(a.sl2, a.sl2);
+    uint8_t* stg = sOut + warp * 2048;
+    float* ldb = s_ld + 64 * warp;
     bool ok = true;
-    float next = n > 0 && t < 64 ? fetch(at) : 0.f;
-    for (int j = 0; j < n; ++j) {
-      const int q0 = at.t * 64, pq = s.pos0 + q0;
-      at.next(qt1, qt0);
-      float* ldb = s_ld + 128 * g + 64 * (j & 1);
-      if (t < 64) {
-        ldb[4 * ((t & 31) >> 1) + (t >= 32 ? 2 : 0) + (t & 1)] = next;
-        if (j + 1 < n) next = fetch(at);
-      }
-      if (g == 0) named_bar(1, 128);   // (every warp of the group passes it once per step, also after an abort)
-      else named_bar(2, 128);
-      if (ok) ok = waitw(s_full, (uint32_t)(j & 1), kErrTimeoutAccum);
-      if (!ok) continue;
-      tc_fence_after();
-      // queries of the tile that see key kj: position from kj - right to kj + left (any, for a sink)
-      const bool edge = q0 + 64 > s.qn || k0 + 128 > s.kn || k0 + 127 > pq + a.right ||
-                        !(k0 + 127 < a.sinks || k0 >= pq + 63 - a.left);
-      uint32_t mask = 0xffffffffu;
-      if (edge) {
-        uint64_t m = low_bits(s.qn - q0) & ~low_bits(kj - a.right - pq);
-        if (kj >= a.sinks) m &= low_bits(kj + a.left - pq + 1);
-        mask = kj < s.kn ? (uint32_t)(m >> (32 * g)) : 0u;
-      }
-      const float4* ld4 = reinterpret_cast<const float4*>(ldb);
-#pragma unroll 1
-      for (int hf = 0; hf < 2; ++hf) {
-        uint32_t sv[16], pv[16], pk[8], dk[8];
-        tmem_ld16(tS + 16 * hf, sv);
-        tmem_ld16(tP + 16 * hf, pv);
-        tmem_ld_wait();
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float4 w4 = ld4[8 * hf + e];     // lse and D of two queries, one broadcast read
-          float x0, x1, d0, d1;
-          f2split(ffma2(f2(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), sc2, f2(-w4.x, -w4.y)), x0, x1);
-          float p0 = ex2(x0), p1 = ex2(x1);
-          f2split(fmul2(f2(p0, p1), fadd2(f2(__uint_as_float(pv[2 * e]), __uint_as_float(pv[2 * e + 1])), f2(-w4.z, -w4.w))),
-                  d0, d1);
-          if (edge) {
-            const uint32_t mm = mask >> (16 * hf);
-            if (!((mm >> (2 * e)) & 1u)) p0 = d0 = 0.f;
-            if (!((mm >> (2 * e + 1)) & 1u)) p1 = d1 = 0.f;
-          }
-          pk[e] = pack2<BF>(p0, p1);
-          dk[e] = pack2<BF>(d0, d1);
+    int t0 = 0;                                 // the item's first step
+    for (int item = 0; ok; ++item) {
+      if (!waitw(&item_full[item % kDkvItems], (uint32_t)((item / kDkvItems) & 1), kErrTimeoutOther)) break;
+      const DkvItem& it = items[item % kDkvItems];
+      if (it.n < 0) break;
+      const int kj = it.k0 + row;
+      // lane c holds the lse and the D of the group's column c, fetched one of the set's steps ahead
+      auto fetch = [&](int h, int q) {
+        const int i = q * 64 + 32 * g + lane;
+        float2 v = make_float2(INFINITY, 0.f);
+        if (i < it.qn) {
+          const long r = ((long)it.b * a.H + h) * a.Sq + i;
+          v = make_float2(a.lse[r], a.D[r]);
+          if (v.x == -INFINITY) v.x = INFINITY;      // a row that sees nothing: P = 0
         }
-        tmem_st8(tS + 8 * hf, pk);      // (over the columns that this thread has read)
-        tmem_st8(tP + 8 * hf, dk);
-      }
-      if (q0 + 64 > s.qn && s.qn < a.Sq) {   // query rows behind the sequence's end
-        const int st = j % kDkvStages;
-        if (waitw(&q_full[st], (uint32_t)((j / kDkvStages) & 1), kErrTimeoutFull)) {
-          zero_rows(sQd + st * 2 * kTile, s.qn - q0, (int)threadIdx.x, 32 * kSoftWarps);
-          zero_rows(sQd + st * 2 * kTile + kTile, s.qn - q0, (int)threadIdx.x, 32 * kSoftWarps);
+        return v;
+      };
+      int j = (t0 & 1) == set ? 0 : 1;          // the set's first step of the item
+      int h = it.hk * a.group, q = it.qt0 + j;
+      auto wrap = [&]() {
+        while (q >= it.qt1) {
+          q -= it.qt1 - it.qt0;
+          ++h;
+        }
+      };
+      wrap();
+      float2 next = j < it.n ? fetch(h, q) : make_float2(0.f, 0.f);
+      for (; j < it.n && ok; j += 2) {
+        const int t = t0 + j, u = t % 3, q0 = q * 64, pq = it.pos0 + q0;
+        __syncwarp();                            // the step before's values have been read
+        ldb[4 * (lane >> 1) + (lane & 1)] = next.x;
+        ldb[4 * (lane >> 1) + 2 + (lane & 1)] = next.y;
+        q += 2;
+        wrap();
+        if (j + 2 < it.n) next = fetch(h, q);
+        __syncwarp();
+        if (!waitw(&s_full[u], (uint32_t)((t / 3) & 1), kErrTimeoutAccum)) { ok = false; break; }
+        tc_fence_after();
+        // queries of the tile that see key kj: position from kj - right to kj + left (any, for a sink)
+        const bool edge = q0 + 64 > it.qn || it.k0 + 128 > it.kn || it.k0 + 127 > pq + a.right ||
+                          !(it.k0 + 127 < a.sinks || it.k0 >= pq + 63 - a.left);
+        uint32_t mask = 0xffffffffu;
+        if (edge) {
+          uint64_t m = low_bits(it.qn - q0) & ~low_bits(kj - a.right - pq);
+          if (kj >= a.sinks) m &= low_bits(kj + a.left - pq + 1);
+          mask = kj < it.kn ? (uint32_t)(m >> (32 * g)) : 0u;
+        }
+        const bool some = edge && __any_sync(0xffffffffu, mask != 0xffffffffu);
+        const float4* ld4 = reinterpret_cast<const float4*>(ldb);
+        const uint32_t tS = tbase + 128 * u + lane_off + 32 * g, tP = tS + 64;
+#pragma unroll 1
+        for (int hf = 0; hf < 2; ++hf) {
+          uint32_t sv[16], pv[16], pk[8], dk[8];
+          tmem_ld16(tS + 16 * hf, sv);
+          tmem_ld16(tP + 16 * hf, pv);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float4 w4 = ld4[8 * hf + e];     // lse and D of two queries, one broadcast read
+            float x0, x1, d0, d1;
+            f2split(ffma2(f2(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), sc2, f2(-w4.x, -w4.y)), x0, x1);
+            float p0 = ex2(x0), p1 = ex2(x1);
+            f2split(fmul2(f2(p0, p1), fadd2(f2(__uint_as_float(pv[2 * e]), __uint_as_float(pv[2 * e + 1])), f2(-w4.z, -w4.w))),
+                    d0, d1);
+            if (some) {
+              const uint32_t mm = mask >> (16 * hf);
+              if (!((mm >> (2 * e)) & 1u)) p0 = d0 = 0.f;
+              if (!((mm >> (2 * e + 1)) & 1u)) p1 = d1 = 0.f;
+            }
+            pk[e] = pack2<BF>(p0, p1);
+            dk[e] = pack2<BF>(d0, d1);
+          }
+          tmem_st8(tS + 8 * hf, pk);      // (over the columns that this thread has read)
+          tmem_st8(tP + 8 * hf, dk);
+        }
+        if (q0 + 64 > it.qn && it.qn < a.Sq) {   // query rows behind the sequence's end
+          const int st = t % kDkvStages;
+          if (!waitw(&q_full[st], (uint32_t)((t / kDkvStages) & 1), kErrTimeoutFull)) { ok = false; break; }
+          zero_rows(sQd + st * 2 * kTile, it.qn - q0, (int)threadIdx.x & 255, 256);
+          zero_rows(sQd + st * 2 * kTile + kTile, it.qn - q0, (int)threadIdx.x & 255, 256);
           fence_proxy_async_smem();
         }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ds_full[u]);
       }
-      tmem_st_wait();
+      // the item's results: warpgroups 0, 1 take dV's columns 32 wg .., 2, 3 dK's
+      if (!ok || !waitw(acc_full, (uint32_t)(item & 1), kErrTimeoutAccum)) break;
+      t0 += it.n;
+      tc_fence_after();
+      uint32_t o[32];
+      tmem_ld32(tbase + 384 + 32 * wg + lane_off, o);
+      tmem_ld_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(ds_full);
-    }
-    const bool have = ok && n > 0 && waitw(acc_full, 0, kErrTimeoutAccum);
-    tc_fence_after();
-    uint32_t o[64];
-    if (have) {       // warpgroup 0 writes dV, warpgroup 1 dK
-      tmem_ld32(tbase + lane_off + 128 + 64 * g, *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
-      tmem_ld32(tbase + lane_off + 160 + 64 * g, *reinterpret_cast<uint32_t(*)[32]>(&o[32]));
-      tmem_ld_wait();
-    }
-    if (ok && (have || n == 0)) {
-      const SinkTensor& out = g == 0 ? a.dv : a.dk;
-      const float mul = g == 0 ? 1.f : a.scale;
-      uint4 w[8];
+      if (lane == 0) mbar_arrive(acc_empty);
+      const SinkTensor& out = wg < 2 ? a.dv : a.dk;
+      const float mul = wg < 2 ? 1.f : a.scale;
+      uint4 w[4];
 #pragma unroll
-      for (int q = 0; q < 8; ++q) {
+      for (int c = 0; c < 4; ++c) {
         uint32_t x[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          x[e] = n == 0 ? 0u : pack2<BF>(__uint_as_float(o[8 * q + 2 * e]) * mul, __uint_as_float(o[8 * q + 2 * e + 1]) * mul);
-        w[q] = make_uint4(x[0], x[1], x[2], x[3]);
+        for (int e = 0; e < 4; ++e) x[e] = pack2<BF>(__uint_as_float(o[8 * c + 2 * e]) * mul, __uint_as_float(o[8 * c + 2 * e + 1]) * mul);
+        w[c] = make_uint4(x[0], x[1], x[2], x[3]);
       }
-      // (the products have read K and V)
-      store_rows<8>(sK + 4096 * warp, w,
-                    static_cast<uint16_t*>(out.p) + (long)b * out.sb + (long)hk * out.sh + (long)(k0 + 32 * quarter) * out.ld, out.ld,
-                    keys - 32 * quarter, lane);
+      store_rows<4, 64>(stg, w,
+                        static_cast<uint16_t*>(out.p) + (long)it.b * out.sb + (long)it.hk * out.sh +
+                            (long)(it.k0 + 32 * quarter) * out.ld + 32 * (wg & 1),
+                        out.ld, it.keys - 32 * quarter, lane);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[item % kDkvItems]);
     }
   }
   __syncthreads();
-  if (warp == kSoftWarps + 1) {
+  if (warp == kDkvWarps + 1) {
     tc_fence_after();
-    tmem_dealloc(tbase, 256);
+    tmem_dealloc(tbase, 512);
   }
 }
 
@@ -926,9 +1020,11 @@ int backward(Ctx* c, const SinkArgs& a, std::string& err) {
   if (!a.dk.p || nokeys) return 0;
   auto kern = sink_dkdv_kernel<BF>;
   if (smem_attr(reinterpret_cast<const void*>(kern), kDkvSmem, c->device, "attention_sink smem attribute", err)) return 1;
+  if (noq && cudaMemsetAsync(a.next_item, 0, sizeof(int), c->stream) != cudaSuccess) return check_launch("attention_sink memset", err);
+  const long items = (long)a.B * a.Hkv * ((a.Sk + 127) / 128);
   ProfScope prof_(c, "attn_sink.dkdv");
-  launch_pdl(c, kern, dim3((unsigned)((long)a.B * a.Hkv * ((a.Sk + 127) / 128))), dim3(kSinkThreads), (size_t)kDkvSmem,
-             mk, mv, mq, mdo, a);
+  launch_pdl(c, kern, dim3((unsigned)std::min<long>(items, (long)c->sm_count)), dim3(kDkvThreads), (size_t)kDkvSmem, mk, mv, mq,
+             mdo, a);
   return check_launch("attention with sinks, dk / dv", err);
 }
 
@@ -1043,8 +1139,11 @@ int sa3k_attention_sink_bwd(sa3k_ctx* ctx, const sa3k_sink_attn* p, const sa3k_t
         return 1;
     }
     a.lse = const_cast<float*>(lse);
-    a.D = static_cast<float*>(scratch_get(c, kSlotSinkD, (size_t)std::max<long>(1, (long)a.B * a.H * a.Sq) * sizeof(float), e));
-    if (!a.D) return 1;
+    // scratch: the item counter | D
+    char* mem = static_cast<char*>(scratch_get(c, kSlotSinkD, 256 + (size_t)a.B * a.H * a.Sq * sizeof(float), e));
+    if (!mem) return 1;
+    a.next_item = reinterpret_cast<int*>(mem);
+    a.D = reinterpret_cast<float*>(mem + 256);
     return p->type == kTypeF16 ? backward<false>(c, a, e) : backward<true>(c, a, e);
   });
 }

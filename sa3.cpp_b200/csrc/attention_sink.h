@@ -23,6 +23,7 @@ struct SinkArgs {
   SinkTensor q, k, v, o, dO, dq, dk, dv;
   float* lse;                      // [B][H][Sq], log2 units
   float* D;                        // backward scratch [B][H][Sq]: rowsum(dO o O)
+  int* next_item;                  // backward scratch: the dk / dv pass's work counter, zeroed by the dq pass
   int* err;
 };
 
