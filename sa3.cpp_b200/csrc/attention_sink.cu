@@ -10,6 +10,7 @@
 #include "attention_sink.h"
 
 #include <algorithm>
+#include <climits>
 #include <cmath>
 
 #include "../../include/sa3k.h"
@@ -111,9 +112,9 @@ __device__ __forceinline__ KeyTiles key_tiles(const SinkArgs& a, const SinkSeq& 
   KeyTiles k{0, 0, 0};
   const int hi = min(s.kn, phi + a.right + 1);
   if (hi <= 0 || phi < plo) return k;
-  k.ns = (min(a.sinks, hi) + 63) >> 6;
-  k.w0 = max(max(0, plo - a.left) >> 6, k.ns);
-  k.n = k.ns + max(0, ((hi + 63) >> 6) - k.w0);
+  k.ns = uniform((min(a.sinks, hi) + 63) >> 6);
+  k.w0 = uniform(max(max(0, plo - a.left) >> 6, k.ns));
+  k.n = uniform(k.ns + max(0, ((hi + 63) >> 6) - k.w0));
   return k;
 }
 
@@ -188,7 +189,7 @@ __global__ void __launch_bounds__(kFwdThreads, 3)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 9);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 128) {
     mbar_init(q_full, 1);
     for (int i = 0; i < 2; ++i) {
@@ -213,7 +214,7 @@ __global__ void __launch_bounds__(kFwdThreads, 3)
   }
   __syncthreads();
   tc_fence_after();
-  const uint32_t tbase = *tmem_slot;
+  const uint32_t tbase = (uint32_t)uniform((int)*tmem_slot);
   pdl_wait();
 
   const int bh = blockIdx.y, b = bh / a.H, h = bh % a.H, r0 = blockIdx.x * 128;
@@ -238,8 +239,7 @@ __global__ void __launch_bounds__(kFwdThreads, 3)
       if (!waitw(&k_full[c & 1], (uint32_t)((c >> 1) & 1), kErrTimeoutFull)) return false;
       tc_fence_after();
       const uint64_t k = kd + (c & 1) * kSlot;
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk) umma_f16_w(tbase, kstep(qd, kk), kstep(k, kk), id_s, kk > 0 ? 1u : 0u);
+      umma4_ss_w<2, 2>(tbase, qd, k, id_s, 0u);
       umma_commit_w(s_full);
       return true;
     };
@@ -264,8 +264,7 @@ __global__ void __launch_bounds__(kFwdThreads, 3)
       if (!waitw(&v_full[c & 1], (uint32_t)((c >> 1) & 1), kErrTimeoutFull)) break;
       tc_fence_after();
       const uint64_t v = vd + (c & 1) * kSlot;
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk) umma_f16_w(tbase + 64, kstep(pd, kk), mnstep(v, kk), id_o, (c > 0 || kk > 0) ? 1u : 0u);
+      umma4_ss_w<2, 128>(tbase + 64, pd, v, id_o, c > 0 ? 1u : 0u);
       umma_commit_w(pv_done);
       if (c > 0 && c + 1 < kt.n) load(sV, mv, &v_full[(c + 1) & 1], c + 1);       // (P V(c - 1) had read its V at p_full)
     }
@@ -424,7 +423,7 @@ __global__ void __launch_bounds__(kSinkThreads, 2)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (warp == kSoftWarps && lane == 0) {
     mbar_init(q_full, 1);
     for (int s = 0; s < kDqStages; ++s) {
@@ -453,7 +452,7 @@ __global__ void __launch_bounds__(kSinkThreads, 2)
   }
   __syncthreads();
   tc_fence_after();
-  const uint32_t tbase = *tmem_slot;
+  const uint32_t tbase = (uint32_t)uniform((int)*tmem_slot);
   pdl_wait();
 
   if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.next_item = 0;     // for the dk / dv pass
@@ -489,9 +488,7 @@ __global__ void __launch_bounds__(kSinkThreads, 2)
       if (!waitw(&ds_full[j & 1], (uint32_t)((j >> 1) & 1), kErrTimeoutReady)) return false;
       tc_fence_after();
       const uint64_t kmn = mndesc0(smem_u32(sKV + (j % kDqStages) * 2 * kTile));
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk)
-        umma_ts_w(tbase + 128, tbase + 192 + 32 * (j & 1) + kk * 8, mnstep(kmn, kk), id_g, (j > 0 || kk > 0) ? 1u : 0u);
+      umma4_ts_w<16, 128>(tbase + 128, tbase + 192 + 32 * (j & 1), kmn, id_g, j > 0 ? 1u : 0u);
       umma_commit_w(&ds_free[j & 1]);
       umma_commit_w(&kv_empty[j % kDqStages]);
       return true;
@@ -502,10 +499,8 @@ __global__ void __launch_bounds__(kSinkThreads, 2)
       if (j > 0 && !waitw(s_read, (uint32_t)((j - 1) & 1), kErrTimeoutOther)) { ok = false; break; }
       tc_fence_after();
       const uint64_t kd = kdesc0(smem_u32(sKV + st * 2 * kTile)), vd = kdesc0(smem_u32(sKV + st * 2 * kTile + kTile));
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk) umma_f16_w(tbase, kstep(qd, kk), kstep(kd, kk), id_s, kk > 0 ? 1u : 0u);
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk) umma_f16_w(tbase + 64, kstep(dd, kk), kstep(vd, kk), id_s, kk > 0 ? 1u : 0u);
+      umma4_ss_w<2, 2>(tbase, qd, kd, id_s, 0u);
+      umma4_ss_w<2, 2>(tbase + 64, dd, vd, id_s, 0u);
       umma_commit_w(s_full);
       if (j > 0) ok = grad(j - 1);
     }
@@ -656,7 +651,7 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(item_empty + kDkvItems);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (warp == kDkvWarps && lane == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&kv_full[i], 1);
@@ -690,7 +685,7 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
   }
   __syncthreads();
   tc_fence_after();
-  const uint32_t tbase = *tmem_slot;
+  const uint32_t tbase = (uint32_t)uniform((int)*tmem_slot);
   pdl_wait();
   const Waiter wait{abort_flag, a.err};
   const WaiterW<> waitw{abort_flag, a.err};
@@ -770,7 +765,7 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
     auto advance = [&](Cursor& c) {
       ++c.item;
       if (!waitw(&item_full[c.item % kDkvItems], (uint32_t)((c.item / kDkvItems) & 1), kErrTimeoutOther)) { ok = false; return false; }
-      c.left = items[c.item % kDkvItems].n;
+      c.left = uniform(items[c.item % kDkvItems].n);
       return c.left > 0;
     };
     auto scores = [&]() {        // S^T = K Q^T and dP^T = V dO^T
@@ -780,10 +775,8 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
       tc_fence_after();
       const uint32_t qa = smem_u32(sQd + st * 2 * kTile), ka = smem_u32(sKV + 32768 * kb), tS = tbase + 128 * u;
       const uint64_t qd = kdesc0(qa), dd = kdesc0(qa + kTile), kd = kdesc0(ka), vd = kdesc0(ka + 2 * kTile);
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk) umma_f16_w(tS, kstep(kd, kk), kstep(qd, kk), id_s, kk > 0 ? 1u : 0u);
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk) umma_f16_w(tS + 64, kstep(vd, kk), kstep(dd, kk), id_s, kk > 0 ? 1u : 0u);
+      umma4_ss_w<2, 2>(tS, kd, qd, id_s, 0u);
+      umma4_ss_w<2, 2>(tS + 64, vd, dd, id_s, 0u);
       umma_commit_w(&s_full[u]);
       ++sc.t;
       if (--sc.left == 0) umma_commit_w(&kv_empty[kb]);
@@ -806,12 +799,8 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
       tc_fence_after();
       const uint32_t qa = smem_u32(sQd + st * 2 * kTile), tS = tbase + 128 * u;
       const uint64_t qmn = mndesc0(qa), dmn = mndesc0(qa + kTile);
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk)     // dV += P^T dO
-        umma_ts_w(tbase + 384, tS + 32 * (kk >> 1) + 8 * (kk & 1), mnstep(dmn, kk), id_g, (!first || kk > 0) ? 1u : 0u);
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk)     // dK += dS^T Q
-        umma_ts_w(tbase + 448, tS + 64 + 32 * (kk >> 1) + 8 * (kk & 1), mnstep(qmn, kk), id_g, (!first || kk > 0) ? 1u : 0u);
+      umma4_ts_w<32, 128>(tbase + 384, tS, dmn, id_g, first ? 0u : 1u);             // dV += P^T dO
+      umma4_ts_w<32, 128>(tbase + 448, tS + 64, qmn, id_g, first ? 0u : 1u);        // dK += dS^T Q
       umma_commit_w(&q_empty[st]);
       ++gr.t;
       if (--gr.left == 0) umma_commit_w(acc_full);
@@ -828,47 +817,48 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
       if (!waitw(&item_full[item % kDkvItems], (uint32_t)((item / kDkvItems) & 1), kErrTimeoutOther)) break;
       const DkvItem& it = items[item % kDkvItems];
       if (it.n < 0) break;
-      const int kj = it.k0 + row;
+      const int k0 = it.k0, kj = k0 + row, qn = it.qn, pos0 = it.pos0, n = it.n, qt0 = it.qt0, qt1 = it.qt1;
+      // rows of the item and their window: query tiles at positions [e0, e1) see every key of the item
+      const bool whole = k0 + 128 <= it.kn, inside = kj < it.kn;
+      const int e0 = k0 + 127 - a.right, e1 = k0 + 127 < a.sinks ? INT_MAX : k0 + a.left - 62;
       // lane c holds the lse and the D of the group's column c, fetched one of the set's steps ahead
       auto fetch = [&](int h, int q) {
         const int i = q * 64 + 32 * g + lane;
         float2 v = make_float2(INFINITY, 0.f);
-        if (i < it.qn) {
+        if (i < qn) {
           const long r = ((long)it.b * a.H + h) * a.Sq + i;
-          v = make_float2(a.lse[r], a.D[r]);
-          if (v.x == -INFINITY) v.x = INFINITY;      // a row that sees nothing: P = 0
+          v = make_float2(a.lse[r], a.D[r]);        // (not looked at before its step: the loads stay in flight)
         }
         return v;
       };
       int j = (t0 & 1) == set ? 0 : 1;          // the set's first step of the item
-      int h = it.hk * a.group, q = it.qt0 + j;
+      int h = it.hk * a.group, q = qt0 + j;
       auto wrap = [&]() {
-        while (q >= it.qt1) {
-          q -= it.qt1 - it.qt0;
+        while (q >= qt1) {
+          q -= qt1 - qt0;
           ++h;
         }
       };
       wrap();
-      float2 next = j < it.n ? fetch(h, q) : make_float2(0.f, 0.f);
-      for (; j < it.n && ok; j += 2) {
-        const int t = t0 + j, u = t % 3, q0 = q * 64, pq = it.pos0 + q0;
+      float2 next = j < n ? fetch(h, q) : make_float2(0.f, 0.f);
+      for (; j < n && ok; j += 2) {
+        const int t = t0 + j, u = t % 3, q0 = q * 64, pq = pos0 + q0;
         __syncwarp();                            // the step before's values have been read
-        ldb[4 * (lane >> 1) + (lane & 1)] = next.x;
+        ldb[4 * (lane >> 1) + (lane & 1)] = next.x == -INFINITY ? INFINITY : next.x;      // a row that sees nothing: P = 0
         ldb[4 * (lane >> 1) + 2 + (lane & 1)] = next.y;
         q += 2;
         wrap();
-        if (j + 2 < it.n) next = fetch(h, q);
+        if (j + 2 < n) next = fetch(h, q);
         __syncwarp();
         if (!waitw(&s_full[u], (uint32_t)((t / 3) & 1), kErrTimeoutAccum)) { ok = false; break; }
         tc_fence_after();
         // queries of the tile that see key kj: position from kj - right to kj + left (any, for a sink)
-        const bool edge = q0 + 64 > it.qn || it.k0 + 128 > it.kn || it.k0 + 127 > pq + a.right ||
-                          !(it.k0 + 127 < a.sinks || it.k0 >= pq + 63 - a.left);
+        const bool edge = !whole || q0 + 64 > qn || pq < e0 || pq >= e1;
         uint32_t mask = 0xffffffffu;
         if (edge) {
-          uint64_t m = low_bits(it.qn - q0) & ~low_bits(kj - a.right - pq);
+          uint64_t m = low_bits(qn - q0) & ~low_bits(kj - a.right - pq);
           if (kj >= a.sinks) m &= low_bits(kj + a.left - pq + 1);
-          mask = kj < it.kn ? (uint32_t)(m >> (32 * g)) : 0u;
+          mask = inside ? (uint32_t)(m >> (32 * g)) : 0u;
         }
         const bool some = edge && __any_sync(0xffffffffu, mask != 0xffffffffu);
         const float4* ld4 = reinterpret_cast<const float4*>(ldb);
@@ -898,11 +888,11 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
           tmem_st8(tS + 8 * hf, pk);      // (over the columns that this thread has read)
           tmem_st8(tP + 8 * hf, dk);
         }
-        if (q0 + 64 > it.qn && it.qn < a.Sq) {   // query rows behind the sequence's end
+        if (q0 + 64 > qn && qn < a.Sq) {   // query rows behind the sequence's end
           const int st = t % kDkvStages;
           if (!waitw(&q_full[st], (uint32_t)((t / kDkvStages) & 1), kErrTimeoutFull)) { ok = false; break; }
-          zero_rows(sQd + st * 2 * kTile, it.qn - q0, (int)threadIdx.x & 255, 256);
-          zero_rows(sQd + st * 2 * kTile + kTile, it.qn - q0, (int)threadIdx.x & 255, 256);
+          zero_rows(sQd + st * 2 * kTile, qn - q0, (int)threadIdx.x & 255, 256);
+          zero_rows(sQd + st * 2 * kTile + kTile, qn - q0, (int)threadIdx.x & 255, 256);
           fence_proxy_async_smem();
         }
         tmem_st_wait();
@@ -912,7 +902,7 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
       }
       // the item's results: warpgroups 0, 1 take dV's columns 32 wg .., 2, 3 dK's
       if (!ok || !waitw(acc_full, (uint32_t)(item & 1), kErrTimeoutAccum)) break;
-      t0 += it.n;
+      t0 += n;
       tc_fence_after();
       uint32_t o[32];
       tmem_ld32(tbase + 384 + 32 * wg + lane_off, o);

@@ -85,4 +85,46 @@ struct Waiter {
   }
 };
 
+// Four k-steps of one product, issued warp-wide by one elected lane: the operands advance inside, so an
+// MMA costs the warp a few instructions (issued one by one, with softmax warps on the same scheduler,
+// the issue was slower than the tensor core).  D = A B for acc 0, D += A B otherwise; AS, BS: steps of
+// the descriptors per k-step.
+template <int AS, int BS>
+__device__ __forceinline__ void umma4_ss_w(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, t, e;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
+      "add.s64 a1, %1, %5;\n\tadd.s64 b1, %2, %6;\n\t"
+      "add.s64 a2, a1, %5;\n\tadd.s64 b2, b1, %6;\n\t"
+      "add.s64 a3, a2, %5;\n\tadd.s64 b3, b2, %6;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, t;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, t;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, t;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc), "n"(AS), "n"(BS)
+      : "memory");
+}
+
+// The same with A in tensor memory (packed 16-bit pairs): k-steps at a, a + 8, a + HALF, a + HALF + 8.
+template <int HALF, int BS>
+__device__ __forceinline__ void umma4_ts_w(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, t, e;\n\t.reg .b32 a1, a2, a3;\n\t.reg .b64 b1, b2, b3;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
+      "add.s32 a1, %1, 8;\n\tadd.s64 b1, %2, %6;\n\t"
+      "add.s32 a2, %1, %5;\n\tadd.s64 b2, b1, %6;\n\t"
+      "add.s32 a3, a2, 8;\n\tadd.s64 b3, b2, %6;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, t;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, t;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, t;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc), "n"(HALF), "n"(BS)
+      : "memory");
+}
+
+// A value that is the same in every lane, for the compiler to know it too (uniform registers).
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+
 }  // namespace sa3k
