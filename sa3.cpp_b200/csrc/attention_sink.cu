@@ -618,7 +618,7 @@ __global__ void __launch_bounds__(kSinkThreads, 2)
 // first 16 columns of their own halves); dV at 384, dK at 448.
 // smem: 2 x (K 16 KB, V 16 KB) | 6 x (Q 8 KB, dO 8 KB) | 16 x 2 KB output rows | 16 x lse, D | items | barriers
 constexpr int kDkvSets = 2, kDkvStages = 6, kDkvItems = 4;
-constexpr int kDkvWarps = 8 * kDkvSets, kDkvThreads = 32 * (kDkvWarps + 2);
+constexpr int kDkvWarps = 8 * kDkvSets, kDkvThreads = 32 * (kDkvWarps + 3);
 constexpr int kDkvSmem = 65536 + kDkvStages * 2 * kTile + kDkvWarps * (2048 + 256) + 256 + 512 + 1024;
 
 struct DkvItem {      // n > 0 steps: query tiles [qt0, qt1) of each of the group's heads; n < 0: no more items
@@ -644,7 +644,8 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
   uint64_t* q_empty = q_full + kDkvStages;              // dV and dK of the slot's tile are done
   uint64_t* s_full = q_empty + kDkvStages;              // [3]
   uint64_t* ds_full = s_full + 3;                       // [3]
-  uint64_t* acc_full = ds_full + 3;
+  uint64_t* g_done = ds_full + 3;                       // [3] dV and dK of the buffer's step are done
+  uint64_t* acc_full = g_done + 3;
   uint64_t* acc_empty = acc_full + 1;
   uint64_t* item_full = acc_empty + 1;                  // [kDkvItems]
   uint64_t* item_empty = item_full + kDkvItems;
@@ -664,12 +665,13 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
     for (int i = 0; i < 3; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&ds_full[i], 8);
+      mbar_init(&g_done[i], 1);
     }
     mbar_init(acc_full, 1);
     mbar_init(acc_empty, kDkvWarps);
     for (int i = 0; i < kDkvItems; ++i) {
       mbar_init(&item_full[i], 1);
-      mbar_init(&item_empty[i], kDkvWarps + 1);
+      mbar_init(&item_empty[i], kDkvWarps + 2);
     }
     *abort_flag = 0;
     fence_barrier_init();
@@ -754,56 +756,56 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
       L = __shfl_sync(0xffffffffu, L, 0);
       ok = __shfl_sync(0xffffffffu, (int)ok, 0);
     }
-  } else if (warp == kDkvWarps + 1) {
-    constexpr uint32_t id_s = sink_idesc<BF>(0), id_g = sink_idesc<BF>(1);
-    // Scores run up to three steps ahead of the gradients: `sc` and `gr` walk the same items.
-    struct Cursor {
-      int item = -1, left = 0, t = 0;      // the item (its number), its steps to come, the step
-    } sc, gr;
-    bool ok = true, more = true;
-    // the next item; false when there is none
-    auto advance = [&](Cursor& c) {
-      ++c.item;
-      if (!waitw(&item_full[c.item % kDkvItems], (uint32_t)((c.item / kDkvItems) & 1), kErrTimeoutOther)) { ok = false; return false; }
-      c.left = uniform(items[c.item % kDkvItems].n);
-      return c.left > 0;
+  } else if (warp >= kDkvWarps + 1) {
+    // Two warps issue the products, one the scores (up to three steps ahead), one the gradients: the
+    // waits and the issue of all 16 products of a step in one warp took 1700 clocks, more than the softmax.
+    const bool grads = warp == kDkvWarps + 2;
+    int st = 0, u = 0;                       // ring slot and buffer of the step, with the parity of their use
+    uint32_t st_ph = 0, u_ph = 0;
+    auto step = [&]() {
+      if (++st == kDkvStages) { st = 0; st_ph ^= 1u; }
+      if (++u == 3) { u = 0; u_ph ^= 1u; }
     };
-    auto scores = [&]() {        // S^T = K Q^T and dP^T = V dO^T
-      const int st = sc.t % kDkvStages, u = sc.t % 3, kb = sc.item & 1;
-      if (!waitw(&kv_full[kb], (uint32_t)((sc.item >> 1) & 1), kErrTimeoutFull)) return false;
-      if (!waitw(&q_full[st], (uint32_t)((sc.t / kDkvStages) & 1), kErrTimeoutFull)) return false;
-      tc_fence_after();
-      const uint32_t qa = smem_u32(sQd + st * 2 * kTile), ka = smem_u32(sKV + 32768 * kb), tS = tbase + 128 * u;
-      const uint64_t qd = kdesc0(qa), dd = kdesc0(qa + kTile), kd = kdesc0(ka), vd = kdesc0(ka + 2 * kTile);
-      umma4_ss_w<2, 2>(tS, kd, qd, id_s, 0u);
-      umma4_ss_w<2, 2>(tS + 64, vd, dd, id_s, 0u);
-      umma_commit_w(&s_full[u]);
-      ++sc.t;
-      if (--sc.left == 0) umma_commit_w(&kv_empty[kb]);
-      return true;
-    };
-    while (ok) {
-      while (ok && more && sc.t - gr.t < 3) {
-        if (sc.left == 0) more = advance(sc);
-        if (more && ok) ok = scores();
+    bool ok = true;
+    int t = 0;
+    for (int item = 0; ok; ++item) {
+      const int slot = item % kDkvItems;
+      if (!waitw(&item_full[slot], (uint32_t)((item / kDkvItems) & 1), kErrTimeoutOther)) break;
+      const int n = uniform(items[slot].n);
+      if (n < 0) break;
+      if (!grads) {              // S^T = K Q^T and dP^T = V dO^T
+        constexpr uint32_t id_s = sink_idesc<BF>(0);
+        const int kb = item & 1;
+        const uint32_t ka = smem_u32(sKV) + 32768 * kb;
+        const uint64_t kd = kdesc0(ka), vd = kdesc0(ka + 2 * kTile);
+        ok = waitw(&kv_full[kb], (uint32_t)((item >> 1) & 1), kErrTimeoutFull);
+        for (int j = 0; j < n && ok; ++j, ++t) {
+          if (t >= 3 && !(ok = waitw(&g_done[u], u_ph ^ 1u, kErrTimeoutOther))) break;
+          if (!(ok = waitw(&q_full[st], st_ph, kErrTimeoutFull))) break;
+          tc_fence_after();
+          const uint32_t qa = smem_u32(sQd) + st * 2 * kTile, tS = tbase + 128 * u;
+          umma4_ss_w<2, 2>(tS, kd, kdesc0(qa), id_s, 0u);
+          umma4_ss_w<2, 2>(tS + 64, vd, kdesc0(qa + kTile), id_s, 0u);
+          umma_commit_w(&s_full[u]);
+          step();
+        }
+        if (ok) umma_commit_w(&kv_empty[kb]);
+      } else {
+        constexpr uint32_t id_g = sink_idesc<BF>(1);
+        for (int j = 0; j < n && ok; ++j) {
+          if (!(ok = waitw(&ds_full[u], u_ph, kErrTimeoutReady))) break;
+          if (j == 0 && item > 0 && !(ok = waitw(acc_empty, (uint32_t)((item - 1) & 1), kErrTimeoutOther))) break;
+          tc_fence_after();
+          const uint32_t qa = smem_u32(sQd) + st * 2 * kTile, tS = tbase + 128 * u, acc = j > 0 ? 1u : 0u;
+          umma4_ts_w<32, 128>(tbase + 384, tS, mndesc0(qa + kTile), id_g, acc);         // dV += P^T dO
+          umma4_ts_w<32, 128>(tbase + 448, tS + 64, mndesc0(qa), id_g, acc);            // dK += dS^T Q
+          umma_commit_w(&g_done[u]);
+          umma_commit_w(&q_empty[st]);
+          step();
+        }
+        if (ok) umma_commit_w(acc_full);
       }
-      if (!ok || gr.t == sc.t) break;
-      const bool first = gr.left == 0;
-      if (first) {
-        if (gr.item >= 0 && lane == 0) mbar_arrive(&item_empty[gr.item % kDkvItems]);
-        if (!advance(gr)) break;
-      }
-      const int st = gr.t % kDkvStages, u = gr.t % 3;
-      if (!waitw(&ds_full[u], (uint32_t)((gr.t / 3) & 1), kErrTimeoutReady)) break;
-      if (first && gr.item > 0 && !waitw(acc_empty, (uint32_t)((gr.item - 1) & 1), kErrTimeoutOther)) break;
-      tc_fence_after();
-      const uint32_t qa = smem_u32(sQd + st * 2 * kTile), tS = tbase + 128 * u;
-      const uint64_t qmn = mndesc0(qa), dmn = mndesc0(qa + kTile);
-      umma4_ts_w<32, 128>(tbase + 384, tS, dmn, id_g, first ? 0u : 1u);             // dV += P^T dO
-      umma4_ts_w<32, 128>(tbase + 448, tS + 64, qmn, id_g, first ? 0u : 1u);        // dK += dS^T Q
-      umma_commit_w(&q_empty[st]);
-      ++gr.t;
-      if (--gr.left == 0) umma_commit_w(acc_full);
+      if (lane == 0) mbar_arrive(&item_empty[slot]);
     }
   } else {
     const int set = warp >> 3, g = (warp >> 2) & 1, wg = warp >> 2, quarter = warp & 3, row = 32 * quarter + lane;
