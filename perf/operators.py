@@ -215,14 +215,13 @@ def _run_own(st):
         B, H, Hkv, Sq, Sk = case["B"], case["H"], case["Hkv"], case["Sq"], case["Sk"]
         p = sa3k.sink_attn(B, H, Sq, Sk, HEAD ** -0.5, case["left"], case["right"], case["sinks"], heads_kv=Hkv,
                            dtype=case["dtype"], align_end=case["end"], q_len=st["q_len"], kv_len=st["kv_len"])
-        sq, sk = (Sq * H * HEAD, HEAD, H * HEAD), (Sk * Hkv * HEAD, HEAD, Hkv * HEAD)
-        t4 = sa3k.t4
-        q, k, v, o = t4(st["q"], *sq), t4(st["k"], *sk), t4(st["v"], *sk), t4(st["o"], *sq)
+        # [B][S][H][64] tensors as the batch, head and row strides that they have
+        t4 = lambda t: sa3k.t4(t, t.stride(0), t.stride(2), t.stride(1))  # noqa: E731
+        q, k, v, o = t4(st["q"]), t4(st["k"]), t4(st["v"]), t4(st["o"])
         if op == "attn_fwd":
             ctx.attention_sink_fwd(p, q, k, v, o, st["lse"])
             return st["o"], st["lse"]
-        ctx.attention_sink_bwd(p, q, k, v, o, t4(st["do"], *sq), st["lse"], t4(st["dq"], *sq), t4(st["dk"], *sk),
-                               t4(st["dv"], *sk))
+        ctx.attention_sink_bwd(p, q, k, v, o, t4(st["do"]), st["lse"], t4(st["dq"]), t4(st["dk"]), t4(st["dv"]))
         return st["dq"], st["dk"], st["dv"]
     if op == "lin_fwd":
         ctx.linear_act_fwd(st["w"], st["x"], st["y"], case["act"], bias=st["bias"], residual=st["residual"], z=st["z"])
