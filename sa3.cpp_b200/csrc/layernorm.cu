@@ -524,16 +524,16 @@ constexpr int kLnMaxRegCols = 32768;   // 1024 threads x 32 values
 
 // Threads per row and chunks per thread.  Rows of up to 256 columns take a part of a warp (the
 // smallest power of two that holds them at 8 columns a thread); longer ones a whole block of at
-// most 1024 threads, at 8, 16 or 32 columns a thread.  In the forward rows of up to 2048 columns stay
-// with one warp, at up to 64 columns a thread: no barrier, and all of a row's loads in flight (4352 x
-// 1536 f32 -> f16: 12.4 us with blocks, 9.6 with warps).
+// most 1024 threads, at 8, 16 or 32 columns a thread.  In the forward rows of up to 1024 columns stay
+// with one warp, at up to 32 columns a thread: no barrier, and all of a row's loads in flight (32768 x
+// 1000 f32 -> f16: 50 us with blocks, 42 with warps; 4352 x 1536: 12.8 with blocks, 15.2 with warps).
 struct LnShape {
   bool block;
   int tpr, threads, nv;
 };
 LnShape ln_shape(int cols, bool forward) {
   LnShape s;
-  if (cols <= (forward ? 2048 : 256)) {
+  if (cols <= (forward ? 1024 : 256)) {
     s.block = false;
     s.tpr = 1;
     while (s.tpr * 8 < cols && s.tpr < 32) s.tpr *= 2;
@@ -571,9 +571,7 @@ int fwd_typed(Ctx* c, const LnArgs& a, bool vec, std::string& err) {
       case 1: return fwd_launch<TX, TY, false, 1>(c, a, s, vec, err);
       case 2: return fwd_launch<TX, TY, false, 2>(c, a, s, vec, err);
       case 3: return fwd_launch<TX, TY, false, 3>(c, a, s, vec, err);
-      case 4: return fwd_launch<TX, TY, false, 4>(c, a, s, vec, err);
-      case 5: case 6: return fwd_launch<TX, TY, false, 6>(c, a, s, vec, err);
-      default: return fwd_launch<TX, TY, false, 8>(c, a, s, vec, err);
+      default: return fwd_launch<TX, TY, false, 4>(c, a, s, vec, err);
     }
   }
   if (s.nv == 1) return fwd_launch<TX, TY, true, 1>(c, a, s, vec, err);
@@ -697,8 +695,8 @@ int check_matrix(const char* what, const void* p, int type, int64_t rows, int64_
 }
 
 int check_shape(int64_t rows, int64_t cols, std::string& err) {
-  if (rows < 0 || cols < 1 || cols > (1 << 24) || rows > 0x7fffffff) {
-    err = "layernorm: need 0 <= rows < 2^31 and 1 <= cols <= 2^24";
+  if (rows < 0 || cols < 1 || cols > (1 << 20) || rows > 0x7fffffff) {
+    err = "layernorm: need 0 <= rows < 2^31 and 1 <= cols <= 2^20";
     return 1;
   }
   return 0;
