@@ -352,15 +352,17 @@ int sa3k_head_prep_bwd(sa3k_ctx* ctx, const float* g, int64_t g_ld, const float*
  *     call that would have to grow it during a capture fails.  Graphs captured from one context
  *     share its scratch: replay them one after another, as the context's own calls run;
  *   - a size of 0 (rows, S, B, Sq, Sk) is allowed and launches nothing for what is empty;
- *   - outputs must not overlap inputs or one another;
+ *   - outputs must not overlap inputs or one another (the residual of sa3k_linear_act_fwd may be y
+ *     itself);
  *   - the current CUDA device is left as the caller had it. */
 
 /* y = (x - mean) * rstd * gamma + beta per row of x[rows][cols], mean and rstd = 1 / sqrt(var + eps)
  * of the row (population variance).  x and y are F32, F16 or BF16 (SA3K_TYPE_*, each its own), row
  * strides x_ld, y_ld in elements; gamma, beta f32 [cols] (NULL: 1 and 0); mean, rstd f32 [rows]
- * (NULL, or kept for the backward).  Arithmetic in f32.  Rows of a multiple of 8 columns with
- * 16-byte aligned bases and row strides run fastest.  The norm of a pre-norm block without the adaLN
- * modulation; counterpart of nn::rms_norm (src/nn.h:40-42) with mean and offset. */
+ * (NULL, or kept for the backward).  rows < 2^31, cols from 1 to 2^20.  Arithmetic in f32.  Rows of a
+ * multiple of 8 columns with 16-byte aligned bases and row strides run fastest.  The norm of a
+ * pre-norm block without the adaLN modulation; counterpart of nn::rms_norm (src/nn.h:40-42) with mean
+ * and offset. */
 int sa3k_layernorm_fwd(sa3k_ctx* ctx, int64_t rows, int64_t cols, int x_type, const void* x, int64_t x_ld,
                        const float* gamma, const float* beta, float eps, int y_type, void* y, int64_t y_ld,
                        float* mean, float* rstd, char* err, int err_len);
@@ -415,6 +417,7 @@ int sa3k_attention_sink_bwd(sa3k_ctx* ctx, const sa3k_sink_attn* p, const sa3k_t
 /* z = dit_lin(W, x) + bias as sa3k_linear_fwd computes it (with the adapter, when given) and
  * y[S][out] = act(z) + residual.  x[S][in], residual, z, y[S][out] are F32 or F16 (`type`, all the
  * same), contiguous; residual and z may be NULL (z: the pre-activation, kept for the backward).
+ * x, dx, bias and the adapter's arrays start on 16 bytes; S <= 2^20 - 16.
  * Products read IEEE half operands with f32 accumulation (SA3K_OPT notes above): x and W are
  * rounded to half, activation and residual are applied to the f32 value, and y is rounded once.
  * Replaces dit_lin followed by its activation and add (src/dit.h:244-254). */

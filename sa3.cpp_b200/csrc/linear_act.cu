@@ -142,15 +142,30 @@ __global__ void __launch_bounds__(128) act_bwd_kernel(const T* __restrict__ dy, 
 int64_t pad64(int64_t v) { return (v + 63) / 64 * 64; }
 size_t al(size_t b) { return (b + 255) & ~(size_t)255; }
 
-int check_args(const Ctx* c, const Weight* w, const sa3k_adapter* ad, int act, int type, const void* x, int64_t S,
+int check_args(const Ctx* c, const Weight* w, const sa3k_adapter* ad, const float* bias, int act, int type, int64_t S,
                std::string& err) {
   if (w->device != c->device) { err = "linear_act: the weight is on another device than the context"; return 1; }
   if (act < kActNone || act > kActGeluTanh) { err = "linear_act: unknown activation"; return 1; }
   if (type != kTypeF32 && type != kTypeF16) { err = "linear_act: the type must be F32 or F16"; return 1; }
   if (S < 0 || S > (1 << 20) - 16) { err = "linear_act: S must be from 0 to 2^20 - 16"; return 1; }
-  if (S > 0 && (!x || !aligned16(x))) { err = "linear_act: x must be given and start on 16 bytes"; return 1; }
-  if (ad && (ad->rank < 1 || ad->rank > 16 || !ad->A || !ad->B)) { err = "adapter rank must be 1..16 with A and B"; return 1; }
-  if (ad && ad->magnitude && !ad->base_norm_sq) { err = "dora adapter needs base_norm_sq"; return 1; }
+  if (!aligned16(bias)) { err = "linear_act: bias must start on 16 bytes"; return 1; }
+  if (!ad) return 0;
+  if (ad->rank < 1 || ad->rank > 16 || !ad->A || !ad->B) { err = "adapter rank must be 1..16 with A and B"; return 1; }
+  if (!aligned16(ad->A) || !aligned16(ad->B) || !aligned16(ad->magnitude) || !aligned16(ad->base_norm_sq)) {
+    err = "linear_act: the adapter's arrays must start on 16 bytes";
+    return 1;
+  }
+  if (ad->magnitude && !ad->base_norm_sq) { err = "dora adapter needs base_norm_sq"; return 1; }
+  return 0;
+}
+
+// x, y, ...: given, and on 16 bytes where the kernels read it in vectors (`vec`), else on its own type
+int check_rows(const char* what, const void* p, int type, bool vec, std::string& err) {
+  if (!p) { err = std::string("linear_act: ") + what + " is NULL"; return 1; }
+  if (reinterpret_cast<uintptr_t>(p) % (vec ? 16 : type == kTypeF32 ? 4 : 2)) {
+    err = std::string("linear_act: ") + what + (vec ? " must start on 16 bytes" : " is not aligned to its type");
+    return 1;
+  }
   return 0;
 }
 
@@ -301,9 +316,11 @@ int sa3k_linear_act_fwd(sa3k_ctx* ctx, const sa3k_weight* w, const sa3k_adapter*
                         const void* x, int64_t S, const void* residual, void* z, void* y, char* err, int err_len) {
   return api_call(ctx, err, err_len, [&](Ctx* c, std::string& e) {
     if (!w) { e = "linear_act: the weight is NULL"; return 1; }
-    if (check_args(c, &w->w, ad, act, type, x, S, e)) return 1;
+    if (check_args(c, &w->w, ad, bias, act, type, S, e)) return 1;
     if (S == 0) return 0;
-    if (!y) { e = "linear_act: y is NULL"; return 1; }
+    if (check_rows("x", x, type, true, e) || check_rows("y", y, type, false, e) ||
+        (residual && check_rows("residual", residual, type, false, e)) || (z && check_rows("z", z, type, false, e)))
+      return 1;
     return linear_act_forward(c, &w->w, ad, bias, act, type, x, S, residual, z, y, e);
   });
 }
@@ -314,11 +331,14 @@ int sa3k_linear_act_bwd(sa3k_ctx* ctx, const sa3k_weight* w, const sa3k_adapter*
   return api_call(ctx, err, err_len, [&](Ctx* c, std::string& e) {
     if (!w) { e = "linear_act: the weight is NULL"; return 1; }
     const bool dora = ad && ad->magnitude;
-    if (check_args(c, &w->w, ad, act, type, ad ? x : (x ? x : dy), S, e)) return 1;
+    if (check_args(c, &w->w, ad, bias, act, type, S, e)) return 1;
     if (ad && (!dA || !dB || (dora && !dm))) { e = "linear_act: an adapter needs dA and dB, and dm for dora"; return 1; }
-    if (S > 0 && !dy) { e = "linear_act: dy is NULL"; return 1; }
-    if (S > 0 && !z && (act != kActNone || dora)) { e = "linear_act: the backward needs the forward's z"; return 1; }
-    if (S > 0 && dx && !aligned16(dx)) { e = "linear_act: dx must start on 16 bytes"; return 1; }
+    if (S > 0) {
+      if (check_rows("dy", dy, type, false, e) || (ad && check_rows("x", x, type, true, e)) ||
+          (z && check_rows("z", z, type, false, e)) || (dx && check_rows("dx", dx, type, true, e)))
+        return 1;
+      if (!z && (act != kActNone || dora)) { e = "linear_act: the backward needs the forward's z"; return 1; }
+    }
     if (S == 0) {
       if (accumulate) return 0;
       const size_t n[4] = {(size_t)w->w.out, ad ? (size_t)(ad->rank * w->w.in) : 0, ad ? (size_t)(ad->rank * w->w.out) : 0,

@@ -40,7 +40,15 @@ OPT_DEQUANT_TMEM = 8
 OPT_FUSE_HEAD_PREP = 9
 
 
-_TORCH_TYPES = {"torch.float32": "f32", "torch.float16": "f16", "torch.bfloat16": "bf16"}
+_TYPES = {}
+
+
+def _torch_types():
+    """torch dtype -> SA3K_TYPE_* of the activations (torch is imported on first use)."""
+    if not _TYPES:
+        import torch
+        _TYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 30})
+    return _TYPES
 
 
 class Sa3kError(RuntimeError):
@@ -55,6 +63,7 @@ class Adapter(ctypes.Structure):
 class Tensor4(ctypes.Structure):
     _fields_ = [("data", ctypes.c_void_p), ("batch_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
                 ("row_stride", ctypes.c_int64)]
+    device = None       # the tensor's CUDA device, where t4() made it
 
 
 class SinkAttnC(ctypes.Structure):
@@ -63,6 +72,7 @@ class SinkAttnC(ctypes.Structure):
                 ("Sq", ctypes.c_int), ("Sk", ctypes.c_int), ("head_dim", ctypes.c_int), ("scale", ctypes.c_float),
                 ("left", ctypes.c_int64), ("right", ctypes.c_int64), ("sinks", ctypes.c_int64),
                 ("align_end", ctypes.c_int), ("q_len", ctypes.c_void_p), ("kv_len", ctypes.c_void_p)]
+    device = None
 
 
 def sink_attn(B, H, Sq, Sk, scale, left=-1, right=0, sinks=0, heads_kv=None, dtype="f16", align_end=False, q_len=None,
@@ -76,9 +86,12 @@ def sink_attn(B, H, Sq, Sk, scale, left=-1, right=0, sinks=0, heads_kv=None, dty
     p.keep = (q_len, kv_len)     # the tensors live as long as the description
     for name, t in (("q_len", q_len), ("kv_len", kv_len)):
         if t is not None:
-            if str(t.dtype) != "torch.int32" or t.numel() != B or not t.is_contiguous() or not t.is_cuda:
+            if t.numel() != B or not t.is_cuda or str(t.dtype) != "torch.int32" or not t.is_contiguous():
                 raise Sa3kError(f"sink_attn: {name} must be a contiguous int32 CUDA tensor of B values")
             setattr(p, name, t.data_ptr())
+            if p.device not in (None, t.get_device()):
+                raise Sa3kError("sink_attn: q_len and kv_len must be on one device")
+            p.device = t.get_device()
     return p
 
 
@@ -87,7 +100,9 @@ class HeadSliceC(ctypes.Structure):
 
 
 def t4(t, batch_stride, head_stride, row_stride):
-    return Tensor4(ctypes.c_void_p(t.data_ptr()), batch_stride, head_stride, row_stride)
+    r = Tensor4(t.data_ptr(), batch_stride, head_stride, row_stride)
+    r.device = t.get_device()
+    return r
 
 
 DIT_INT_FIELDS = ("io", "dim", "depth", "heads", "head_dim", "cond_dim", "mem_tokens", "rot", "time_dim",
@@ -343,99 +358,125 @@ class Context:
                                                 ctypes.byref(dv) if dv else None, err, 512), err)
 
     # ------------------------------------------------------- transformer-block operators
+    # (called per token when serving, so the checks are kept cheap)
     def _on_device(self, what, *tensors):
         for t in tensors:
-            if t is not None and t.device.index != self.device:
+            if t is not None and t.get_device() != self.device:
                 raise Sa3kError(f"{what}: a tensor is on {t.device}, the context on cuda:{self.device}")
 
     @staticmethod
     def _type_id(what, t):
-        name = _TORCH_TYPES.get(str(t.dtype))
-        if name is None:
+        ids = _torch_types()
+        if t.dtype not in ids:
             raise Sa3kError(f"{what}: unsupported type {t.dtype}")
-        return TYPE_IDS[name]
+        return ids[t.dtype]
 
     @staticmethod
     def _f32_vector(what, n, *tensors):
         for t in tensors:
-            if t is not None and (str(t.dtype) != "torch.float32" or t.numel() != n or not t.is_contiguous()):
+            if t is not None and (t.numel() != n or _torch_types().get(t.dtype) != 0 or not t.is_contiguous()):
                 raise Sa3kError(f"{what}: expected a contiguous float32 vector of {n} values")
 
     @staticmethod
     def _matrix(what, shape, *tensors):
         for t in tensors:
-            if t is not None and (tuple(t.shape) != tuple(shape) or (t.shape[1] > 1 and t.stride(1) != 1)):
+            if t is not None and (t.shape != shape or (shape[1] > 1 and t.stride(1) != 1)):
                 raise Sa3kError(f"{what}: expected a [{shape[0]}][{shape[1]}] matrix with contiguous rows")
+
+    def _err_buf(self):
+        try:
+            return self._err
+        except AttributeError:
+            self._err = ctypes.create_string_buffer(512)
+            return self._err
+
+    def _call(self, fn, *args):
+        if fn(self._h, *args, self._err_buf(), 512) != 0:
+            raise Sa3kError(self._err.value.decode(errors="replace"))
 
     def layernorm_fwd(self, x, y, gamma=None, beta=None, eps=1e-5, mean=None, rstd=None):
         """y = layer norm of the rows of x [rows][cols] (f32, f16 or bf16 each); mean, rstd [rows] are kept
         when given."""
-        rows, cols = x.shape
-        self._matrix("layernorm", (rows, cols), x, y)
+        shape = x.shape
+        rows, cols = shape
+        self._matrix("layernorm", shape, x, y)
         self._f32_vector("layernorm", cols, gamma, beta)
         self._f32_vector("layernorm", rows, mean, rstd)
         self._on_device("layernorm", x, y, gamma, beta, mean, rstd)
-        err = ctypes.create_string_buffer(512)
-        _check(lib().sa3k_layernorm_fwd(self._h, rows, cols, self._type_id("layernorm", x), x.data_ptr(), x.stride(0),
-                                        _vp(gamma), _vp(beta), eps, self._type_id("layernorm", y), y.data_ptr(),
-                                        y.stride(0), _vp(mean), _vp(rstd), err, 512), err)
+        self._call(lib().sa3k_layernorm_fwd, rows, cols, self._type_id("layernorm", x), x.data_ptr(), x.stride(0),
+                   _vp(gamma), _vp(beta), eps, self._type_id("layernorm", y), y.data_ptr(), y.stride(0), _vp(mean),
+                   _vp(rstd))
 
     def layernorm_bwd(self, x, dy, dx, mean, rstd, gamma=None, dgamma=None, dbeta=None, accumulate=False):
         """dx (x's type, or None), dgamma and dbeta (f32, or None) for upstream dy."""
-        rows, cols = x.shape
-        self._matrix("layernorm", (rows, cols), x, dy, dx)
+        shape = x.shape
+        rows, cols = shape
+        self._matrix("layernorm", shape, x, dy, dx)
         self._f32_vector("layernorm", cols, gamma, dgamma, dbeta)
         self._f32_vector("layernorm", rows, mean, rstd)
         self._on_device("layernorm", x, dy, dx, mean, rstd, gamma, dgamma, dbeta)
         if dx is not None and dx.dtype != x.dtype:
             raise Sa3kError("layernorm: dx has x's type")
-        err = ctypes.create_string_buffer(512)
-        _check(lib().sa3k_layernorm_bwd(self._h, rows, cols, self._type_id("layernorm", x), x.data_ptr(), x.stride(0),
-                                        _vp(gamma), _vp(mean), _vp(rstd), self._type_id("layernorm", dy), dy.data_ptr(),
-                                        dy.stride(0), _vp(dx), 0 if dx is None else dx.stride(0), _vp(dgamma),
-                                        _vp(dbeta), 1 if accumulate else 0, err, 512), err)
+        self._call(lib().sa3k_layernorm_bwd, rows, cols, self._type_id("layernorm", x), x.data_ptr(), x.stride(0),
+                   _vp(gamma), _vp(mean), _vp(rstd), self._type_id("layernorm", dy), dy.data_ptr(), dy.stride(0),
+                   _vp(dx), 0 if dx is None else dx.stride(0), _vp(dgamma), _vp(dbeta), 1 if accumulate else 0)
+
+    def _sink_args(self, p, lse, *tensors):
+        for t in (p,) + tensors:
+            if t is not None and t.device is not None and t.device != self.device:
+                raise Sa3kError(f"attention_sink: a tensor is not on the context's device cuda:{self.device}")
+        if lse is not None:
+            if 0 <= p.B * p.H <= 65535 and p.Sq >= 0:     # (other sizes are refused by the call)
+                self._f32_vector("attention_sink (lse)", p.B * p.H * p.Sq, lse)
+            self._on_device("attention_sink", lse)
 
     def attention_sink_fwd(self, p, q, k, v, o, lse=None):
         """Forward of the attention that p (sink_attn()) describes; q, k, v, o are t4() tensors."""
-        err = ctypes.create_string_buffer(512)
-        _check(lib().sa3k_attention_sink_fwd(self._h, ctypes.byref(p), ctypes.byref(q), ctypes.byref(k), ctypes.byref(v),
-                                             ctypes.byref(o), _vp(lse), err, 512), err)
+        ref = ctypes.byref
+        self._sink_args(p, lse, q, k, v, o)
+        self._call(lib().sa3k_attention_sink_fwd, ref(p), ref(q), ref(k), ref(v), ref(o), _vp(lse))
 
     def attention_sink_bwd(self, p, q, k, v, o, dO, lse, dq, dk=None, dv=None):
-        err = ctypes.create_string_buffer(512)
-        _check(lib().sa3k_attention_sink_bwd(self._h, ctypes.byref(p), ctypes.byref(q), ctypes.byref(k), ctypes.byref(v),
-                                             ctypes.byref(o), ctypes.byref(dO), _vp(lse), ctypes.byref(dq),
-                                             ctypes.byref(dk) if dk else None, ctypes.byref(dv) if dv else None, err,
-                                             512), err)
+        """dq, and dk, dv (both or neither), for upstream dO, from the forward's o and lse."""
+        ref = ctypes.byref
+        self._sink_args(p, lse, q, k, v, o, dO, dq, dk, dv)
+        self._call(lib().sa3k_attention_sink_bwd, ref(p), ref(q), ref(k), ref(v), ref(o), ref(dO), _vp(lse), ref(dq),
+                   ref(dk) if dk else None, ref(dv) if dv else None)
 
     def _act_args(self, w, act, S, ins, outs, vectors):
         if act not in ACTIVATIONS:
             raise Sa3kError(f"linear_act: unknown activation {act!r}")
-        kind = next(t.dtype for t in ins + outs if t is not None)
-        for t, n in [(t, w.inn) for t in ins] + [(t, w.out) for t in outs]:
-            if t is not None and (tuple(t.shape) != (S, n) or not t.is_contiguous() or t.dtype != kind):
-                raise Sa3kError(f"linear_act: expected contiguous [{S}][{n}] tensors of one type")
+        kind = None
+        for group, shape in ((ins, (S, w.inn)), (outs, (S, w.out))):
+            for t in group:
+                if t is None:
+                    continue
+                kind = t.dtype if kind is None else kind
+                if t.shape != shape or t.dtype != kind or not t.is_contiguous():
+                    raise Sa3kError(f"linear_act: expected contiguous [{S}][{shape[1]}] tensors of one type")
         self._f32_vector("linear_act", w.out, *vectors)
         self._on_device("linear_act", *ins, *outs, *vectors)
-        return ACTIVATIONS[act], TYPE_IDS.get(_TORCH_TYPES.get(str(kind)), -1)
+        return ACTIVATIONS[act], _torch_types().get(kind, -1)
 
     def linear_act_fwd(self, w, x, y, act="none", bias=None, residual=None, z=None, ad=None):
         """y = act(dit_lin(w, x) + bias) + residual; x, y, residual, z contiguous f16 or f32 (one type)."""
         S = x.shape[0]
         a, t = self._act_args(w, act, S, (x,), (y, residual, z), (bias,))
-        err = ctypes.create_string_buffer(512)
-        _check(lib().sa3k_linear_act_fwd(self._h, w._h, ctypes.byref(ad) if ad else None, _vp(bias), a, t, x.data_ptr(),
-                                         S, _vp(residual), _vp(z), y.data_ptr(), err, 512), err)
+        self._call(lib().sa3k_linear_act_fwd, w._h, ctypes.byref(ad) if ad else None, _vp(bias), a, t, x.data_ptr(), S,
+                   _vp(residual), _vp(z), y.data_ptr())
 
     def linear_act_bwd(self, w, x, z, dy, dx, act="none", bias=None, dbias=None, ad=None, dA=None, dB=None, dm=None,
                        accumulate=False):
         """dx, dbias and the adapter gradients for upstream dy (x may be None without an adapter)."""
         S = dy.shape[0]
         a, t = self._act_args(w, act, S, (x, dx), (z, dy), (bias, dbias))
-        err = ctypes.create_string_buffer(512)
-        _check(lib().sa3k_linear_act_bwd(self._h, w._h, ctypes.byref(ad) if ad else None, _vp(bias), a, t, _vp(x), S,
-                                         _vp(z), dy.data_ptr(), _vp(dx), _vp(dbias), _vp(dA), _vp(dB), _vp(dm),
-                                         1 if accumulate else 0, err, 512), err)
+        if ad:
+            self._f32_vector("linear_act", ad.rank * w.inn, dA)
+            self._f32_vector("linear_act", ad.rank * w.out, dB)
+            self._f32_vector("linear_act", w.out, dm)
+            self._on_device("linear_act", dA, dB, dm)
+        self._call(lib().sa3k_linear_act_bwd, w._h, ctypes.byref(ad) if ad else None, _vp(bias), a, t, _vp(x), S, _vp(z),
+                   dy.data_ptr(), _vp(dx), _vp(dbias), _vp(dA), _vp(dB), _vp(dm), 1 if accumulate else 0)
 
     def head_prep_fwd(self, y, T, ncols, H, slices, tps, eps, rot, base, out):
         err = ctypes.create_string_buffer(512)
