@@ -326,13 +326,14 @@ int launch(Ctx* c, const SinkArgs& a, std::string& err) {
   auto kern = sink_rows_kernel<BF>;
   if (smem_attr(reinterpret_cast<const void*>(kern), kRowsSmem, c->device, "attention_sink smem attribute", err)) return 1;
   const int tiles = (a.Sq * a.group + 15) / 16;
-  // CTAs per (batch entry, head): a power of two up to 16, until there are two per SM.  Up to 4 pay when
-  // every warp keeps two of its 32-key steps (1 x 24 heads, 576 keys: 6.6 us with one, 6.1 with four),
-  // more when it keeps five (4 x 8 heads, 2051 keys: 8.1 us with four, 9.0 with eight; 1 x 8 heads,
-  // 65536 keys: 92 us with four, 49 with eight).
-  const long span = std::min<long>(a.Sk, (long)a.sinks + std::min<long>((long)a.left + a.right + a.Sq, a.Sk));
+  // CTAs per tile: a power of two up to 16, as long as all stay resident, two per SM (more than that
+  // run in two waves: 8 x 24 heads, 1088 keys, 17.5 us with two CTAs, 12.2 with one; 1 x 24 heads,
+  // 40000 keys, 57 us with 16, 46 with 8).  Up to 4 pay when every warp keeps two of its 32-key steps
+  // (1 x 24 heads, 576 keys: 6.6 us with one, 6.1 with four), more when it keeps five (4 x 8 heads, 2051
+  // keys: 8.1 us with four, 9.0 with eight; 1 x 8 heads, 65536 keys: 92 us with four, 49 with eight).
+  const long span = std::min<long>(a.Sk, (long)a.sinks + std::min<long>((long)a.left + a.right + std::min(a.Sq, 16), a.Sk));
   int nrank = 1;
-  while (nrank < 16 && (long)a.B * a.Hkv * tiles * nrank < 2 * (long)c->sm_count &&
+  while (nrank < 16 && (long)a.B * a.Hkv * tiles * nrank <= (long)c->sm_count &&
          span > (long)nrank * kRowsWarps * (nrank < 4 ? 64 : 160))
     nrank *= 2;
   if (nrank > 8 && cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
@@ -356,8 +357,15 @@ int launch(Ctx* c, const SinkArgs& a, std::string& err) {
 
 }  // namespace
 
-// At most 64 rows share a key / value head: four 16-row tiles, whose keys come from L2 after the first.
-bool sink_rows_applies(const SinkArgs& a) { return (long)a.Sq * a.group <= 64; }
+// Up to 16 query rows (a group's tile of a 128-row kernel would be nearly empty), and more while all
+// 16-row tiles are resident at once, two per SM: the 128-row kernel does not split a row's keys, so
+// few of its tiles take the time of the longest window (us here / there: 1 x 24 heads, 192 rows,
+// 4000 keys 34 / 47; 8 key heads of a group of 4, 32 rows, 8192 keys 21 / 90; 1 x 24 heads, 192 rows
+// in a window of 128 keys 6.1 / 8.3).  Beyond that a tile reads the keys for 16 rows where the other
+// reads them for 128 (8 x 24 heads, 32 rows, 1088 keys: 22 / 20; 64 rows 34 / 20).
+bool sink_rows_applies(const Ctx* c, const SinkArgs& a) {
+  return a.Sq <= 16 || (long)a.B * a.Hkv * (((long)a.Sq * a.group + 15) / 16) <= 2 * (long)c->sm_count;
+}
 
 int sink_rows_forward(Ctx* c, const SinkArgs& a, bool bf16, std::string& err) {
   return bf16 ? launch<true>(c, a, err) : launch<false>(c, a, err);

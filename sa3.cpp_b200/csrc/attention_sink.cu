@@ -973,7 +973,7 @@ int make_seq_map(SeqMap* t, bool bf, const SinkTensor& x, int B, int H, int S, s
 
 template <bool BF>
 int forward(Ctx* c, const SinkArgs& a, std::string& err) {
-  if (sink_rows_applies(a)) return sink_rows_forward(c, a, BF, err);
+  if (sink_rows_applies(c, a)) return sink_rows_forward(c, a, BF, err);
   // (a stand-in key tensor for a forward without keys: its map is never loaded from)
   const bool nokeys = a.Sk == 0;
   SeqMap mq, mk, mv;

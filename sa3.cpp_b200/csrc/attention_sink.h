@@ -45,7 +45,7 @@ __device__ __forceinline__ bool sink_sees(const SinkArgs& a, const SinkSeq& s, i
 }
 
 // the forward for a few query rows per key / value head (attention_rows.cu)
-bool sink_rows_applies(const SinkArgs& a);
+bool sink_rows_applies(const Ctx* c, const SinkArgs& a);
 int sink_rows_forward(Ctx* c, const SinkArgs& a, bool bf16, std::string& err);
 
 }  // namespace sa3k

@@ -235,6 +235,18 @@ def test_attention_sink(ctx, case, token_major, pad):
 
 
 @pytest.mark.parametrize("token_major", [True, False])
+@pytest.mark.parametrize("case", range(1, len(SINK_CASES)))
+def test_attention_sink_of_many_heads(ctx, case, token_major):
+    """The same masks with enough heads that the forward takes 128-row tiles."""
+    kw = dict(SINK_CASES[case])
+    more = 48 // (kw["B"] * kw["Hkv"]) + 1
+    a = Attn(**{**kw, "H": kw["H"] * more, "Hkv": kw["Hkv"] * more}, token_major=token_major, pad=8, seed=300 + case)
+    a.fwd(ctx)
+    ctx.sync()
+    a.check(grads=False)
+
+
+@pytest.mark.parametrize("token_major", [True, False])
 @pytest.mark.parametrize("case", range(len(ROW_CASES)))
 def test_attention_sink_few_rows(ctx, case, token_major):
     a = Attn(**ROW_CASES[case], token_major=token_major, seed=100 + case)
@@ -309,7 +321,7 @@ def test_attention_sink_gradient_against_differences(ctx):
 
 
 def test_attention_sink_empty_sizes(ctx):
-    for dims in (dict(B=0, Sq=8, Sk=8), dict(B=2, Sq=0, Sk=8), dict(B=2, Sq=8, Sk=0), dict(B=2, Sq=300, Sk=0)):
+    for dims in (dict(B=0, Sq=8, Sk=8), dict(B=2, Sq=0, Sk=8), dict(B=2, Sq=8, Sk=0), dict(B=2, Sq=300, Sk=0), dict(B=2, Sq=2500, Sk=0)):
         a = Attn(H=2, Hkv=1, left=4, right=0, sinks=2, **dims)
         a.fwd(ctx)
         a.bwd(ctx)
@@ -346,6 +358,100 @@ def test_attention_sink_refusals(ctx):
         ctx.attention_sink_bwd(a.p, *ok[:3], ok[3], a.t4(a.dO), None, a.t4(a.dq))
     with pytest.raises(sa3k.Sa3kError, match="int32"):
         sa3k.sink_attn(2, 4, 32, 32, 0.125, q_len=torch.zeros(2, device="cuda"))
+
+
+LONG_TOKENS = [   # one stream, one or two heads: clusters of 8 and 16 blocks; the last has keys of no block
+    dict(B=1, H=1, Hkv=1, Sq=1, Sk=20011, left=-1, right=0, sinks=0, end=True),
+    dict(B=1, H=4, Hkv=1, Sq=1, Sk=40000, left=30000, right=0, sinks=100, end=True, dtype="bf16"),
+    dict(B=9, H=1, Hkv=1, Sq=1, Sk=6000, left=-1, right=0, sinks=3, end=True, kn=[6000, 0, 1, 31, 32, 33, 130, 2049, 5999]),
+    dict(B=1, H=1, Hkv=1, Sq=64, Sk=3001, left=2000, right=0, sinks=65, end=True),
+    dict(B=1, H=1, Hkv=1, Sq=65, Sk=3001, left=2000, right=0, sinks=65, end=True),
+]
+
+
+@pytest.mark.parametrize("case", range(len(LONG_TOKENS)))
+def test_attention_sink_long_cache(ctx, case):
+    a = Attn(**LONG_TOKENS[case], seed=200 + case)
+    a.fwd(ctx)
+    ctx.sync()
+    a.check(grads=False)
+
+
+@pytest.mark.parametrize("B,H,Hkv,S,left,sinks", [(4, 16, 16, 700, 64, 64), (2, 8, 4, 1500, 400, 3), (1, 40, 40, 1100, -1, 0)])
+def test_attention_sink_gradients_of_many_tiles(ctx, B, H, Hkv, S, left, sinks):
+    """More (head, key tile) items than SMs; the ones that are long go first."""
+    a = Attn(B, H, Hkv, S, S, left, 0, sinks, seed=17)
+    for _ in range(2):      # the items' counter is set for each call
+        a.dq.fill_(9.0), a.dk.fill_(9.0), a.dv.fill_(9.0)
+        a.fwd(ctx)
+        a.bwd(ctx)
+    ctx.sync()
+    a.check()
+
+
+def test_attention_sink_unseen_keys(ctx):
+    """Keys that no query sees: their gradients are zero, in tiles of their own too."""
+    a = Attn(1, 2, 2, 100, 1000, 10, 0, 2, seed=5)
+    a.fwd(ctx)
+    a.bwd(ctx)
+    ctx.sync()
+    a.check()
+    assert float(a.dk[:, :, 100:].abs().max()) == 0.0 and float(a.dv[:, :, 100:].abs().max()) == 0.0
+
+
+@pytest.mark.parametrize("Sq", [3, 200])
+def test_attention_sink_mixed_layouts_and_broadcast(ctx, Sq):
+    """Each tensor in an order of its own ([S][B][H], [H][B][S], ...), keys and values shared by the batch
+    (stride 0)."""
+    import torch
+    B, H, Sk = 3, 4, 260
+    a = Attn(B, H, H, Sq, Sk, 50, 0, 9, end=True, seed=Sq)
+    order = lambda t, *dims: torch.empty([t.shape[d] for d in dims] + [64], device="cuda", dtype=t.dtype).permute(  # noqa: E731
+        *[dims.index(d) for d in range(3)], 3).copy_(t)
+    a.q, a.dO, a.o = order(a.q, 2, 0, 1), order(a.dO, 1, 0, 2), order(a.o, 1, 2, 0)
+    a.dq, a.dk, a.dv = order(a.dq, 0, 1, 2), order(a.dk, 2, 1, 0), order(a.dv, 1, 0, 2)
+    a.k, a.v = a.k[:1].expand(B, -1, -1, -1), order(a.v, 2, 0, 1)[:1].expand(B, -1, -1, -1)
+    a.fwd(ctx)
+    a.bwd(ctx)
+    ctx.sync()
+    a.check()
+
+
+def test_two_contexts_at_once(ctx):
+    """Contexts on streams of their own share nothing."""
+    import torch
+    import sa3k
+    own, streams = [sa3k.Context(0, use_torch_stream=False) for _ in range(2)], [torch.cuda.Stream() for _ in range(2)]
+    try:
+        for c, s in zip(own, streams):
+            c.set_stream(s.cuda_stream)
+        both = [Attn(2, 8, 8, 500, 500, 100, 0, 16, seed=60 + i) for i in range(2)]
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for c, a in zip(own, both):
+                a.fwd(c)
+                a.bwd(c)
+        for c, a in zip(own, both):
+            c.sync()
+        for a in both:
+            a.check()
+    finally:
+        for c in own:
+            c.close()
+
+
+def test_attention_sink_wrapper_refusals(ctx):
+    import torch
+    import sa3k
+    a = Attn(1, 2, 2, 32, 32, 8, 0, 4)
+    t = [a.t4(x) for x in (a.q, a.k, a.v, a.o)]
+    host = torch.zeros(1, 2, 32, 64, dtype=torch.float16)
+    with pytest.raises(sa3k.Sa3kError, match="not on the context's device"):
+        ctx.attention_sink_fwd(a.p, sa3k.t4(host, 4096, 2048, 64), *t[1:], a.lse)
+    with pytest.raises(sa3k.Sa3kError, match="float32 vector of 64"):
+        ctx.attention_sink_fwd(a.p, *t, a.lse[..., :31])
+    with pytest.raises(sa3k.Sa3kError, match="float32 vector of 64"):
+        ctx.attention_sink_fwd(a.p, *t, a.lse.double())
 
 
 # --------------------------------------------------------------- linear with activation, residual
@@ -387,7 +493,7 @@ def test_linear_act(ctx, S, inn, out, kind, t, act, residual, keep, cache):
     if not cache and kind in ("f16", "f32"):
         pytest.skip("only quantized weights have a form without the half copy")
     if not cache and out % 16:
-        pytest.skip("without the half copy the engine takes widths of 16 (its refusal: test_gpu_linear)")
+        pytest.skip("without the half copy, the engine's gradients take widths of 16")
     ctx.set_option(sa3k.OPT_WEIGHT_F16_CACHE, 1 if cache else 0)
     w, W = _weight(ctx, kind, inn, out, S + out)
     ctx.set_option(sa3k.OPT_WEIGHT_F16_CACHE, 1)
@@ -484,10 +590,49 @@ def test_linear_act_refusals_and_empty(ctx):
     with pytest.raises(sa3k.Sa3kError, match="dA and dB"):
         ctx.linear_act_bwd(w, x, y, y, None, "silu",
                            ad=ctx.adapter(torch.zeros(16, 64, device="cuda"), torch.zeros(48, 16, device="cuda"), 1.0))
+    with pytest.raises(sa3k.Sa3kError, match="bias must start"):
+        ctx.linear_act_fwd(w, x, y, bias=torch.zeros(49, device="cuda")[1:])
+    with pytest.raises(sa3k.Sa3kError, match="adapter's arrays"):
+        ctx.linear_act_fwd(w, x, y, ad=ctx.adapter(torch.zeros(16 * 64 + 1, device="cuda")[1:].view(16, 64),
+                                                   torch.zeros(48, 16, device="cuda"), 1.0))
     db = torch.ones(48, device="cuda")
     ctx.linear_act_fwd(w, x[:0], y[:0], "silu")
     ctx.linear_act_bwd(w, None, y[:0], y[:0], x[:0], "silu", dbias=db)
     assert float(db.abs().max()) == 0.0
+
+
+@pytest.mark.parametrize("S,t", [(5, "f16"), (40, "f16"), (40, "f32"), (1100, "f16"), (700, "f32")])
+def test_linear_act_residual_in_place_and_unaligned(ctx, S, t):
+    """The residual may be y itself; y, z and the residual need no more than their type's alignment."""
+    import torch
+    w, W = _weight(ctx, "q8_0", 128, 520, 6)
+    rnd = _rand(S)
+    x, res, bias = rnd(S, 128).to(_dt(t)), rnd(S, 520).to(_dt(t)), rnd(520)
+    y, z = torch.empty_like(res), torch.empty_like(res)
+    ctx.linear_act_fwd(w, x, y, "gelu", bias=bias, residual=res, z=z)
+    inplace = res.clone()
+    ctx.linear_act_fwd(w, x, inplace, "gelu", bias=bias, residual=inplace)
+    assert torch.equal(inplace, y)
+    off = lambda: torch.zeros(S * 520 + 1, device="cuda", dtype=_dt(t))[1:].view(S, 520)  # noqa: E731
+    y1, z1, r1 = off(), off(), off()
+    r1.copy_(res)
+    ctx.linear_act_fwd(w, x, y1, "gelu", bias=bias, residual=r1, z=z1)
+    # The same f32 products, but the compiler contracts another kernel's sums and activation otherwise: f32
+    # values at most 2^-20 (|act| + |residual|) apart (the bound of an activation above), and after rounding
+    # a step of the type more; a step is 2 finfo.eps / 2 of the value
+    D, step = torch.float64, torch.finfo(_dt(t)).eps
+    near = lambda a, b, m: bool(((a.to(D) - b.to(D)).abs() <= 2 ** -20 * m + step * b.to(D).abs() + 2.0 ** -24).all())  # noqa: E731
+    mag = res.to(D).abs() * 2 + y.to(D).abs() + x.to(D).abs() @ W.T.abs() + bias.to(D).abs()
+    assert near(y1, y, mag) and near(z1, z, mag)
+    z1.copy_(z)
+    dy, dx, dx1 = rnd(S, 520).to(_dt(t)), torch.empty_like(x), torch.empty_like(x)
+    dy1 = off()
+    dy1.copy_(dy)
+    ctx.linear_act_bwd(w, None, z, dy, dx, "gelu")
+    ctx.linear_act_bwd(w, None, z1, dy1, dx1, "gelu")
+    # dz (a half operand) a step apart in places, |act'| <= 1.13, then dx's own step
+    lim = 2.0 ** -10 * (1.13 * dy.to(D).abs() @ W.abs()) + step * dx.to(D).abs() + 2.0 ** -24
+    assert bool(((dx.to(D) - dx1.to(D)).abs() <= lim).all())
 
 
 # ---------------------------------------------------------------------- together, graphs, streams
