@@ -348,9 +348,9 @@ int sa3k_head_prep_bwd(sa3k_ctx* ctx, const float* g, int64_t g_ld, const float*
  * activation and residual: what a pre-norm transformer block is made of, forward and backward.
  * Besides the conventions above:
  *   - the calls are asynchronous on the context's stream, and allocate only when a context's scratch
- *     has to grow; scratch that a stream capture has used stays valid for the context's life, and a
- *     call that would have to grow it during a capture fails.  Graphs captured from one context
- *     share its scratch: replay them one after another, as the context's own calls run;
+ *     has to grow, which it may during a stream capture too.  Scratch that a capture has used stays
+ *     valid for the context's life.  Graphs captured from one context share its scratch: replay them
+ *     one after another, as the context's own calls run;
  *   - a size of 0 (rows, S, B, Sq, Sk) is allowed and launches nothing for what is empty;
  *   - outputs must not overlap inputs or one another (the residual of sa3k_linear_act_fwd may be y
  *     itself);

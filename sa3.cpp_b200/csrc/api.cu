@@ -43,11 +43,16 @@ void* scratch_get(Ctx* c, int slot, size_t bytes, std::string& err) {
       s = Scratch{};
     }
     const size_t want = (bytes + 255) & ~(size_t)255;
-    if (cudaMalloc(&s.ptr, want) != cudaSuccess) {
+    // (an allocation is no work of the stream: it may be made beside a capture, which without this would
+    // be invalidated)
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    if (capturing) cudaThreadExchangeStreamCaptureMode(&mode);
+    const cudaError_t e = cudaMalloc(&s.ptr, want);
+    if (capturing) cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e != cudaSuccess) {
       cudaGetLastError();
       s.ptr = nullptr;
-      err = capturing ? "scratch cannot grow during a stream capture: make one eager call of this size first"
-                      : "out of device memory for scratch";
+      err = "out of device memory for scratch";
       return nullptr;
     }
     s.bytes = want;

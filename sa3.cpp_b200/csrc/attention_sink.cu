@@ -26,8 +26,9 @@ namespace {
 // row) each, and P / dS go back to tensor memory as packed 16-bit pairs to be the next product's A
 // operand.  Several CTAs share an SM and its tensor memory (three of the forward, two of dq; dk / dv has
 // one with three sets of buffers), so one CTA's softmax and the start and end of its work run under the
-// others' products.  The first tile of a window, the last of a sequence and the tiles at its edges are masked; tiles that no row of
-// the CTA sees are never loaded, so the work follows the window and not the sequence.
+// others' products.  The first tile of a window, the last of a sequence and the tiles at its edges are
+// masked; tiles that no row of the CTA sees are never loaded, so the work follows the window and not
+// the sequence.
 constexpr int kSoftWarps = 8, kSinkThreads = 32 * (kSoftWarps + 2);
 constexpr int kTile = 8192;                 // 64 rows x 64 values x 2 bytes
 
@@ -403,7 +404,7 @@ __global__ void __launch_bounds__(kFwdThreads, 3)
 // a tile's 64 keys each.  The threads copy S and dP to registers and give their columns back at
 // once, so the next tile's products run under this tile's exponentials; dS has columns of its own.
 // Measured: 49 us for 4 x 24 heads, 1088 rows in a band of 256 with 64 sinks, 60 us for 3 x 24 heads of
-// 2047 ragged rows in a window of 512 (one persistent CTA pair per SM over all tiles took 52 and 69).
+// 2047 ragged rows in a window of 512 (two persistent CTAs per SM over all tiles took 52 and 69).
 // TMEM: S [0, 64), dP [64, 128), dQ [128, 192), dS in two buffers of 32 columns at 192 and 224.
 constexpr int kDqStages = 3;
 constexpr int kDqSmem = 49152 + kDqStages * 2 * kTile + 256 + 1024;
@@ -618,9 +619,9 @@ __global__ void __launch_bounds__(kSinkThreads, 2)
 // after the other form one stream of steps.  16 softmax warps in two sets take alternate steps (in a
 // set a thread owns a key row and 32 of the step's 64 query columns), and there are three buffers for
 // S^T and dP^T, so a set finds its next scores ready: with one CTA of 8 warps and one buffer twice per
-// SM every step waited for four products in series (1450 clocks a step and SM, then 700; with scores and
-// gradients issued by warps of their own 580: 66 us for 4 x 24 heads, 1088 rows in a band of 256 with
-// 64 sinks).
+// SM every step waited for four products in series (1450 clocks a step and SM, then 700; 4 x 24 heads,
+// 1088 rows in a band of 256 with 64 sinks: 80 us then, 66 since scores and gradients have an issuing
+// warp each).
 // Items are handed out by a counter, heaviest first (those with sinks are seen by every later query).
 // TMEM: buffer u < 3 at 128 u: S^T [0, 64), dP^T [64, 128) (P^T, dS^T of columns 32 g .. overwrite the
 // first 16 columns of their own halves); dV at 384, dK at 448.

@@ -764,28 +764,34 @@ def test_block_captured_replayed_and_outgrown(ctx):
         own.close()
 
 
-def test_capture_that_would_grow_scratch_is_refused(ctx):
-    """The first call of a size inside a capture fails with an error; the context stays usable."""
+def test_first_call_inside_a_capture(ctx):
+    """Scratch grows beside a capture without invalidating it; what an earlier capture holds stays valid, and
+    the random generator that the capture took is given back."""
     import torch
     import sa3k
     own = sa3k.Context(0, use_torch_stream=False)
     side = torch.cuda.Stream()
     own.set_stream(side.cuda_stream)
     try:
-        a = Attn(1, 2, 2, 64, 64, 8, 0, 4)
-        a.lse.fill_(0)
+        both = [Attn(1, 2, 2, 64, 64, 8, 0, 4), Attn(3, 8, 8, 400, 400, 70, 0, 4)]
+        blocks = [Block(own, 1, 40, seed=5), Block(own, 2, 300, seed=6)]
         torch.cuda.synchronize()
-        g = torch.cuda.CUDAGraph()
-        with pytest.raises((sa3k.Sa3kError, RuntimeError)):
-            with torch.cuda.graph(g, stream=side):
+        graphs = []
+        for a, b in zip(both, blocks):
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1], stream=side):
+                a.fwd(own)
                 a.bwd(own)
-        del g
-        torch.cuda.synchronize()
+                b.fwd()
+                b.bwd()
         with torch.cuda.stream(side):
-            a.fwd(own)
-            a.bwd(own)
+            for g in graphs * 2:
+                g.replay()
         own.sync()
-        a.check()
+        for a, b in zip(both, blocks):
+            a.check()
+            _close(b.outputs(), b.reference())
+        assert torch.isfinite(torch.randn(3, device="cuda")).all()
     finally:
         own.close()
 
