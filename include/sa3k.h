@@ -396,7 +396,8 @@ typedef struct sa3k_sink_attn {
  * wanted).  A row that sees no key gets o = 0 and lse = -inf.  Bases start on 16 bytes and strides
  * are multiples of 8 elements.  Scores, softmax and sums are f32; the probabilities are rounded to
  * the inputs' type for the product with v.  Keys and values inside kv_len have to be finite, whether
- * a row sees them or not.  Counterpart of attn_sliding (src/nn.h:79-100) for a sequence with memory
+ * a row sees them or not; with Sq = 1 only those that are seen (the rest of a cache may hold anything).
+ * Counterpart of attn_sliding (src/nn.h:79-100) for a sequence with memory
  * tokens in front (src/dit.h:154-155). */
 int sa3k_attention_sink_fwd(sa3k_ctx* ctx, const sa3k_sink_attn* p, const sa3k_tensor4* q, const sa3k_tensor4* k,
                             const sa3k_tensor4* v, const sa3k_tensor4* o, float* lse, char* err, int err_len);

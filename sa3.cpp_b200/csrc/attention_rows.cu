@@ -115,7 +115,9 @@ __global__ void __launch_bounds__(32 * kRowsWarps, 2) sink_rows_kernel(const __g
   const uint16_t* kp = static_cast<const uint16_t*>(a.k.p) + (long)b * a.k.sb + (long)hk * a.k.sh;
   const uint16_t* vp = static_cast<const uint16_t*>(a.v.p) + (long)b * a.v.sb + (long)hk * a.v.sh;
   auto step_key = [&](int j) { return (j < ns ? j : w0 + (j - ns)) * 32; };
-  auto load = [&](int c) {       // this warp's step c into ring slot c % kRowsStages (rows behind the end: zeros)
+  // keys that no row of the tile sees come in as zeros, whatever they hold: 0 x NaN would spoil a product
+  const int lo = plo - a.left;
+  auto load = [&](int c) {       // this warp's step c into ring slot c % kRowsStages
     const int j = first + c * stride;
     if (j < n) {
       const int k0 = step_key(j);
@@ -124,7 +126,7 @@ __global__ void __launch_bounds__(32 * kRowsWarps, 2) sink_rows_kernel(const __g
       for (int i = 0; i < 8; ++i) {
         const int r = 4 * i + (lane >> 3), ch = lane & 7, key = k0 + r;
         const uint32_t off = r * 128 + ((ch ^ (r & 7)) << 4);
-        const bool in = key < s.kn;
+        const bool in = key < hi && (key >= lo || key < a.sinks);
         const long kr = in ? key : 0;
         cp16(dst + off, kp + kr * a.k.ld + 8 * ch, in);
         cp16(dst + 4096 + off, vp + kr * a.v.ld + 8 * ch, in);

@@ -389,6 +389,24 @@ def test_attention_sink_gradients_of_many_tiles(ctx, B, H, Hkv, S, left, sinks):
     a.check()
 
 
+@pytest.mark.parametrize("Hkv,end", [(4, True), (1, True), (2, False)])
+def test_attention_sink_token_and_evicted_keys(ctx, Hkv, end):
+    """A single token does not read what lies outside its window: NaN and infinities there stay there."""
+    import torch
+    a = Attn(2, 4, Hkv, 1, 777, 100, 5, 37, end=end, kn=[777, 401], seed=8)
+    want = Attn(2, 4, Hkv, 1, 777, 100, 5, 37, end=end, kn=[777, 401], seed=8)
+    j = torch.arange(777, device="cuda")
+    for b in range(2):
+        pos = a.kn[b] - 1 if end else 0
+        gone = ~(((j >= pos - 100) | (j < 37)) & (j <= pos + 5))
+        a.k[b, :, gone], a.v[b, :, gone] = float("nan"), float("inf")
+    a.fwd(ctx)
+    want.fwd(ctx)
+    ctx.sync()
+    want.check(grads=False)
+    assert torch.equal(a.o, want.o) and torch.equal(a.lse, want.lse)
+
+
 def test_attention_sink_unseen_keys(ctx):
     """Keys that no query sees: their gradients are zero, in tiles of their own too."""
     a = Attn(1, 2, 2, 100, 1000, 10, 0, 2, seed=5)
