@@ -32,7 +32,7 @@ __global__ void __launch_bounds__(256) act_residual_kernel(const float* zf, long
 template <class T, int W>
 __global__ void __launch_bounds__(128) act_splits_kernel(const float* __restrict__ partial, int splits, long n, int N,
                                                          const float* __restrict__ scale, const float* __restrict__ bias, int act,
-                                                         const T* __restrict__ residual, T* __restrict__ z, T* __restrict__ y) {
+                                                         const T* residual, T* __restrict__ z, T* y) {   // (y may be the residual)
   pdl_prologue();
   const long i = ((long)blockIdx.x * 128 + threadIdx.x) * W;
   if (i >= n) return;
