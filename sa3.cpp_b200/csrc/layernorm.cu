@@ -143,9 +143,13 @@ __device__ __forceinline__ void store_chunk(T* p, int c, int t, int tpr, int col
   }
 }
 
-// Forward with the row in registers: NV chunks of 8 columns per thread.
+// Forward with the row in registers: NV chunks of 8 columns per thread.  With one vector
+// chunk a block is held to 32 registers a thread (no spills; the scalar form would), so that an SM holds
+// its full 2048 threads: what bounds the kernel is how many rows are between their loads and their stores
+// (4352 x 1536 f32 to f16 12.0 us against 12.6 without, 16384 rows 36.7 against 38.7; gamma and beta
+// loaded ahead of the sums cost registers: 13.7).
 template <class TX, class TY, bool BLOCK, int NV, bool VEC>
-__global__ void __launch_bounds__(BLOCK ? 1024 : 256) ln_fwd_kernel(const LnArgs a, int tpr) {
+__global__ void __launch_bounds__(BLOCK ? 1024 : 256, BLOCK && NV == 1 && VEC ? 2 : 1) ln_fwd_kernel(const LnArgs a, int tpr) {
   __shared__ float2 red[2][32];
   pdl_prologue();
   const int t = BLOCK ? threadIdx.x : threadIdx.x & (tpr - 1);
@@ -526,7 +530,7 @@ constexpr int kLnMaxRegCols = 32768;   // 1024 threads x 32 values
 // smallest power of two that holds them at 8 columns a thread); longer ones a whole block of at
 // most 1024 threads, at 8, 16 or 32 columns a thread.  In the forward rows of up to 1024 columns stay
 // with one warp, at up to 32 columns a thread: no barrier, and all of a row's loads in flight (32768 x
-// 1000 f32 -> f16: 50 us with blocks, 42 with warps; 4352 x 1536: 12.8 with blocks, 15.2 with warps).
+// 1000 f32 -> f16: 46 us with blocks, 42 with warps; 4352 x 1536: 12.0 with blocks, 15.2 with warps).
 struct LnShape {
   bool block;
   int tpr, threads, nv;
