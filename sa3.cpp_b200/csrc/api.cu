@@ -224,11 +224,19 @@ int sa3k_ctx_create(int device, sa3k_ctx** out, char* err, int err_len) {
   if (!c) return fill_err(err, err_len, "out of host memory");
   c->c.device = device;
   c->c.sm_count = (size_t)prop.multiProcessorCount;
+  // the error word and the split-K counters are one allocation, zeroed before any call can be captured
+  constexpr size_t words = 64 + kSplitCounters;
   if (cudaStreamCreateWithFlags(&c->c.stream, cudaStreamNonBlocking) != cudaSuccess ||
-      cudaMalloc(&c->c.d_err, sizeof(int)) != cudaSuccess || cudaMemset(c->c.d_err, 0, sizeof(int)) != cudaSuccess) {
+      cudaMalloc(&c->c.d_err, words * sizeof(int)) != cudaSuccess ||
+      cudaMemsetAsync(c->c.d_err, 0, words * sizeof(int), c->c.stream) != cudaSuccess ||
+      cudaStreamSynchronize(c->c.stream) != cudaSuccess) {
+    if (c->c.d_err) cudaFree(c->c.d_err);
+    if (c->c.stream) cudaStreamDestroy(c->c.stream);
+    cudaGetLastError();
     delete c;
     return fill_err(err, err_len, "failed to create the context stream / error word");
   }
+  c->c.split_cnt = c->c.d_err + 64;
   c->c.own_stream = true;
   *out = c;
   return 0;

@@ -65,21 +65,15 @@ static int make_map(CUtensorMap* m, CUtensorMapDataType dt, const void* base, ui
 }
 
 // Per-tile split counters of the split-K GEMMs (split-K runs only with at most sm_count / 2
-// output tiles).  Zeroed once when allocated; the kernel resets each counter it completes.
+// output tiles).  Zeroed when the context is made, never in a stream that may be captured: a
+// recorded memset would not have run when the next call looks at them.  The kernel resets each
+// counter it completes.
 static int* split_counters(Ctx* c, std::string& err) {
-  constexpr size_t kCounters = 1024;
-  const bool fresh = (int)c->scratch.size() <= kSlotSplitCnt || !c->scratch[(size_t)kSlotSplitCnt].ptr;
-  int* p = static_cast<int*>(scratch_get(c, kSlotSplitCnt, kCounters * sizeof(int), err));
-  if (!p) return nullptr;
-  if (fresh && cudaMemsetAsync(p, 0, kCounters * sizeof(int), c->stream) != cudaSuccess) {
-    check_launch("split counters", err);
-    return nullptr;
-  }
-  if ((size_t)c->sm_count / 2 > kCounters) {
+  if ((size_t)c->sm_count / 2 > kSplitCounters) {
     err = "gemm: too many SMs for the split-K counters";
     return nullptr;
   }
-  return p;
+  return c->split_cnt;
 }
 
 // Tail split: when the tiles leave a last, partial round on `slots` CTAs (or CTA pairs), split

@@ -49,11 +49,14 @@ struct ProfEntry {
   std::vector<std::pair<cudaEvent_t, cudaEvent_t>> pending;
 };
 
+constexpr size_t kSplitCounters = 1024;
+
 struct Ctx {
   int device = 0;
   cudaStream_t stream = nullptr;
   bool own_stream = false;
   int* d_err = nullptr;              // device error word written by bounded waits
+  int* split_cnt = nullptr;          // [kSplitCounters] split-K tile counters, zero between launches
   std::vector<Scratch> scratch;      // indexed by the slot enums of the callers
   std::vector<void*> retired;        // outgrown scratch that a captured graph may still address
   size_t sm_count = 148;
@@ -137,7 +140,7 @@ inline int check_launch(const char* what, std::string& err) {
 }
 
 // Scratch slots owned by a context (see api.cu for the linear path's slots).
-enum : int { kSlotSplitK = 63, kSlotHeadSlices = 62, kSlotRope = 61, kSlotSplitCnt = 60, kSlotChainX = 59,
+enum : int { kSlotSplitK = 63, kSlotHeadSlices = 62, kSlotRope = 61, kSlotChainX = 59,
              kSlotChainU = 58, kSlotLnPart = 56, kSlotSinkD = 55, kSlotActX = 54,
              kSlotActZ = 53, kSlotActPart = 52, kSlotActAdapter = 51 };   // (57: materialize.cu)
 
