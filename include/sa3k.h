@@ -397,6 +397,8 @@ typedef struct sa3k_sink_attn {
  * are multiples of 8 elements.  Scores, softmax and sums are f32; the probabilities are rounded to
  * the inputs' type for the product with v.  Keys and values inside kv_len have to be finite, whether
  * a row sees them or not; with Sq = 1 only those that are seen (the rest of a cache may hold anything).
+ * The sums of v are formed before the division by the softmax's sum, with weights of up to 2^8: 2^8 times the
+ * sum of a row's |v| has to stay in f32's range.  A NaN in a visible key makes the rows that see it NaN.
  * Counterpart of attn_sliding (src/nn.h:79-100) for a sequence with memory
  * tokens in front (src/dit.h:154-155). */
 int sa3k_attention_sink_fwd(sa3k_ctx* ctx, const sa3k_sink_attn* p, const sa3k_tensor4* q, const sa3k_tensor4* k,

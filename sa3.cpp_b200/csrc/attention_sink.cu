@@ -74,22 +74,29 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8])
 // 2^x of a pair without the MUFU unit, whose 16 values a clock per SM are the forward's scarcest:
 // x = n + f with n = round(x) (adding 1.5 * 2^23 leaves n in the low mantissa bits) and a polynomial
 // for 2^f on [-1/2, 1/2], degree 4, fitted here by iteratively reweighted least squares for the least
-// relative error (2.6e-6, of either sign), n added into the exponent field.  x is clamped at -125:
-// what lies below gives 2^-125.
+// relative error (2.6e-6, of either sign; the degree 3 of attention_tc.cu has 8e-5, which would go into
+// lse and from there into every probability of the backward).  2^n is made from n's bits and multiplied
+// in, so that a NaN stays one; x is clamped at -127, where n's exponent field is 0: a masked score gives 0,
+// as in the MUFU unit.
+__device__ __forceinline__ float max_nan(float a, float b) {     // (fmaxf drops a NaN)
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 __device__ __forceinline__ void ex2_pair(float x0, float x1, float& y0, float& y1) {
   constexpr float kMagic = 12582912.f;
-  const uint64_t x = f2(fmaxf(x0, -125.f), fmaxf(x1, -125.f));
+  const uint64_t x = f2(max_nan(x0, -127.f), max_nan(x1, -127.f));
   const uint64_t t = fadd2(x, f2(kMagic, kMagic));
   const uint64_t f = ffma2(fadd2(t, f2(-kMagic, -kMagic)), f2(-1.f, -1.f), x);
   uint64_t p = ffma2(f2(0.009570101f, 0.009570101f), f, f2(0.05591786f, 0.05591786f));
   p = ffma2(p, f, f2(0.24024744f, 0.24024744f));
   p = ffma2(p, f, f2(0.6931218f, 0.6931218f));
   p = ffma2(p, f, f2(0.9999993f, 0.9999993f));
-  float p0, p1, t0, t1;
-  f2split(p, p0, p1);
+  float t0, t1;
   f2split(t, t0, t1);
-  y0 = __uint_as_float((__float_as_uint(t0) << 23) + __float_as_uint(p0));   // (the magic's own bits leave the word)
-  y1 = __uint_as_float((__float_as_uint(t1) << 23) + __float_as_uint(p1));
+  const uint64_t s = f2(__uint_as_float((__float_as_uint(t0) << 23) + 0x3f800000u),    // (the magic's own bits leave the word)
+                        __uint_as_float((__float_as_uint(t1) << 23) + 0x3f800000u));
+  f2split(fmul2(p, s), y0, y1);
 }
 // pair e of a row: one of every kPolyOf by the polynomial (2 x 24 heads, 2048 rows, band 256: 34.5 us
 // against 35.1 without; 24 heads, 8192 rows: 93.0 against 94.5.  The backward passes gain nothing and

@@ -78,3 +78,50 @@ def test_split_product_captured_before_any_eager_call(ctx, first):
         own.close()
         for c in held:
             rt.cudaFree(c)
+
+
+# ---------------------------------------------------------------------- values that are not finite
+def _sees(Sq, Sk, left, right, sinks):
+    import torch
+    p, j = torch.arange(Sq, device="cuda")[:, None], torch.arange(Sk, device="cuda")[None]
+    return (j <= p + right) & ((j < sinks) | (j >= p - left))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("Sq", [256, 16])      # 128-row tiles; 16-row tiles
+def test_attention_sink_nan_in_a_visible_key(ctx, dtype, Sq):
+    """One NaN key per head, at every residue of the column: the rows that see it are NaN, the others are what
+    they are without it."""
+    import torch
+    a, clean = (Attn(1, 48, 48, Sq, 256, 100, 0, 8, dtype=dtype, seed=21) for _ in range(2))
+    at = [(5 * h) % Sq for h in range(48)]                # sink tile, whole tiles, edges; all residues mod 8
+    for h, j in enumerate(at):
+        a.k[0, h, j, 7 + h % 3] = float("nan")
+    a.fwd(ctx)
+    clean.fwd(ctx)
+    ctx.sync()
+    clean.check(grads=False)
+    see = _sees(Sq, 256, 100, 0, 8)
+    for h, j in enumerate(at):
+        hit = see[:, j]
+        assert bool(a.o[0, h, hit].isnan().all()) and bool(a.lse[0, h, hit].isnan().all()), (h, j)
+        assert torch.equal(a.o[0, h, ~hit], clean.o[0, h, ~hit]) and torch.equal(a.lse[0, h, ~hit], clean.lse[0, h, ~hit])
+
+
+@pytest.mark.parametrize("Sq", [256, 16])
+def test_attention_sink_huge_values_outside_the_window(ctx, Sq):
+    """A value near bf16's largest weighs exactly nothing in the rows that do not see its key.  (Those that do are
+    not compared: with probabilities of up to 2^8 before the division, 2^126 leaves the f32 sums' range.)"""
+    import torch
+    a, clean = (Attn(1, 48, 48, Sq, 256, 20, 0, 0, dtype="bf16", seed=22) for _ in range(2))
+    at = [(h * 5) % Sq for h in range(48)]
+    for h, j in enumerate(at):
+        a.v[0, h, j] = 2.0 ** 126
+    a.fwd(ctx)
+    clean.fwd(ctx)
+    ctx.sync()
+    clean.check(grads=False)
+    see = _sees(Sq, 256, 20, 0, 0)
+    for h, j in enumerate(at):
+        assert torch.equal(a.o[0, h, ~see[:, j]], clean.o[0, h, ~see[:, j]]), (h, j)
+    assert torch.equal(a.lse, clean.lse)
