@@ -71,52 +71,11 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8])
                : "memory");
 }
 
-// 2^x of a pair without the MUFU unit, whose 16 values a clock per SM are the forward's scarcest:
-// x = n + f with n = round(x) (adding 1.5 * 2^23 leaves n in the low mantissa bits) and a polynomial
-// for 2^f on [-1/2, 1/2], degree 4, fitted here by iteratively reweighted least squares for the least
-// relative error (2.6e-6, of either sign; the degree 3 of attention_tc.cu has 8e-5, which would go into
-// lse and from there into every probability of the backward).  2^n is made from n's bits and multiplied
-// in, so that a NaN stays one; x is clamped at -127, where n's exponent field is 0: a masked score gives 0,
-// as in the MUFU unit.
-__device__ __forceinline__ float max_nan(float a, float b) {     // (fmaxf drops a NaN)
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void ex2_pair(float x0, float x1, float& y0, float& y1) {
-  constexpr float kMagic = 12582912.f;
-  const uint64_t x = f2(max_nan(x0, -127.f), max_nan(x1, -127.f));
-  const uint64_t t = fadd2(x, f2(kMagic, kMagic));
-  const uint64_t f = ffma2(fadd2(t, f2(-kMagic, -kMagic)), f2(-1.f, -1.f), x);
-  uint64_t p = ffma2(f2(0.009570101f, 0.009570101f), f, f2(0.05591786f, 0.05591786f));
-  p = ffma2(p, f, f2(0.24024744f, 0.24024744f));
-  p = ffma2(p, f, f2(0.6931218f, 0.6931218f));
-  p = ffma2(p, f, f2(0.9999993f, 0.9999993f));
-  float t0, t1;
-  f2split(t, t0, t1);
-  const uint64_t s = f2(__uint_as_float((__float_as_uint(t0) << 23) + 0x3f800000u),    // (the magic's own bits leave the word)
-                        __uint_as_float((__float_as_uint(t1) << 23) + 0x3f800000u));
-  f2split(fmul2(p, s), y0, y1);
-}
-// pair e of a row: one of every kPolyOf by the polynomial (2 x 24 heads, 2048 rows, band 256: 34.5 us
-// against 35.1 without; 24 heads, 8192 rows: 93.0 against 94.5.  The backward passes gain nothing and
-// take the MUFU unit alone)
-constexpr int kPolyOf = 4;
-__device__ __forceinline__ void ex2_at(int e, float x0, float x1, float& y0, float& y1) {
-  if (e % kPolyOf == 1) {
-    ex2_pair(x0, x1, y0, y1);
-  } else {
-    y0 = ex2(x0);
-    y1 = ex2(x1);
-  }
-}
-
 // The 64-key tiles that rows at positions [plo, phi] see: the sink tiles [0, ns), then the window's
 // [w0, w0 + n - ns).
 struct KeyTiles {
   int ns, w0, n;
   __device__ __forceinline__ int tile(int j) const { return j < ns ? j : w0 + (j - ns); }
-  __device__ __forceinline__ bool has(int t) const { return t < ns || (t >= w0 && t < w0 + (n - ns)); }
 };
 __device__ __forceinline__ KeyTiles key_tiles(const SinkArgs& a, const SinkSeq& s, int plo, int phi) {
   KeyTiles k{0, 0, 0};
@@ -174,8 +133,10 @@ __device__ __forceinline__ void store_rows(uint8_t* buf, const uint4 (&w)[NC], u
 // memory, so S of the next tile is formed under this tile's exponentials, and P V under the next
 // one's: a tile's chain is the softmax alone (with P over S's columns the products' latency was 40%
 // of it).  What then bounds the kernel is the exponentials (16 a clock per SM, 512 clocks a tile) and
-// the f32 work around them.  Measured: 34.5 us for 2 x 24 heads, 2048 rows in a band of 256 with 64
-// sinks (390 TFLOP/s), 93 us for 24 heads, 8192 causal rows in a window of 1024 (520 TFLOP/s).
+// the f32 work around them.  All of them take the MUFU unit: a polynomial for every fourth pair, with the
+// clamp and the scaling that keep NaN and give masked scores 0, was slower (36.0 us against 35.6, 100.7 against 98.2).
+// Measured per call: 35.6 us for 2 x 24 heads, 2048 rows in a band of 256 with 64 sinks (379
+// TFLOP/s), 98.2 us for 24 heads, 8192 causal rows in a window of 1024 (493 TFLOP/s).
 constexpr int kFwdThreads = 160;
 constexpr int kFwdSmem = 32768 + 4 * kTile + 128 + 1024;
 
@@ -350,8 +311,7 @@ __global__ void __launch_bounds__(kFwdThreads, 3)
       for (int e = 0; e < 32; ++e) {
         float x0, x1;
         f2split(ffma2(f2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), sc2, nb2), x0, x1);
-        float p0, p1;
-        ex2_at(e, x0, x1, p0, p1);
+        const float p0 = ex2(x0), p1 = ex2(x1);
         ls[e & 1] = fadd2(ls[e & 1], f2(p0, p1));
         v[e] = pack2<BF>(p0, p1);
       }
