@@ -6,14 +6,17 @@
 //
 // Both are bound by memory: each value of x (and dy) is read once and held in registers while its
 // row's sums are formed, and each result is written once.  The variance is taken around the mean
-// of the held values, not from a sum of squares, so a large common offset costs no digits.  All
-// arithmetic is f32 whatever the types; a result is rounded once, when it is stored.
+// of the held values, not from a sum of squares, and what the f32 mean m is off by, the mean e of the
+// x - m, is taken out of it and of every x - m: a large common offset costs the forward no digits (rows
+// of 1e4 + N(0, 1): y was off by 1e-3 without e).  The backward takes mean and rstd as they are kept, in
+// f32.  All arithmetic is f32 whatever the types; a result is rounded once, when it is stored.
 //
 // A row belongs to TPR threads: a part of a warp for short rows, else a whole block.  The backward
 // keeps every thread's columns' sums of dy xh and dy in registers over all the rows that its block
 // walks, and writes one partial row per block; a second kernel adds the partials in block order,
 // so the parameter gradients do not depend on timing.
 #include <cmath>
+#include <type_traits>
 
 #include "../../include/sa3k.h"
 #include "ops_api.h"
@@ -71,34 +74,49 @@ struct LnArgs {
   float* part;                    // backward: [gridDim.x][2][cols] partial dgamma | dbeta
 };
 
-// Sum of two values over the TPR threads of a row; every thread gets it.  `red`: 2 x 32 pairs,
-// alternated by the caller (`ph`) so that one barrier per reduction is enough.
+// Sums over the TPR threads of a row; every thread gets them.  `red`: 2 x 32 pairs, alternated by the
+// caller (`ph`) so that one barrier per reduction is enough.
 template <bool BLOCK>
-__device__ __forceinline__ float2 row_sum(float a, float b, int tpr, float2 (*red)[32], int ph) {
+__device__ __forceinline__ float row_sum(float a, int tpr, float2 (*red)[32], int ph) {
   if (BLOCK) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      a += __shfl_xor_sync(0xffffffffu, a, o);
-      b += __shfl_xor_sync(0xffffffffu, b, o);
-    }
+    a = warp_sum(a);
     const int nw = blockDim.x >> 5;
     if (nw > 1) {
-      if ((threadIdx.x & 31) == 0) red[ph][threadIdx.x >> 5] = make_float2(a, b);
+      if ((threadIdx.x & 31) == 0) red[ph][threadIdx.x >> 5].x = a;
       __syncthreads();
-      const float2 t = (threadIdx.x & 31) < nw ? red[ph][threadIdx.x & 31] : make_float2(0.f, 0.f);
-      a = t.x;
-      b = t.y;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        a += __shfl_xor_sync(0xffffffffu, a, o);
-        b += __shfl_xor_sync(0xffffffffu, b, o);
-      }
+      a = warp_sum((threadIdx.x & 31) < nw ? red[ph][threadIdx.x & 31].x : 0.f);
     }
   } else {
-    for (int o = tpr >> 1; o > 0; o >>= 1) {
-      a += __shfl_xor_sync(0xffffffffu, a, o);
-      b += __shfl_xor_sync(0xffffffffu, b, o);
+    for (int o = tpr >> 1; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+  }
+  return a;
+}
+
+// Two sums at once.  In a block each half of a warp keeps one of them from the first exchange on: 5 + 6
+// shuffles instead of 20.
+template <bool BLOCK>
+__device__ __forceinline__ float2 row_sum2(float a, float b, int tpr, float2 (*red)[32], int ph) {
+  if (BLOCK) {
+    const int lane = threadIdx.x & 31, nw = blockDim.x >> 5;
+    const bool hi = lane & 16;
+    float v = (hi ? b : a) + __shfl_xor_sync(0xffffffffu, hi ? a : b, 16);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (nw > 1) {
+      if ((lane & 15) == 0) (hi ? red[ph][threadIdx.x >> 5].y : red[ph][threadIdx.x >> 5].x) = v;
+      __syncthreads();
+      v = 0.f;
+#pragma unroll
+      for (int w = lane & 15, k = 0; k < 2; ++k, w += 16)
+        if (w < nw) v += hi ? red[ph][w].y : red[ph][w].x;
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     }
+    return make_float2(__shfl_sync(0xffffffffu, v, 0), __shfl_sync(0xffffffffu, v, 16));
+  }
+  for (int o = tpr >> 1; o > 0; o >>= 1) {
+    a += __shfl_xor_sync(0xffffffffu, a, o);
+    b += __shfl_xor_sync(0xffffffffu, b, o);
   }
   return make_float2(a, b);
 }
@@ -143,11 +161,19 @@ __device__ __forceinline__ void store_chunk(T* p, int c, int t, int tpr, int col
   }
 }
 
+// rstd of a row from the sums of d^2 and d, d = x - m; off = mean(d), what the mean m is off by
+__device__ __forceinline__ float ln_rstd(float2 s, const LnArgs& a, float& off) {
+  const float inv = 1.f / (float)a.cols;
+  off = s.y * inv;
+  const float var = fmaf(-off, off, s.x * inv);
+  return 1.0f / sqrtf((var < 0.f ? 0.f : var) + a.eps);     // (a NaN stays one)
+}
+
 // Forward with the row in registers: NV chunks of 8 columns per thread.  With one vector
 // chunk a block is held to 32 registers a thread (no spills; the scalar form would), so that an SM holds
 // its full 2048 threads: what bounds the kernel is how many rows are between their loads and their stores
 // (4352 x 1536 f32 to f16 12.0 us against 12.6 without, 16384 rows 36.7 against 38.7; gamma and beta
-// loaded ahead of the sums cost registers: 13.7).
+// loaded ahead of the sums cost registers: 13.7).  With the mean's correction 11.9 and 37.1.
 template <class TX, class TY, bool BLOCK, int NV, bool VEC>
 __global__ void __launch_bounds__(BLOCK ? 1024 : 256, BLOCK && NV == 1 && VEC ? 2 : 1) ln_fwd_kernel(const LnArgs a, int tpr) {
   __shared__ float2 red[2][32];
@@ -165,30 +191,49 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 256, BLOCK && NV == 1 && VEC ? 
   for (int c = 0; c < NV; ++c)
 #pragma unroll
     for (int e = 0; e < 8; ++e) s += v[c][e];
-  const float mu = row_sum<BLOCK>(s, 0.f, tpr, red, 0).x / (float)a.cols;
-  float q = 0.f;
+  const float mu = row_sum<BLOCK>(s, tpr, red, 0) / (float)a.cols;
+  float q = 0.f, sd = 0.f;
 #pragma unroll
   for (int c = 0; c < NV; ++c)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float d = v[c][e] - mu;
-      if (col_of<VEC>(c, e, t, tpr) < a.cols) q = fmaf(d, d, q);
+      v[c][e] -= mu;
+      if (col_of<VEC>(c, e, t, tpr) < a.cols) {
+        sd += v[c][e];
+        q = fmaf(v[c][e], v[c][e], q);
+      }
     }
-  const float rs = 1.0f / sqrtf(row_sum<BLOCK>(q, 0.f, tpr, red, 1).x / (float)a.cols + a.eps);
+  float off;
+  const float rs = ln_rstd(row_sum2<BLOCK>(q, sd, tpr, red, 1), a, off);
   if (!ok) return;
   if (t == 0) {
-    if (a.mean) a.mean[r] = mu;
+    if (a.mean) a.mean[r] = mu + off;
     if (a.rstd) a.rstd[r] = rs;
   }
   TY* y = static_cast<TY*>(a.out) + r * a.out_ld;
+  const float nor = -off * rs;
 #pragma unroll
   for (int c = 0; c < NV; ++c) {
+    if constexpr (VEC && std::is_same<TY, float>::value) {     // four values at a time: fewer registers
+      const int i = col_of<true>(c, 0, t, tpr);
+      if (i >= a.cols) continue;
+#pragma unroll
+      for (int h = 0; h < 8; h += 4) {
+        const float4 one = make_float4(1.f, 1.f, 1.f, 1.f), zero = make_float4(0.f, 0.f, 0.f, 0.f);
+        const float4 gm = a.gamma ? *reinterpret_cast<const float4*>(a.gamma + i + h) : one;
+        const float4 bt = a.beta ? *reinterpret_cast<const float4*>(a.beta + i + h) : zero;
+        *reinterpret_cast<float4*>(y + i + h) =
+            make_float4(fmaf(fmaf(v[c][h], rs, nor), gm.x, bt.x), fmaf(fmaf(v[c][h + 1], rs, nor), gm.y, bt.y),
+                        fmaf(fmaf(v[c][h + 2], rs, nor), gm.z, bt.z), fmaf(fmaf(v[c][h + 3], rs, nor), gm.w, bt.w));
+      }
+      continue;
+    }
     float gm[8], bt[8], o[8];
     if (a.gamma) load_chunk<VEC>(a.gamma, c, t, tpr, a.cols, gm);
     if (a.beta) load_chunk<VEC>(a.beta, c, t, tpr, a.cols, bt);
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      o[e] = fmaf((v[c][e] - mu) * rs, a.gamma ? gm[e] : 1.f, a.beta ? bt[e] : 0.f);
+      o[e] = fmaf(fmaf(v[c][e], rs, nor), a.gamma ? gm[e] : 1.f, a.beta ? bt[e] : 0.f);
     store_chunk<VEC>(y, c, t, tpr, a.cols, o);
   }
 }
@@ -203,20 +248,22 @@ __global__ void __launch_bounds__(1024) ln_fwd_long_kernel(const LnArgs a) {
   const TX* x = static_cast<const TX*>(a.x) + r * a.x_ld;
   float s = 0.f;
   for (int i = threadIdx.x; i < a.cols; i += blockDim.x) s += to_f32(x[i]);
-  const float mu = row_sum<true>(s, 0.f, 0, red, 0).x / (float)a.cols;
-  float q = 0.f;
+  const float mu = row_sum<true>(s, 0, red, 0) / (float)a.cols;
+  float q = 0.f, sd = 0.f;
   for (int i = threadIdx.x; i < a.cols; i += blockDim.x) {
     const float d = to_f32(x[i]) - mu;
+    sd += d;
     q = fmaf(d, d, q);
   }
-  const float rs = 1.0f / sqrtf(row_sum<true>(q, 0.f, 0, red, 1).x / (float)a.cols + a.eps);
+  float off;
+  const float rs = ln_rstd(row_sum2<true>(q, sd, 0, red, 1), a, off);
   if (threadIdx.x == 0) {
-    if (a.mean) a.mean[r] = mu;
+    if (a.mean) a.mean[r] = mu + off;
     if (a.rstd) a.rstd[r] = rs;
   }
   TY* y = static_cast<TY*>(a.out) + r * a.out_ld;
   for (int i = threadIdx.x; i < a.cols; i += blockDim.x)
-    y[i] = from_f32<TY>(fmaf((to_f32(x[i]) - mu) * rs, a.gamma ? a.gamma[i] : 1.f, a.beta ? a.beta[i] : 0.f));
+    y[i] = from_f32<TY>(fmaf((to_f32(x[i]) - mu - off) * rs, a.gamma ? a.gamma[i] : 1.f, a.beta ? a.beta[i] : 0.f));
 }
 
 // Backward with the row in registers; the block's threads walk rows with stride gridDim.x (x rows
@@ -271,7 +318,7 @@ __global__ void __launch_bounds__(1024) ln_bwd_kernel(const LnArgs a, int tpr) {
           s2 = fmaf(dv[c][e], xv[c][e], s2);
         }
       }
-    const float2 s = row_sum<BLOCK>(s1, s2, tpr, red, ph);
+    const float2 s = row_sum2<BLOCK>(s1, s2, tpr, red, ph);
     const float m1 = s.x * inv, m2 = s.y * inv;
     if (a.out && ok) {
       TX* dx = static_cast<TX*>(a.out) + r * a.out_ld;
@@ -498,7 +545,7 @@ __global__ void __launch_bounds__(1024) ln_bwd_long_kernel(const LnArgs a) {
     s1 += g;
     s2 = fmaf(g, (to_f32(x[i]) - mu) * rs, s2);
   }
-  const float2 s = row_sum<true>(s1, s2, 0, red, 0);
+  const float2 s = row_sum2<true>(s1, s2, 0, red, 0);
   const float m1 = s.x / (float)a.cols, m2 = s.y / (float)a.cols;
   TX* dx = static_cast<TX*>(a.out) + r * a.out_ld;
   for (int i = threadIdx.x; i < a.cols; i += blockDim.x) {

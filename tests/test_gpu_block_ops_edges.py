@@ -125,3 +125,24 @@ def test_attention_sink_huge_values_outside_the_window(ctx, Sq):
     for h, j in enumerate(at):
         assert torch.equal(a.o[0, h, ~see[:, j]], clean.o[0, h, ~see[:, j]]), (h, j)
     assert torch.equal(a.lse, clean.lse)
+
+
+# ------------------------------------------------------------------------------------ layer norm
+@pytest.mark.parametrize("cols", [200, 1000, 1536, 1537, 4100, 9000, 20000, 40000])
+@pytest.mark.parametrize("offset", [1e4, -3e5, 0.0])
+def test_layernorm_offset_costs_no_digits(ctx, cols, offset):
+    """Rows far from zero, every form of the forward.  With m the f32 mean, d = x - m is exact (x and m are
+    within a factor of two), and what m is off by is taken out as the mean of d: a chain of 74 additions of
+    terms whose mean is about one standard deviation, then a few roundings of the result."""
+    import torch
+    x = _rand(cols)(5, cols) + offset
+    y, mean, rstd = torch.empty_like(x), torch.empty(5, device="cuda"), torch.empty(5, device="cuda")
+    ctx.layernorm_fwd(x, y, None, None, 1e-5, mean, rstd)
+    ctx.sync()
+    w = ref.layernorm(x, None, None, 1e-5, torch.float32, 74)
+    c = 74 * 2.0 ** -24
+    # (the first mean is off by c |offset| at most, which widens the terms by as much)
+    wide = 1 + c * abs(offset)
+    ref.assert_within("y", y, w["y"], 2 * c * wide + w["y"].abs() * (c * wide ** 2 + 2 ** -21))
+    ref.assert_within("mean", mean, w["mean"], 2 ** -23 * w["mean"].abs() + 2 * c * wide)
+    ref.assert_within("rstd", rstd, w["rstd"], w["rstd"] * (2 * c * wide ** 2 + 2 ** -21))
