@@ -63,7 +63,7 @@ class Adapter(ctypes.Structure):
 class Tensor4(ctypes.Structure):
     _fields_ = [("data", ctypes.c_void_p), ("batch_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
                 ("row_stride", ctypes.c_int64)]
-    device = None       # the tensor's CUDA device, where t4() made it
+    of = None           # the tensor that t4() made it of
 
 
 class SinkAttnC(ctypes.Structure):
@@ -100,8 +100,9 @@ class HeadSliceC(ctypes.Structure):
 
 
 def t4(t, batch_stride, head_stride, row_stride):
-    r = Tensor4(t.data_ptr(), batch_stride, head_stride, row_stride)
-    r.device = t.get_device()
+    r = Tensor4()
+    r.data, r.batch_stride, r.head_stride, r.row_stride = t.data_ptr(), batch_stride, head_stride, row_stride
+    r.of = t
     return r
 
 
@@ -421,27 +422,52 @@ class Context:
                    _vp(gamma), _vp(mean), _vp(rstd), self._type_id("layernorm", dy), dy.data_ptr(), dy.stride(0),
                    _vp(dx), 0 if dx is None else dx.stride(0), _vp(dgamma), _vp(dbeta), 1 if accumulate else 0)
 
-    def _sink_args(self, p, lse, *tensors):
-        for t in (p,) + tensors:
-            if t is not None and t.device is not None and t.device != self.device:
-                raise Sa3kError(f"attention_sink: a tensor is not on the context's device cuda:{self.device}")
+    def _sink_args(self, p, lse, queries, keys):
+        """Tensors [B][H][Sq] and [B][H_kv][Sk] of the description p: device, type, and that what the sizes and
+        strides reach lies in the tensor's storage (Tensor4s that t4() has not made are taken as they are)."""
+        dev, kind, B, Sq = self.device, (_TYPES or _torch_types()).get, p.B, p.Sq
+        if p.device is not None and p.device != dev:
+            raise Sa3kError(f"attention_sink: a tensor is not on the context's device cuda:{dev}")
+        want = p.type
+        for group, heads, rows in ((queries, p.H, Sq), (keys, p.H_kv, p.Sk)):
+            b, h, s = B - 1, heads - 1, rows - 1
+            for t in group:
+                if t is None or t.of is None:
+                    continue
+                x = t.of
+                if x.get_device() != dev:
+                    raise Sa3kError(f"attention_sink: a tensor is not on the context's device cuda:{dev}")
+                if kind(x.dtype) != want:
+                    raise Sa3kError("attention_sink: a tensor's type is not the description's dtype")
+                # (a contiguous tensor's own values first: its storage takes longer to ask for)
+                reach = b * t.batch_stride + h * t.head_stride + s * t.row_stride + 64
+                if not (x.is_contiguous() and reach <= x.numel()) and reach > x.untyped_storage().nbytes() // 2 - x.storage_offset():
+                    self._sink_reach(p, t, heads, rows)
         if lse is not None:
-            if 0 <= p.B * p.H <= 65535 and p.Sq >= 0:     # (other sizes are refused by the call)
-                self._f32_vector("attention_sink (lse)", p.B * p.H * p.Sq, lse)
-            self._on_device("attention_sink", lse)
+            n = B * p.H * Sq
+            if lse.numel() != n or _TYPES.get(lse.dtype) != 0 or not lse.is_contiguous():
+                if 0 <= B * p.H <= 65535 and Sq >= 0:     # (other sizes are refused by the call)
+                    self._f32_vector("attention_sink (lse)", n, lse)
+            if lse.get_device() != dev:
+                self._on_device("attention_sink", lse)
+
+    @staticmethod
+    def _sink_reach(p, t, heads, rows):
+        """Refuse sizes and strides past the end of t's storage, unless the call itself refuses or ignores them."""
+        used = [s for n, s in ((p.B, t.batch_stride), (heads, t.head_stride), (rows, t.row_stride)) if n > 1]
+        if p.B < 1 or rows < 1 or p.H_kv < 1 or p.H % p.H_kv or p.B * p.H > 65535 or any(s % 8 or s < 0 for s in used):
+            return
+        raise Sa3kError(f"attention_sink: [{p.B}][{heads}][{rows}][64] at these strides reaches past a tensor's end")
 
     def attention_sink_fwd(self, p, q, k, v, o, lse=None):
         """Forward of the attention that p (sink_attn()) describes; q, k, v, o are t4() tensors."""
-        ref = ctypes.byref
-        self._sink_args(p, lse, q, k, v, o)
-        self._call(lib().sa3k_attention_sink_fwd, ref(p), ref(q), ref(k), ref(v), ref(o), _vp(lse))
+        self._sink_args(p, lse, (q, o), (k, v))
+        self._call(lib().sa3k_attention_sink_fwd, p, q, k, v, o, _vp(lse))     # (ctypes takes the structures' addresses)
 
     def attention_sink_bwd(self, p, q, k, v, o, dO, lse, dq, dk=None, dv=None):
         """dq, and dk, dv (both or neither), for upstream dO, from the forward's o and lse."""
-        ref = ctypes.byref
-        self._sink_args(p, lse, q, k, v, o, dO, dq, dk, dv)
-        self._call(lib().sa3k_attention_sink_bwd, ref(p), ref(q), ref(k), ref(v), ref(o), ref(dO), _vp(lse), ref(dq),
-                   ref(dk) if dk else None, ref(dv) if dv else None)
+        self._sink_args(p, lse, (q, o, dO, dq), (k, v, dk, dv))
+        self._call(lib().sa3k_attention_sink_bwd, p, q, k, v, o, dO, _vp(lse), dq, dk, dv)
 
     def _act_args(self, w, act, S, ins, outs, vectors):
         if act not in ACTIVATIONS:
