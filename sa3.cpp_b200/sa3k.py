@@ -58,6 +58,7 @@ class Sa3kError(RuntimeError):
 class Adapter(ctypes.Structure):
     _fields_ = [("A", ctypes.c_void_p), ("B", ctypes.c_void_p), ("magnitude", ctypes.c_void_p),
                 ("base_norm_sq", ctypes.c_void_p), ("scale", ctypes.c_float), ("rank", ctypes.c_int)]
+    of = None           # A, B, m, bns of Context.adapter()
 
 
 class Tensor4(ctypes.Structure):
@@ -484,10 +485,22 @@ class Context:
         self._on_device("linear_act", *ins, *outs, *vectors)
         return ACTIVATIONS[act], _torch_types().get(kind, -1)
 
+    def _act_adapter(self, w, ad, *grads):
+        """The arrays of an adapter that adapter() made, and its gradients, fit the weight."""
+        sizes = ad.rank * w.inn, ad.rank * w.out, w.out, w.out
+        for group in (ad.of or (), grads):
+            for n, t in zip(sizes, group):
+                if t is not None and not hasattr(t, "get_device"):
+                    raise Sa3kError("linear_act (adapter): expected CUDA tensors")
+                self._f32_vector("linear_act (adapter)", n, t)
+            self._on_device("linear_act", *group)
+
     def linear_act_fwd(self, w, x, y, act="none", bias=None, residual=None, z=None, ad=None):
         """y = act(dit_lin(w, x) + bias) + residual; x, y, residual, z contiguous f16 or f32 (one type)."""
         S = x.shape[0]
         a, t = self._act_args(w, act, S, (x,), (y, residual, z), (bias,))
+        if ad:
+            self._act_adapter(w, ad)
         self._call(lib().sa3k_linear_act_fwd, w._h, ctypes.byref(ad) if ad else None, _vp(bias), a, t, x.data_ptr(), S,
                    _vp(residual), _vp(z), y.data_ptr())
 
@@ -497,10 +510,7 @@ class Context:
         S = dy.shape[0]
         a, t = self._act_args(w, act, S, (x, dx), (z, dy), (bias, dbias))
         if ad:
-            self._f32_vector("linear_act", ad.rank * w.inn, dA)
-            self._f32_vector("linear_act", ad.rank * w.out, dB)
-            self._f32_vector("linear_act", w.out, dm)
-            self._on_device("linear_act", dA, dB, dm)
+            self._act_adapter(w, ad, dA, dB, dm)
         self._call(lib().sa3k_linear_act_bwd, w._h, ctypes.byref(ad) if ad else None, _vp(bias), a, t, _vp(x), S, _vp(z),
                    dy.data_ptr(), _vp(dx), _vp(dbias), _vp(dA), _vp(dB), _vp(dm), 1 if accumulate else 0)
 
@@ -537,7 +547,9 @@ class Context:
     @staticmethod
     def adapter(A, B, scale, m=None, bns=None):
         rank = A.shape[0]
-        return Adapter(_ptr(A), _ptr(B), _ptr(m), _ptr(bns), scale, rank)
+        ad = Adapter(_ptr(A), _ptr(B), _ptr(m), _ptr(bns), scale, rank)
+        ad.of = A, B, m, bns
+        return ad
 
     def linear_fwd(self, w, x, y, ad=None, bias=None):
         err = ctypes.create_string_buffer(512)

@@ -103,3 +103,29 @@ def test_attention_devices_come_first(none):
     raw = sa3k.Tensor4(a.t["q"].data_ptr(), 8192, 64, 256)
     for f in a.calls(none, a.describe(dtype="bf16"), q=raw):
         _refuses(f, "ctx is NULL")
+
+
+def test_linear_act_adapter_arrays(none):
+    """The arrays of an adapter fit the weight that it is used with."""
+    import sa3k
+
+    class W:
+        _h, inn, out = None, 64, 48
+
+    f = lambda *s: torch.zeros(*s)  # noqa: E731
+    x, y, dx = (torch.zeros(4, n, dtype=torch.float16) for n in (64, 48, 64))
+    good = dict(A=f(8, 64), B=f(48, 8), m=f(48), bns=f(48))
+    grads = dict(dA=f(8, 64), dB=f(48, 8), dm=f(48))
+    fwd = lambda a: none.linear_act_fwd(W, x, y, "silu", ad=sa3k.Context.adapter(a["A"], a["B"], 1.0, a["m"], a["bns"]))  # noqa: E731
+    bwd = lambda a, g: none.linear_act_bwd(W, x, y, y, dx, "silu", ad=sa3k.Context.adapter(a["A"], a["B"], 1.0, a["m"], a["bns"]), **g)  # noqa: E731
+    for call in (lambda: fwd(good), lambda: bwd(good, grads)):
+        _refuses(call, "ctx is NULL")
+    for n, bad in (("A", f(8, 63)), ("A", f(64, 8).t()), ("B", f(47, 8)), ("B", f(48, 8).half()), ("m", f(47)), ("bns", f(49)),
+                   ("A", f(8, 64).numpy())):
+        _refuses(lambda: fwd({**good, n: bad}), "linear_act .adapter.")
+        _refuses(lambda: bwd({**good, n: bad}, grads), "linear_act .adapter.")
+    for n, bad in (("dA", f(7, 64)), ("dB", f(48, 9)), ("dm", f(47)), ("dA", f(8, 64).double())):
+        _refuses(lambda: bwd(good, {**grads, n: bad}), "linear_act .adapter.")
+    none.device = 0
+    for call in (lambda: fwd(good), lambda: bwd(good, grads)):
+        _refuses(call, "the context on")
