@@ -51,9 +51,12 @@ int sa3k_ctx_set_stream(sa3k_ctx* ctx, void* cuda_stream, char* err, int err_len
 /* Context options (sa3k_ctx_set_option).  No counterpart in the reference.
  *   SA3K_OPT_WEIGHT_F16_CACHE  1 (default): a Q8_0 / Q4_K weight uploaded afterwards also keeps
  *       an IEEE half (f16) operand copy, made once by the bit-exact dequantizer (the frozen base
- *       never changes, so the tensor cores then read f16 tiles directly).  0: codes + scales only.
+ *       never changes, so the tensor cores then read f16 tiles directly).  0: codes + scales only,
+ *       but for output widths that are no multiple of 4 (Q8_0) or 2 (Q4_K): the GEMMs cannot read
+ *       such scales, and these weights always keep the copy.
  *   SA3K_OPT_SMEM_DEQUANT  1: GEMMs over quantized weights dequantize each TMA-loaded tile in
- *       shared memory even when an f16 copy exists.  0 (default): use the copy when present.
+ *       shared memory even when an f16 copy exists (not at the widths just named).  0 (default): use
+ *       the copy when present.
  * Both paths round the same f32 dequantized value once to f16, so results are identical.
  *
  * Operand type.  Every tensor-core contraction of the library (the GEMM engine, the rank-16
@@ -430,7 +433,10 @@ int sa3k_linear_act_fwd(sa3k_ctx* ctx, const sa3k_weight* w, const sa3k_adapter*
 /* Backward for upstream dy, from the forward's z (not needed for SA3K_ACT_NONE without a dora
  * adapter): dz = dy act'(z), dx[S][in] = dz W (+ the adapter's part; NULL: not wanted), dbias[out] =
  * colsum dz (NULL: not wanted) and, with an adapter, dA, dB, dm as sa3k_linear_bwd (x is needed then).
- * accumulate != 0 adds into dbias, dA, dB, dm; dx is overwritten.  The residual's gradient is dy. */
+ * accumulate != 0 adds into dbias, dA, dB, dm; dx is overwritten.  The residual's gradient is dy.
+ * dz is rounded to half as an operand of dx and the adapter gradients (dbias is summed before): what lies
+ * below 2^-25 vanishes there and what passes 65504 overflows, for F32 activations too.  With an adapter
+ * `out` is a multiple of 8. */
 int sa3k_linear_act_bwd(sa3k_ctx* ctx, const sa3k_weight* w, const sa3k_adapter* ad, const float* bias, int act, int type,
                         const void* x, int64_t S, const void* z, const void* dy, void* dx, float* dbias, float* dA,
                         float* dB, float* dm, int accumulate, char* err, int err_len);

@@ -410,7 +410,7 @@ int sa3k_weight_upload(sa3k_ctx* ctx, int type, const void* blocks, int64_t in, 
     if (cudaMalloc(&w.f16, (size_t)(in * out * 2)) != cudaSuccess) return fail("out of device memory (weight)");
   }
   if (weight_repack(&ctx->c, &w, e)) return fail(e);
-  if ((type == kTypeQ8_0 || type == kTypeQ4_K) && ctx->c.weight_cache) {
+  if (quantized(w) && (ctx->c.weight_cache || !scales_fit_tma(w))) {
     if (cudaMalloc(&w.f16, (size_t)(in * out * 2)) != cudaSuccess) return fail("out of device memory (weight cache)");
     if (weight_cache_f16(&ctx->c, &w, e)) return fail(e);
   }

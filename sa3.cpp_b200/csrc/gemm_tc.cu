@@ -375,8 +375,7 @@ int gemm(Ctx* c, const GemmDesc& d, std::string& err) {
   const bool weight_b = d.bsrc == kB_WEIGHT_NT || d.bsrc == kB_WEIGHT_TN;
   // quantized weights run through the in-smem dequant path unless a f16 operand copy exists
   // and the context has not asked for the in-smem path explicitly
-  const bool quant = weight_b && d.w && (d.w->type == kTypeQ8_0 || d.w->type == kTypeQ4_K) &&
-                     !(d.w->f16 && !c->smem_dequant);
+  const bool quant = weight_b && d.w && dequantizes_inside(c, *d.w);
   if (d.epi && (quant || d.bsrc != kB_WEIGHT_NT || d.a_mn || d.out_trans || d.out_h_trans || d.out_h_t || d.accumulate ||
                 (d.out != nullptr) == (d.out_h != nullptr) || (d.out ? d.ldo : d.ldo_h) != d.N)) {
     err = "gemm: the activation epilogue needs an f16 weight operand and one dense row-major output";

@@ -214,8 +214,7 @@ int linear_act_forward(Ctx* c, const Weight* w, const sa3k_adapter* ad, const fl
   LinearFwd f;
   f.w = w; f.ad = ad ? &prep : nullptr; f.bias = bias; f.x_h = x_h; f.M = S;
   f.ut = ut; f.ut_ld = pad64(S);
-  const bool half_copy = w->f16 && !(c->smem_dequant && (w->type == kTypeQ8_0 || w->type == kTypeQ4_K));
-  if (half_copy) {     // activation and residual in the GEMM's epilogue
+  if (!dequantizes_inside(c, *w)) {     // activation and residual in the GEMM's epilogue
     ActEpi e;
     e.act = act; e.residual = residual; e.z = z;
     f.epi = &e;
@@ -333,6 +332,8 @@ int sa3k_linear_act_bwd(sa3k_ctx* ctx, const sa3k_weight* w, const sa3k_adapter*
     const bool dora = ad && ad->magnitude;
     if (check_args(c, &w->w, ad, bias, act, type, S, e)) return 1;
     if (ad && (!dA || !dB || (dora && !dm))) { e = "linear_act: an adapter needs dA and dB, and dm for dora"; return 1; }
+    // (rows of B^T and of dora's factors are operands of TMA: 16-byte steps of halves)
+    if (ad && w->w.out % 8) { e = "linear_act: the backward of an adapter needs an output width that is a multiple of 8"; return 1; }
     if (S > 0) {
       if (check_rows("dy", dy, type, false, e) || (ad && check_rows("x", x, type, true, e)) ||
           (z && check_rows("z", z, type, false, e)) || (dx && check_rows("dx", dx, type, true, e)))

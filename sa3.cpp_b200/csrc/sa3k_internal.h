@@ -25,12 +25,17 @@ struct Weight {
   int8_t* codes = nullptr;           // Q8_0 int8 [out][in] | Q4_K nibble pairs [out][in/2]
   float* scales = nullptr;           // Q8_0 f32 [in/32][out] | Q4_K float2 [in/32][out]
   __half* f16 = nullptr;     // f16 [out][in] operand copy (F16/F32 always; Q8_0/Q4_K
-                                     // when the context keeps a dequantized cache)
+                                     // when the context keeps a dequantized cache, or scales_fit_tma is false)
   int8_t* codes_t = nullptr;         // Q8_0 int8 [in][out] | Q4_K nibble pairs [in][out/2]: the codes
                                      // transposed, made on the first input-gradient GEMM that
                                      // dequantizes in the kernel (gemm_wq)
   int device = 0;
 };
+
+inline bool quantized(const Weight& w) { return w.type == kTypeQ8_0 || w.type == kTypeQ4_K; }
+// TMA reads the rows of a quantized base's scales, [in/32][out], in steps of 16 bytes: a GEMM can
+// dequantize the base itself when `out` is a multiple of 4 (Q8_0) or 2 (Q4_K)
+inline bool scales_fit_tma(const Weight& w) { return w.out * (w.type == kTypeQ4_K ? 8 : 4) % 16 == 0; }
 
 // Growable device scratch owned by a context.
 struct Scratch {
@@ -81,6 +86,11 @@ struct Ctx {
   std::vector<ProfEntry> prof;
   std::vector<cudaEvent_t> ev_pool;
 };
+
+// The GEMMs over this base dequantize it themselves (they read the f16 operand copy otherwise).
+inline bool dequantizes_inside(const Ctx* c, const Weight& w) {
+  return quantized(w) && !(w.f16 && !(c->smem_dequant && scales_fit_tma(w)));
+}
 
 // RAII bracket around one kernel launch of class `name`.
 struct ProfScope {

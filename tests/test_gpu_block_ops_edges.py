@@ -146,3 +146,87 @@ def test_layernorm_offset_costs_no_digits(ctx, cols, offset):
     ref.assert_within("y", y, w["y"], 2 * c * wide + w["y"].abs() * (c * wide ** 2 + 2 ** -21))
     ref.assert_within("mean", mean, w["mean"], 2 ** -23 * w["mean"].abs() + 2 * c * wide)
     ref.assert_within("rstd", rstd, w["rstd"], w["rstd"] * (2 * c * wide ** 2 + 2 ** -21))
+
+
+# ------------------------------------------------------------------------ widths of quantized bases
+ODD_WIDTHS = [  # S, in, out, weight, type
+    (5, 128, 77, "q8_0", "f16"), (33, 128, 77, "q8_0", "f16"), (200, 192, 129, "q8_0", "f32"), (40, 128, 520, "q8_0", "f16"),
+    (300, 64, 1001, "q8_0", "f16"), (33, 256, 77, "q4_k", "f16"), (300, 256, 1000, "q4_k", "f32"), (130, 512, 264, "q4_k", "f16"),
+    (70, 128, 202, "q8_0", "f16"), (520, 256, 3, "q8_0", "f16"),
+]
+
+
+@pytest.mark.parametrize("inside", ["no copy", "forced"])
+@pytest.mark.parametrize("S,inn,out,kind,t", ODD_WIDTHS)
+def test_linear_act_any_width_without_the_half_copy(ctx, S, inn, out, kind, t, inside):
+    """Every output width is taken whether the products dequantize the base themselves or not, few rows and many."""
+    import torch
+    import sa3k
+    option, value = (sa3k.OPT_WEIGHT_F16_CACHE, 0) if inside == "no copy" else (sa3k.OPT_SMEM_DEQUANT, 1)
+    ctx.set_option(option, value)
+    try:
+        w, W = _weight(ctx, kind, inn, out, S + out)
+        rnd = _rand(S * 3 + out)
+        dt, D = _dt(t), torch.float64
+        x, bias, res, zin, dy = rnd(S, inn).to(dt), rnd(out), rnd(S, out).to(dt), rnd(S, out).to(dt), rnd(S, out).to(dt)
+        y, z, dx = (torch.full((S, n), float("nan"), device="cuda", dtype=dt) for n in (out, out, inn))
+        ctx.linear_act_fwd(w, x, y, "silu", bias=bias, residual=res, z=z)
+        ctx.linear_act_bwd(w, None, zin, dy, dx, "silu")
+        ctx.sync()
+    finally:
+        ctx.set_option(option, 1 - value)
+    # roundings as in test_linear_act: the weight and (f32) x to half, f32 sums, the result
+    eps = 2.0 ** -11 + (2.0 ** -11 if t == "f32" else 0.0)
+    small = 2.0 ** -25 if t == "f16" else 1e-30
+    zr = x.to(D) @ W.T + bias.to(D)
+    zt = (eps + inn * 2.0 ** -24) * (x.to(D).abs() @ W.T.abs() + bias.to(D).abs())
+    yr = ref.act(zr, "silu") + res.to(D)
+    ref.assert_within("z", z, zr, ref.u(dt) * zr.abs() + zt + small)
+    ref.assert_within("y", y, yr, ref.u(dt) * yr.abs() + 1.13 * zt + 2 ** -20 * (zr.abs() + yr.abs()) + small)
+    zz = zin.to(D).requires_grad_(True)
+    ref.act(zz, "silu").backward(dy.to(D))
+    dz = zz.grad
+    e2 = 2.0 ** -10 + out * 2.0 ** -24 + 2 ** -19
+    lost = (2 ** -25 + 2 ** -19) * W.abs().sum(0)
+    dxr = dz @ W
+    ref.assert_within("dx", dx, dxr, ref.u(dt) * dxr.abs() + e2 * (dz.abs() @ W.abs()) + lost * dy.abs().max().double() + small)
+
+
+@pytest.mark.parametrize("dora", [False, True])
+def test_linear_act_adapter_widths(ctx, dora):
+    """An adapter's backward takes widths of 8 and refuses others before it has written anything."""
+    import torch
+    import sa3k
+    for out in (72, 77):
+        w, W = _weight(ctx, "q8_0", 128, out, 5)
+        rnd = _rand(out)
+        A, Bm = rnd(16, 128) / 128 ** 0.5, 0.1 * rnd(out, 16)
+        bns, nrm = torch.empty(out, device="cuda"), torch.empty(out, device="cuda")
+        ctx.row_norms(w, 1e-12, bns, nrm)
+        m = 1.1 * nrm if dora else None
+        ad = ctx.adapter(A, Bm, 0.7, m, bns if dora else None)
+        x, dy = rnd(50, 128).half(), rnd(50, out).half()
+        y, z, dx = (torch.full((50, n), 9.0, device="cuda").half() for n in (out, out, 128))
+        ctx.linear_act_fwd(w, x, y, "silu", z=z, ad=ad)
+        leaves = [v.double().requires_grad_(True) for v in (x, A, Bm, *((m,) if dora else ()))]
+        V = W + 0.7 * leaves[2] @ leaves[1]
+        if dora:
+            V = V * (leaves[3] / ((V ** 2).sum(1) + 128 * 1e-12).sqrt())[:, None]
+        yr = ref.act(leaves[0] @ V.T, "silu")
+        rel = lambda a, b: float((a.double() - b).norm() / b.norm())  # noqa: E731
+        assert rel(y, yr.detach()) < 5 * 2.0 ** -11      # (half operands in a chain, see test_linear_act_with_adapter)
+        grads = [torch.full(s, 9.0, device="cuda") for s in ((out,), (16, 128), (out, 16), (out,))]
+        bwd = lambda: ctx.linear_act_bwd(w, x, z, dy, dx, "silu", dbias=grads[0], ad=ad, dA=grads[1], dB=grads[2],  # noqa: E731
+                                         dm=grads[3] if dora else None)
+        if out % 8:
+            with pytest.raises(sa3k.Sa3kError, match="multiple of 8"):
+                bwd()
+            ctx.sync()
+            assert all(bool((g == 9.0).all()) for g in (*grads, dx))
+            continue
+        bwd()
+        ctx.sync()
+        yr.backward(dy.double())
+        got = [dx, grads[1], grads[2], *((grads[3],) if dora else ())]
+        for g, leaf in zip(got, leaves):
+            assert rel(g, leaf.grad) < 5 * 2.0 ** -11
