@@ -8,6 +8,7 @@
 #include "materialize.h"
 #include "sa3k_common.cuh"
 
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
 #include <cstring>
@@ -24,8 +25,10 @@ static int fill_err(char* err, int len, const std::string& msg) {
   return 1;
 }
 
-// A buffer whose address went into a stream capture is never freed before the context: when it is
-// outgrown it is retired, since the captured graph may be replayed at any later time.
+// A buffer whose address went into the caller's stream capture is never freed before the context: when
+// it is outgrown it is retired, since the captured graph may be replayed at any later time.  Its successor is
+// half as large again at least, so that what captures of ever larger sizes hold is a few times the largest.
+// The library's own recorded graphs (`recording`) are made anew when the generation changes and hold nothing.
 void* scratch_get(Ctx* c, int slot, size_t bytes, std::string& err) {
   if ((int)c->scratch.size() <= slot) c->scratch.resize((size_t)slot + 1);
   Scratch& s = c->scratch[(size_t)slot];
@@ -33,21 +36,28 @@ void* scratch_get(Ctx* c, int slot, size_t bytes, std::string& err) {
   const bool capturing = cudaStreamIsCapturing(c->stream, &cs) == cudaSuccess && cs != cudaStreamCaptureStatusNone;
   if (s.bytes < bytes) {
     ++c->gen;   // recorded graphs may hold the old buffer
+    size_t want = (bytes + 255) & ~(size_t)255, more = want;
     if (s.ptr) {
       if (s.captured || capturing) {
         c->retired.push_back(s.ptr);
+        more = std::max(want, (s.bytes + s.bytes / 2 + 255) & ~(size_t)255);
       } else {
         cudaStreamSynchronize(c->stream);
         cudaFree(s.ptr);
       }
       s = Scratch{};
     }
-    const size_t want = (bytes + 255) & ~(size_t)255;
     // (an allocation is no work of the stream: it may be made beside a capture, which without this would
     // be invalidated)
     cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
     if (capturing) cudaThreadExchangeStreamCaptureMode(&mode);
-    const cudaError_t e = cudaMalloc(&s.ptr, want);
+    cudaError_t e = cudaMalloc(&s.ptr, more);
+    if (e == cudaSuccess) {
+      want = more;
+    } else if (more > want) {
+      cudaGetLastError();
+      e = cudaMalloc(&s.ptr, want);
+    }
     if (capturing) cudaThreadExchangeStreamCaptureMode(&mode);
     if (e != cudaSuccess) {
       cudaGetLastError();
@@ -57,7 +67,7 @@ void* scratch_get(Ctx* c, int slot, size_t bytes, std::string& err) {
     }
     s.bytes = want;
   }
-  if (capturing) s.captured = true;
+  if (capturing && !c->recording) s.captured = true;
   return s.ptr;
 }
 

@@ -1150,8 +1150,10 @@ static int run_step(DitModel& m, std::string& err) {
     return dit_step(m, err);
   }
   c->stream = m.cap_stream;
+  c->recording = true;
   std::string e2;
   const int rc = dit_step(m, e2);
+  c->recording = false;
   c->stream = user;
   cudaGraph_t g = nullptr;
   const cudaError_t ce = cudaStreamEndCapture(m.cap_stream, &g);

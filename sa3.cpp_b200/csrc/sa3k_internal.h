@@ -64,6 +64,7 @@ struct Ctx {
   int* split_cnt = nullptr;          // [kSplitCounters] split-K tile counters, zero between launches
   std::vector<Scratch> scratch;      // indexed by the slot enums of the callers
   std::vector<void*> retired;        // outgrown scratch that a captured graph may still address
+  bool recording = false;            // the capture under way is the library's own (the DiT step's graph)
   size_t sm_count = 148;
   bool timing = false;
   bool timing_graph = false;         // timing events live in a captured CUDA graph

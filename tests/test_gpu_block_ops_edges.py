@@ -230,3 +230,68 @@ def test_linear_act_adapter_widths(ctx, dora):
         got = [dx, grads[1], grads[2], *((grads[3],) if dora else ())]
         for g, leaf in zip(got, leaves):
             assert rel(g, leaf.grad) < 5 * 2.0 ** -11
+
+
+# ------------------------------------------------------------------------------- scratch and captures
+def _used():
+    import torch
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    free, total = torch.cuda.mem_get_info()
+    return total - free
+
+
+def test_scratch_of_captures_that_grow(ctx):
+    """Captured calls of ever larger sizes hold a few times the largest one's scratch, not the sum of all."""
+    import torch
+    own, side = _own_context()
+    try:
+        with torch.cuda.stream(side):
+            w, _ = _weight(own, "f16", 64, 2048, 3)
+        top = 12000
+        z, dy = (torch.zeros(top, 2048, device="cuda").half() for _ in range(2))
+        dx, db = torch.zeros(top, 64, device="cuda").half(), torch.zeros(2048, device="cuda")
+        call = lambda s: own.linear_act_bwd(w, None, z[:s], dy[:s], dx[:s], "silu", dbias=db)  # noqa: E731
+        torch.cuda.synchronize()
+        call(64)
+        own.sync()
+        before, graphs = _used(), []
+        for s in range(2000, top + 1, 500):
+            graphs.append(_capture(side, lambda s=s: call(s)))
+        held = _used() - before
+        largest = top * 2048 * 2 + (top // 16 + 1) * 2 * 2048 * 4           # dz in half, partial column sums
+        assert held < 4 * largest, (held, largest)
+        with torch.cuda.stream(side):
+            for g in graphs:
+                g.replay()
+        own.sync()
+        graphs.clear()
+    finally:
+        own.close()
+
+
+def test_step_graph_gives_its_scratch_back(ctx):
+    """The DiT step's own recorded graph is made anew when its scratch grows: the old scratch is freed."""
+    import test_gpu_dit as dit_test
+    import sa3k
+
+    def run(lengths):
+        own = sa3k.Context(0, use_torch_stream=False)
+        try:
+            start = _used()
+            dit, _, _, _, rng = dit_test._build(own, dict(dit_test.CFG, depth=1))
+            for T in lengths:
+                f32 = lambda *s: rng.standard_normal(s).astype(np.float32)  # noqa: E731
+                ins = f32(1, T, 64), f32(1, T, 64), f32(1, 64), f32(1, 16, 64), f32(1, 64)
+                for _ in range(3):           # eager, recorded, replayed
+                    dit.forward_backward(1, T, 16, *ins, loss=np.zeros(1, np.float32))
+            own.sync()
+            return _used() - start
+        finally:
+            own.close()
+
+    lengths = list(range(4000, 12001, 1000))
+    run(lengths[:1])                                       # (modules are loaded)
+    alone, grown = run(lengths[-1:]), run(lengths)
+    # the rotation table alone is 512 bytes a token: 32 MB over the shorter lengths
+    assert grown - alone < 12 << 20, (grown, alone)
