@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 256, BLOCK && NV == 1 && VEC ? 
   const float rs = ln_rstd(row_sum2<BLOCK>(q, sd, tpr, red, 1), a, off);
   if (!ok) return;
   if (t == 0) {
-    if (a.mean) a.mean[r] = mu + off;
+    if (a.mean) a.mean[r] = isfinite(off) ? mu + off : mu;     // (a row with an infinity has that mean)
     if (a.rstd) a.rstd[r] = rs;
   }
   TY* y = static_cast<TY*>(a.out) + r * a.out_ld;
@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(1024) ln_fwd_long_kernel(const LnArgs a) {
   float off;
   const float rs = ln_rstd(row_sum2<true>(q, sd, 0, red, 1), a, off);
   if (threadIdx.x == 0) {
-    if (a.mean) a.mean[r] = mu + off;
+    if (a.mean) a.mean[r] = isfinite(off) ? mu + off : mu;     // (a row with an infinity has that mean)
     if (a.rstd) a.rstd[r] = rs;
   }
   TY* y = static_cast<TY*>(a.out) + r * a.out_ld;

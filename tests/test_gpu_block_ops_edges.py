@@ -148,6 +148,31 @@ def test_layernorm_offset_costs_no_digits(ctx, cols, offset):
     ref.assert_within("rstd", rstd, w["rstd"], w["rstd"] * (2 * c * wide ** 2 + 2 ** -21))
 
 
+@pytest.mark.parametrize("cols", [7, 200, 1000, 1536, 1537, 9000, 40000])
+def test_layernorm_rows_that_are_not_finite(ctx, cols):
+    """An infinity or a NaN spoils its own row and no other, forward and backward."""
+    import torch
+    rnd = _rand(cols)
+    x, dy, gamma, beta = rnd(9, cols), rnd(9, cols), 1 + 0.1 * rnd(cols), rnd(cols)
+    bad = x.clone()
+    bad[1, cols // 2], bad[4, 0], bad[7, cols - 1] = float("inf"), float("nan"), float("-inf")
+    rows = torch.tensor([1, 4, 7], device="cuda")
+    rest = torch.tensor([0, 2, 3, 5, 6, 8], device="cuda")
+
+    def run(t):
+        y, dx, mean, rstd = torch.empty_like(t), torch.empty_like(t), torch.empty(9, device="cuda"), torch.empty(9, device="cuda")
+        ctx.layernorm_fwd(t, y, gamma, beta, 1e-5, mean, rstd)
+        ctx.layernorm_bwd(t, dy, dx, mean, rstd, gamma)
+        ctx.sync()
+        return y, mean, rstd, dx
+
+    for got, want in zip(run(bad), run(x)):
+        assert torch.equal(got[rest], want[rest])
+    y, mean, rstd, dx = run(bad)
+    assert bool(y[rows].isnan().all()) and bool(rstd[rows].isnan().all()) and bool(dx[rows].isnan().all())
+    assert float(mean[1]) == float("inf") and bool(mean[4].isnan()) and float(mean[7]) == float("-inf")
+
+
 # ------------------------------------------------------------------------ widths of quantized bases
 ODD_WIDTHS = [  # S, in, out, weight, type
     (5, 128, 77, "q8_0", "f16"), (33, 128, 77, "q8_0", "f16"), (200, 192, 129, "q8_0", "f32"), (40, 128, 520, "q8_0", "f16"),
