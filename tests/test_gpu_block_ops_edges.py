@@ -173,6 +173,34 @@ def test_layernorm_rows_that_are_not_finite(ctx, cols):
     assert float(mean[1]) == float("inf") and bool(mean[4].isnan()) and float(mean[7]) == float("-inf")
 
 
+# ------------------------------------------------------- the layer norm backward's ring of rows
+RING = [  # rows, cols: every block refills its slots several times; each of the kernel's forms; odd last pairs
+    (30001, 264), (9999, 768), (7001, 1536), (4003, 2048), (2500, 2560), (3001, 4096), (1999, 5120), (2001, 5128), (1201, 8192),
+    (296, 8192), (150, 8192),
+]
+
+
+@pytest.mark.parametrize("rows,cols", RING)
+@pytest.mark.parametrize("xt,yt", [("f32", "f16"), ("f16", "f16"), ("bf16", "f32"), ("f32", "f32")])
+def test_layernorm_backward_of_many_rows(ctx, rows, cols, xt, yt):
+    import torch
+    rnd = _rand(rows + cols)
+    x, gamma = (rnd(rows, cols) + 0.5 * rnd(cols)).to(_dt(xt)), 1 + 0.3 * rnd(cols)
+    dy = rnd(rows, cols).to(_dt(yt))
+    mean, rstd = x.double().mean(1).float(), (x.double().var(1, unbiased=False) + 1e-5).rsqrt().float()
+    dx = torch.full_like(x, float("nan"))
+    dg, db = (torch.full((cols,), float("nan"), device="cuda") for _ in range(2))
+    ctx.layernorm_bwd(x, dy, dx, mean, rstd, gamma, dg, db)
+    g = ref.layernorm_grads(x, dy, gamma, mean, rstd, 74, 64 + rows // 64)
+    for n, got in (("dx", dx), ("dgamma", dg), ("dbeta", db)):
+        ref.assert_within(n, got, g[n], g[n + "_tol"])
+    again = torch.empty_like(dx)
+    dg2, db2 = torch.ones_like(dg), torch.ones_like(db)
+    ctx.layernorm_bwd(x, dy, again, mean, rstd, gamma, dg2, db2, accumulate=True)
+    ctx.sync()
+    assert torch.equal(again, dx) and torch.equal(dg2, dg + 1) and torch.equal(db2, db + 1)
+
+
 # ------------------------------------------------------------------------ widths of quantized bases
 ODD_WIDTHS = [  # S, in, out, weight, type
     (5, 128, 77, "q8_0", "f16"), (33, 128, 77, "q8_0", "f16"), (200, 192, 129, "q8_0", "f32"), (40, 128, 520, "q8_0", "f16"),
@@ -320,3 +348,62 @@ def test_step_graph_gives_its_scratch_back(ctx):
     alone, grown = run(lengths[-1:]), run(lengths)
     # the rotation table alone is 512 bytes a token: 32 MB over the shorter lengths
     assert grown - alone < 12 << 20, (grown, alone)
+
+
+# --------------------------------------------------------------------- the same bits, and replays
+@pytest.mark.parametrize("kw", [
+    dict(B=1, H=1, Hkv=1, Sq=1, Sk=20011, left=-1, right=0, sinks=0, end=True),              # clusters of 16
+    dict(B=2, H=24, Hkv=8, Sq=1, Sk=3000, left=800, right=0, sinks=64, end=True, dtype="bf16"),
+    dict(B=1, H=3, Hkv=3, Sq=40, Sk=900, left=300, right=0, sinks=4, end=True),
+    dict(B=2, H=24, Hkv=8, Sq=600, Sk=600, left=200, right=0, sinks=30, dtype="bf16"),
+])
+def test_attention_sink_repeats_and_replays(ctx, kw):
+    """Twenty calls give the same bits; a captured call gives them too, on inputs that came after the capture."""
+    import torch
+    own, side = _own_context()
+    try:
+        a = Attn(**kw, seed=31)
+        torch.cuda.synchronize()
+        a.fwd(own)
+        a.bwd(own)
+        own.sync()
+        g = _capture(side, lambda: (a.fwd(own), a.bwd(own)))
+        with torch.cuda.stream(side):
+            a.q.copy_(a.q.flip(1)), a.v.neg_()
+            a.fwd(own)
+            a.bwd(own)
+            first = [t.clone() for t in (a.o, a.lse, a.dq, a.dk, a.dv)]
+            for i in range(20):
+                for t in (a.o, a.lse, a.dq, a.dk, a.dv):
+                    t.fill_(9.0)
+                if i % 2:
+                    g.replay()
+                else:
+                    a.fwd(own)
+                    a.bwd(own)
+                for x, y in zip(first, (a.o, a.lse, a.dq, a.dk, a.dv)):
+                    assert torch.equal(x, y)
+        own.sync()
+        a.check()
+    finally:
+        own.close()
+
+
+@pytest.mark.parametrize("S,inn,out", [(1, 1536, 6144), (33, 1536, 6144), (20, 4096, 128), (1100, 1536, 1544), (4352, 512, 1536)])
+def test_linear_act_repeats(ctx, S, inn, out):
+    """Few rows, split-K and pair tiles: the same bits every time (without an adapter, whose gradients use atomics)."""
+    import torch
+    w, _ = _weight(ctx, "q8_0", inn, out, 3)
+    rnd = _rand(S)
+    x, res, dy, bias = rnd(S, inn).half(), rnd(S, out).half(), rnd(S, out).half(), rnd(out)
+    runs = []
+    for _ in range(6):
+        y, z, dx = (torch.full((S, n), float("nan"), device="cuda").half() for n in (out, out, inn))
+        db = torch.empty(out, device="cuda")
+        ctx.linear_act_fwd(w, x, y, "gelu_tanh", bias=bias, residual=res, z=z)
+        ctx.linear_act_bwd(w, None, z, dy, dx, "gelu_tanh", dbias=db)
+        runs.append((y, z, dx, db))
+    ctx.sync()
+    for other in runs[1:]:
+        for a, b in zip(runs[0], other):
+            assert torch.equal(a, b)
