@@ -145,7 +145,6 @@ __global__ void __launch_bounds__(kFwdThreads, 3)
     sink_fwd_kernel(const __grid_constant__ SeqMap mq, const __grid_constant__ SeqMap mk, const __grid_constant__ SeqMap mv,
                     const __grid_constant__ SinkArgs a) {
   extern __shared__ uint8_t smem_raw[];
-  pdl_trigger();
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;
   uint8_t* sP = smem + 16384;
@@ -187,6 +186,7 @@ __global__ void __launch_bounds__(kFwdThreads, 3)
   }
   __syncthreads();
   tc_fence_after();
+  pdl_trigger();   // (tensor memory is taken: see pdl_trigger)
   const uint32_t tbase = (uint32_t)uniform((int)*tmem_slot);
   pdl_wait();
 
@@ -381,7 +381,6 @@ __global__ void __launch_bounds__(kSinkThreads, 2)
     sink_dq_kernel(const __grid_constant__ SeqMap mq, const __grid_constant__ SeqMap mdo, const __grid_constant__ SeqMap mo,
                    const __grid_constant__ SeqMap mk, const __grid_constant__ SeqMap mv, const __grid_constant__ SinkArgs a) {
   extern __shared__ uint8_t smem_raw[];
-  pdl_trigger();
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;                   // Q 16 KB | dO 16 KB | O 16 KB
   uint8_t* sKV = smem + 49152;
@@ -426,6 +425,7 @@ __global__ void __launch_bounds__(kSinkThreads, 2)
   }
   __syncthreads();
   tc_fence_after();
+  pdl_trigger();   // (tensor memory is taken: see pdl_trigger)
   const uint32_t tbase = (uint32_t)uniform((int)*tmem_slot);
   pdl_wait();
 
@@ -606,7 +606,6 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
     sink_dkdv_kernel(const __grid_constant__ SeqMap mk, const __grid_constant__ SeqMap mv, const __grid_constant__ SeqMap mq,
                      const __grid_constant__ SeqMap mdo, const __grid_constant__ SinkArgs a) {
   extern __shared__ uint8_t smem_raw[];
-  pdl_trigger();
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sKV = smem;                                  // [2] K | V
   uint8_t* sQd = smem + 65536;                          // [kDkvStages] Q | dO
@@ -663,6 +662,7 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
   }
   __syncthreads();
   tc_fence_after();
+  pdl_trigger();   // (tensor memory is taken: see pdl_trigger)
   const uint32_t tbase = (uint32_t)uniform((int)*tmem_slot);
   pdl_wait();
   const Waiter wait{abort_flag, a.err};

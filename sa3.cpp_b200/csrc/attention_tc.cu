@@ -149,7 +149,6 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
     attn_tc_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v, const TcArgs a) {
   extern __shared__ uint8_t smem_raw[];
-  pdl_trigger();   // the next kernel may be scheduled once every CTA of this grid runs
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;
   uint8_t* sKV = smem + 32768;
@@ -203,6 +202,7 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
   }
   __syncthreads();
   tc_fence_after();
+  pdl_trigger();   // (tensor memory is taken: see pdl_trigger)
   const uint32_t tbase = *tmem_slot;
   pdl_wait();      // outputs of earlier kernels are read only from here on
   const Waiter wait{abort_flag, a.err};     // single-thread roles (the TMA producer)
@@ -426,7 +426,6 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
                       const __grid_constant__ CUtensorMap tm_o, const __grid_constant__ CUtensorMap tm_dq,
                       const TcArgs a) {
   extern __shared__ uint8_t smem_raw[];
-  pdl_trigger();   // the next kernel may be scheduled once every CTA of this grid runs
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQd = smem;                  // [2 items][Q 16 KB | dO 16 KB | O 16 KB]
   uint8_t* sKV = smem + 98304;
@@ -483,6 +482,7 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
   }
   __syncthreads();
   tc_fence_after();
+  pdl_trigger();   // (tensor memory is taken: see pdl_trigger)
   const uint32_t tbase = *tmem_slot;
   pdl_wait();      // outputs of earlier kernels are read only from here on
   const Waiter wait{abort_flag, a.err};     // single-thread roles (the TMA producer)
@@ -743,7 +743,6 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
                         const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
                         const TcArgs a) {
   extern __shared__ uint8_t smem_raw[];
-  pdl_trigger();   // the next kernel may be scheduled once every CTA of this grid runs
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sK = smem;
   uint8_t* sV = smem + 16384;
@@ -794,6 +793,7 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
   }
   __syncthreads();
   tc_fence_after();
+  pdl_trigger();   // (tensor memory is taken: see pdl_trigger)
   const uint32_t tbase = *tmem_slot;
   pdl_wait();      // outputs of earlier kernels are read only from here on
   const uint32_t tV = tbase + 384, tK = tbase + 448;
@@ -992,7 +992,6 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
     attn_short_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                           const __grid_constant__ CUtensorMap tm_v, const TcArgs a) {
   extern __shared__ uint8_t smem_raw[];
-  pdl_trigger();
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sstg = smem + 2 * SF_BUF;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sstg + SF_STG);
@@ -1039,6 +1038,7 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
   }
   __syncthreads();
   tc_fence_after();
+  pdl_trigger();   // (tensor memory is taken: see pdl_trigger)
   const uint32_t tbase = *tmem_slot;
   pdl_wait();
   const Waiter wait{abort_flag, a.err};
@@ -1213,7 +1213,6 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
                          const __grid_constant__ CUtensorMap tm_o, const __grid_constant__ CUtensorMap tm_k,
                          const __grid_constant__ CUtensorMap tm_v, const TcArgs a) {
   extern __shared__ uint8_t smem_raw[];
-  pdl_trigger();
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sstg = smem + 2 * SQ_BUF;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sstg + SQ_STG);
@@ -1262,6 +1261,7 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
   }
   __syncthreads();
   tc_fence_after();
+  pdl_trigger();   // (tensor memory is taken: see pdl_trigger)
   const uint32_t tbase = *tmem_slot;
   pdl_wait();
   const Waiter wait{abort_flag, a.err};

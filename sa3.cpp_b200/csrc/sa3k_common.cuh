@@ -46,6 +46,10 @@ __device__ __forceinline__ void record_error(int* err, int code) {
 // scheduled once every CTA of this grid has started; pdl_wait blocks until the previous grid has
 // completed and its memory is visible, so nothing that a predecessor writes may be read before
 // it.  Without the launch attribute both are no-ops.
+// A kernel that takes tensor memory and leaves room on its SM for another that does (the attention
+// kernels, from 67 KB of shared memory a CTA on) triggers only when it has it.  Otherwise a successor's CTA
+// could take the columns first and wait for this grid, which would wait for the columns.  (The GEMM
+// kernels, above 176 KB each, share an SM with none of these.)
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_prologue() {

@@ -407,3 +407,23 @@ def test_linear_act_repeats(ctx, S, inn, out):
     for other in runs[1:]:
         for a, b in zip(runs[0], other):
             assert torch.equal(a, b)
+
+
+def test_dense_and_windowed_attention_in_turn(ctx):
+    """Kernels of 512, 256 and 128 tensor-memory columns follow one another on one stream, each started early."""
+    import torch
+    a = Attn(1, 16, 16, 500, 500, 100, 100, 0, token_major=False, seed=41)
+    o2, lse2 = torch.empty_like(a.q), torch.empty(16 * 500, device="cuda")
+    grads = [torch.empty(1, 16, 500, 64, device="cuda") for _ in range(3)]
+    for _ in range(30):
+        a.fwd(ctx)
+        ctx.attention_fwd(1, 16, 500, 500, 0.125, 100, a.t4(a.q), a.t4(a.k), a.t4(a.v), a.t4(o2), lse2)
+        a.bwd(ctx)
+        ctx.attention_bwd(1, 16, 500, 500, 0.125, 100, a.t4(a.q), a.t4(a.k), a.t4(a.v), a.t4(o2), a.t4(a.dO), lse2,
+                          *(a.t4(t) for t in grads))
+    ctx.sync()
+    a.check()
+    assert float((a.o.double() - o2.double()).norm() / o2.double().norm()) < 1e-3   # two roundings of P and o each
+    for mine, dense in zip((a.dq, a.dk, a.dv), grads):
+        # P, dS and the gradient rounded to half on this side, P and dS on the other
+        assert float((mine.double() - dense.double()).norm() / dense.double().norm()) < 3e-3
