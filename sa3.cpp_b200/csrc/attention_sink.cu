@@ -617,8 +617,10 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
   uint64_t* kv_empty = kv_full + 2;                     // [2] the item's last scores are done
   uint64_t* q_full = kv_empty + 2;
   uint64_t* q_empty = q_full + kDkvStages;              // dV and dK of the slot's tile are done
-  uint64_t* s_full = q_empty + kDkvStages;              // [3]
-  uint64_t* ds_full = s_full + 3;                       // [3]
+  // scores of a step are there: [6], a barrier per buffer and set.  With one per buffer a set would look at
+  // every second phase only, and could not tell the next phase but one from the last it saw
+  uint64_t* s_full = q_empty + kDkvStages;
+  uint64_t* ds_full = s_full + 3 * kDkvSets;            // [3]
   uint64_t* g_done = ds_full + 3;                       // [3] dV and dK of the buffer's step are done
   uint64_t* acc_full = g_done + 3;
   uint64_t* acc_empty = acc_full + 1;
@@ -637,8 +639,8 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
     }
+    for (int i = 0; i < 3 * kDkvSets; ++i) mbar_init(&s_full[i], 1);
     for (int i = 0; i < 3; ++i) {
-      mbar_init(&s_full[i], 1);
       mbar_init(&ds_full[i], 8);
       mbar_init(&g_done[i], 1);
     }
@@ -736,11 +738,12 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
     // Two warps issue the products, one the scores (up to three steps ahead), one the gradients: the
     // waits and the issue of all 16 products of a step in one warp took 1700 clocks, more than the softmax.
     const bool grads = warp == kDkvWarps + 2;
-    int st = 0, u = 0;                       // ring slot and buffer of the step, with the parity of their use
+    int st = 0, u = 0, f = 0;                // ring slot, buffer and barrier of the step, with the parity of their use
     uint32_t st_ph = 0, u_ph = 0;
     auto step = [&]() {
       if (++st == kDkvStages) { st = 0; st_ph ^= 1u; }
       if (++u == 3) { u = 0; u_ph ^= 1u; }
+      if (++f == 3 * kDkvSets) f = 0;
     };
     bool ok = true;
     int t = 0;
@@ -762,7 +765,7 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
           const uint32_t qa = smem_u32(sQd) + st * 2 * kTile, tS = tbase + 128 * u;
           umma4_ss_w<2, 2>(tS, kd, kdesc0(qa), id_s, 0u);
           umma4_ss_w<2, 2>(tS + 64, vd, kdesc0(qa + kTile), id_s, 0u);
-          umma_commit_w(&s_full[u]);
+          umma_commit_w(&s_full[f]);
           step();
         }
         if (ok) umma_commit_w(&kv_empty[kb]);
@@ -828,7 +831,8 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
         wrap();
         if (j + 2 < n) next = fetch(h, q);
         __syncwarp();
-        if (!waitw(&s_full[u], (uint32_t)((t / 3) & 1), kErrTimeoutAccum)) { ok = false; break; }
+        constexpr int F = 3 * kDkvSets;
+        if (!waitw(&s_full[t % F], (uint32_t)((t / F) & 1), kErrTimeoutAccum)) { ok = false; break; }
         tc_fence_after();
         // queries of the tile that see key kj: position from kj - right to kj + left (any, for a sink)
         const bool edge = !whole || q0 + 64 > qn || pq < e0 || pq >= e1;

@@ -28,3 +28,20 @@ def test_attention_kernels_trigger_with_tensor_memory_in_hand():
                 assert m.start() > barrier, f"{name}: {kernel} triggers before it has its tensor memory"
             assert "pdl_trigger()" in body and body.index("pdl_trigger()") < body.index("pdl_wait()"), kernel
     assert seen == 8
+
+
+def test_dkdv_sets_see_every_phase_of_the_barriers_they_wait_on():
+    """Two sets of warps take alternate steps; a set that waited on every second phase of a barrier could take an
+    older phase for the one it waits for (the parity is the same)."""
+    body = dict(_kernels("attention_sink.cu"))["sink_dkdv_kernel"]
+    const = {n: int(v) for n, v in re.findall(r"(kDkvSets|kDkvStages|kDkvItems) = (\d+)", open(os.path.join(CSRC, "attention_sink.cu")).read())}
+    period, phase = re.search(r"waitw\(&s_full\[t % (\w+)\], \(uint32_t\)\(\(t / (\w+)\) & 1\)", body).groups()
+    assert period == phase
+    expr = re.search(r"constexpr int " + period + r" = ([^;]+);", body).group(1)
+    F = eval(expr, {}, const)
+    last = {}
+    for t in range(20 * F):
+        who = t % const["kDkvSets"], t % F          # the set of step t, the barrier it waits on
+        assert t // F == last.get(who, -1) + 1, who
+        last[who] = t // F
+    assert f"for (int i = 0; i < {expr}; ++i) mbar_init(&s_full[i], 1)" in body
