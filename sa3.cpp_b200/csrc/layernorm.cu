@@ -25,9 +25,9 @@
 namespace sa3k {
 namespace {
 
-// out[i] (+)= sum over b of part[b][which][i]: a block takes 8 columns (a 32-byte sector) in 64 slices of
-// the partial rows, which are then added in order.
-__global__ void __launch_bounds__(512) fold_partials_kernel(const float* part, int nblocks, int cols, float* out0,
+// out[i] (+)= sum over b of part[b][which][i], `planes` of them per b: a block takes 8 columns (a 32-byte
+// sector) in 64 slices of the partial rows, which are then added in order.
+__global__ void __launch_bounds__(512) fold_partials_kernel(const float* part, int nblocks, int planes, int cols, float* out0,
                                                             float* out1, int acc0, int acc1) {
   __shared__ float s[8][65];
   pdl_prologue();
@@ -38,7 +38,7 @@ __global__ void __launch_bounds__(512) fold_partials_kernel(const float* part, i
   float v = 0.f;
   if (i < cols) {
 #pragma unroll 4
-    for (int b = w; b < nblocks; b += 64) v += p[(long)b * 2 * cols];
+    for (int b = w; b < nblocks; b += 64) v += p[(long)b * planes * cols];
   }
   s[e][w] = v;
   __syncthreads();
@@ -51,11 +51,11 @@ __global__ void __launch_bounds__(512) fold_partials_kernel(const float* part, i
 
 }  // namespace
 
-int k_fold_partials(Ctx* c, const float* part, int nblocks, int cols, float* out0, float* out1, int acc0, int acc1,
-                    std::string& err) {
+int k_fold_partials(Ctx* c, const float* part, int nblocks, int planes, int cols, float* out0, float* out1, int acc0,
+                    int acc1, std::string& err) {
   ProfScope prof_(c, "fold_partials");
-  launch_pdl(c, fold_partials_kernel, dim3((unsigned)((cols + 7) / 8), 2), dim3(512), 0, part, nblocks, cols, out0, out1,
-             acc0, acc1);
+  launch_pdl(c, fold_partials_kernel, dim3((unsigned)((cols + 7) / 8), (unsigned)planes), dim3(512), 0, part, nblocks, planes,
+             cols, out0, out1, acc0, acc1);
   return check_launch("fold partials", err);
 }
 
@@ -718,7 +718,7 @@ int bwd_typed(Ctx* c, LnArgs a, bool vec, float* dgamma, float* dbeta, int accum
     rc = vec ? bwd_launch<TX, TY, true, 4, true>(c, a, s, blocks, err) : bwd_launch<TX, TY, true, 4, false>(c, a, s, blocks, err);
   }
   if (rc || !params) return rc;
-  return k_fold_partials(c, a.part, blocks, a.cols, dgamma, dbeta, accumulate, accumulate, err);
+  return k_fold_partials(c, a.part, blocks, 2, a.cols, dgamma, dbeta, accumulate, accumulate, err);
 }
 
 // type-erased dispatch over the nine (x, y) type pairs

@@ -76,7 +76,7 @@ int act_splits(Ctx* c, const GemmDesc& d, const float* partial, int splits, T* y
 }
 
 // dz = f16(g dy act'(z)), and with part the partial column sums over the block's kActRows rows:
-// part[blockIdx.y][0] of dy act'(z) (the bias gradient), [1] of dy act'(z) (z - bias) / g (dora's dg).
+// part[blockIdx.y][0] of dy act'(z) (the bias gradient), with DORA [1] of dy act'(z) (z - bias) / g (dora's dg).
 // One pass: dy and z are read and dz is written once, in 16-byte accesses of 8 columns a thread (VEC)
 // or one column a thread (widths and bases that allow none).  Bound by memory: 2047 x 6144 f16 moves
 // 75 MB.
@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(128) act_bwd_kernel(const T* __restrict__ dy, 
     }
   }
   if (!part) return;
-  float* p = part + (long)blockIdx.y * 2 * out + o;
+  float* p = part + (long)blockIdx.y * (DORA ? 2 : 1) * out + o;
 #pragma unroll
   for (int e = 0; e < W; ++e) {
     p[e] = sb[e];
@@ -271,11 +271,11 @@ int linear_act_backward(Ctx* c, const Weight* w, const sa3k_adapter* ad, const f
   }
   const int64_t dz_ld = (out + 7) / 8 * 8;   // (TMA reads rows that start on 16 bytes)
   // scratch: dz | dut | dg | cb | c3 | partial sums
-  const int chunks = (int)((S + kActRows - 1) / kActRows);
+  const int chunks = (int)((S + kActRows - 1) / kActRows), planes = dora ? 2 : 1;
   const bool sums = dbias || dora;
   const size_t b_dz = al((size_t)(S * dz_ld) * 2), b_dut = ad ? al((size_t)(16 * pad64(S)) * 2) : 0,
                b_dg = dora ? al((size_t)out * 4) : 0, b_cb = dora ? al((size_t)(16 * out) * 2) : 0, b_c3 = dora ? al(1024) : 0,
-               b_part = sums ? al((size_t)chunks * 2 * out * 4) : 0;
+               b_part = sums ? al((size_t)chunks * planes * out * 4) : 0;
   char* mem = static_cast<char*>(scratch_get(c, kSlotActPart, b_dz + b_dut + b_dg + b_cb + b_c3 + b_part, err));
   if (!mem) return 1;
   LinearBwd b;
@@ -290,7 +290,7 @@ int linear_act_backward(Ctx* c, const Weight* w, const sa3k_adapter* ad, const f
   if (type == kTypeF16 ? act_bwd<__half>(c, dy, z, bias, g, act, S, out, b.dz, dz_ld, part, err)
                        : act_bwd<float>(c, dy, z, bias, g, act, S, out, b.dz, dz_ld, part, err))
     return 1;
-  if (sums && k_fold_partials(c, part, chunks, (int)out, dbias, dora ? b.dg : nullptr, accumulate, 0, err)) return 1;
+  if (sums && k_fold_partials(c, part, chunks, planes, (int)out, dbias, dora ? b.dg : nullptr, accumulate, 0, err)) return 1;
   b.dz_ready = true;
   b.dz_ld = dz_ld;
   if (type == kTypeF16) b.dx_h = static_cast<__half*>(dx);

@@ -48,10 +48,10 @@ int api_call(sa3k_ctx* ctx, char* err, int len, F&& fn) {
   }
 }
 
-// out0[i] (+)= sum over b of part[b][0][i], out1[i] (+)= sum over b of part[b][1][i] (either may be
-// null), summed in a fixed order (layernorm.cu)
-int k_fold_partials(Ctx* c, const float* part, int nblocks, int cols, float* out0, float* out1, int acc0, int acc1,
-                    std::string& err);
+// out0[i] (+)= sum over b of part[b][0][i] and, of two planes, out1[i] (+)= sum over b of part[b][1][i]
+// (either may be null), summed in a fixed order (layernorm.cu)
+int k_fold_partials(Ctx* c, const float* part, int nblocks, int planes, int cols, float* out0, float* out1, int acc0,
+                    int acc1, std::string& err);
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 

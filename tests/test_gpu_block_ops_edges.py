@@ -350,6 +350,28 @@ def test_step_graph_gives_its_scratch_back(ctx):
     assert grown - alone < 12 << 20, (grown, alone)
 
 
+def test_linear_act_backward_scratch(ctx):
+    """The partial sums of a backward without a dora adapter take one plane of S / 16 rows."""
+    import torch
+    own, side = _own_context()
+    try:
+        with torch.cuda.stream(side):
+            w, _ = _weight(own, "f16", 64, 4096, 3)
+        S = 64000
+        z, dy = (torch.zeros(S, 4096, device="cuda").half() for _ in range(2))
+        dx, db = torch.zeros(S, 64, device="cuda").half(), torch.zeros(4096, device="cuda")
+        torch.cuda.synchronize()
+        own.linear_act_bwd(w, None, z[:64], dy[:64], dx[:64], "silu", dbias=db)
+        own.sync()
+        before = _used()
+        own.linear_act_bwd(w, None, z, dy, dx, "silu", dbias=db)
+        own.sync()
+        held, plane = _used() - before, S // 16 * 4096 * 4
+        assert held < S * 4096 * 2 + plane + plane // 2, (held, plane)
+    finally:
+        own.close()
+
+
 # --------------------------------------------------------------------- the same bits, and replays
 @pytest.mark.parametrize("kw", [
     dict(B=1, H=1, Hkv=1, Sq=1, Sk=20011, left=-1, right=0, sinks=0, end=True),              # clusters of 16
