@@ -288,7 +288,7 @@ typedef struct sa3k_tensor4 {
 
 /* o = softmax(scale * q k^T [+ band mask]) v per (batch, head), head_dim 64; q, k, v, o f16 (IEEE half).
  * window < 0: dense (the DiT's sdpa); window >= 0: keys with |i - j| <= window only (the banded
- * attention of BASELINE config 3).  lse [B*H][Sq] (f32, log2 units) is kept for the backward.
+ * attention of the audio transformer: 2048 frames, 256 to each side).  lse [B*H][Sq] (f32, log2 units) is kept for the backward.
  * Replaces nn::sdpa (src/nn.h:135-144) and the band of attn_sliding (src/nn.h:79-100). */
 int sa3k_attention_fwd(sa3k_ctx* ctx, int B, int H, int Sq, int Sk, int head_dim, float scale,
                        int window, const sa3k_tensor4* q, const sa3k_tensor4* k,
@@ -409,7 +409,9 @@ int sa3k_attention_sink_fwd(sa3k_ctx* ctx, const sa3k_sink_attn* p, const sa3k_t
 
 /* Backward for upstream dO, from the forward's o and lse: dq, and dk, dv (both or neither NULL; a
  * shared head's are summed over its query heads), in the inputs' type.  No atomics: results do not
- * depend on timing. */
+ * depend on timing.  The probabilities P and dS = P (dO v - rowsum(dO o)) are rounded to the inputs' type as
+ * operands: with F16 what lies below 2^-25 vanishes and what passes 65504 overflows, so dO wants the scale
+ * at which F16 gradients are kept (BF16 has f32's range). */
 int sa3k_attention_sink_bwd(sa3k_ctx* ctx, const sa3k_sink_attn* p, const sa3k_tensor4* q, const sa3k_tensor4* k,
                             const sa3k_tensor4* v, const sa3k_tensor4* o, const sa3k_tensor4* dO, const float* lse,
                             const sa3k_tensor4* dq, const sa3k_tensor4* dk, const sa3k_tensor4* dv, char* err,
@@ -426,7 +428,8 @@ int sa3k_attention_sink_bwd(sa3k_ctx* ctx, const sa3k_sink_attn* p, const sa3k_t
  * x, dx, bias and the adapter's arrays start on 16 bytes; S <= 2^20 - 16.
  * Products read IEEE half operands with f32 accumulation (SA3K_OPT notes above): x and W are
  * rounded to half, activation and residual are applied to the f32 value, and y is rounded once.
- * Replaces dit_lin followed by its activation and add (src/dit.h:244-254). */
+ * Counterpart of dit_lin followed by its activation and add (src/dit.h:244-254); the DiT step has
+ * passes of its own for these. */
 int sa3k_linear_act_fwd(sa3k_ctx* ctx, const sa3k_weight* w, const sa3k_adapter* ad, const float* bias, int act, int type,
                         const void* x, int64_t S, const void* residual, void* z, void* y, char* err, int err_len);
 
@@ -436,7 +439,7 @@ int sa3k_linear_act_fwd(sa3k_ctx* ctx, const sa3k_weight* w, const sa3k_adapter*
  * accumulate != 0 adds into dbias, dA, dB, dm; dx is overwritten.  The residual's gradient is dy.
  * dz is rounded to half as an operand of dx and the adapter gradients (dbias is summed before): what lies
  * below 2^-25 vanishes there and what passes 65504 overflows, for F32 activations too.  With an adapter
- * `out` is a multiple of 8. */
+ * `out` is a multiple of 8; dora's dm is formed from z as it was kept, rounded to `type`. */
 int sa3k_linear_act_bwd(sa3k_ctx* ctx, const sa3k_weight* w, const sa3k_adapter* ad, const float* bias, int act, int type,
                         const void* x, int64_t S, const void* z, const void* dy, void* dx, float* dbias, float* dA,
                         float* dB, float* dm, int accumulate, char* err, int err_len);

@@ -3,7 +3,7 @@
 // Replaces nn::sdpa (src/nn.h:135-144: mul_mat(k, q) -> soft_max_ext(scale) -> mul_mat(v^T, kq))
 // and its autodiff backward (SOFT_MAX_BACK + OUT_PROD), for the DiT's dense self-attention
 // (src/dit.h:199-221), its cross-attention to the conditioning (src/dit.h:225-240) and the
-// banded variant |q - k| <= window (the mask of src/same_ae.h:96-106, BASELINE config 3).
+// banded variant |q - k| <= window (the mask of src/same_ae.h:96-106).
 //
 // Flash-style tiling: nothing of size S x S touches HBM.  Forward keeps a running row max / sum
 // and writes O and the row log-sum-exp; the backward recomputes P from that LSE.  The backward

@@ -7,8 +7,8 @@
 // is read once for its group.  Work is split along the keys twice: the warps of a CTA take the 32-key
 // steps that the window and the sinks cover in turn, and the CTAs of a cluster (1 to 16) take turns
 // before that, so that a batch of one still reaches most SMs.  Every warp keeps its own running
-// maximum, sum and output (f32, registers) and three steps of K and V (8 KB each, cp.async) in
-// flight; warps are joined through shared memory and CTAs through their cluster's, in rank order, so
+// maximum, sum and output (f32, registers) and a ring of three steps of K and V (8 KB each, cp.async),
+// of which two are in flight while one is worked on; warps are joined through shared memory and CTAs through their cluster's, in rank order, so
 // there is no workspace and the result does not depend on timing.
 #include <algorithm>
 

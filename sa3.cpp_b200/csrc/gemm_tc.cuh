@@ -102,7 +102,8 @@ __device__ __forceinline__ float act_element(const Args& args, float v, long row
 // The residual's chunks (32 rows x 128 bytes, like the output's) of one epilogue warp: TMA brings a
 // chunk into the staging buffer that its output will leave from (direct loads, 16 bytes of 32 rows at
 // a time, thrashed the few KB of L1 that are left and cost 30 us on a 4352 x 6144 x 1536 product).
-// With two buffers a chunk is fetched while the one before it is worked on.
+// With two buffers the next chunk is requested when this one's output is on its way: its latency is
+// covered by the next accumulator columns' load within a tile, and by the wait for the accumulator across tiles.
 template <int BUFS>
 struct ResidualPipe {
   uint8_t* stg;

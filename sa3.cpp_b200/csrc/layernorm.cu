@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(1024) ln_bwd_kernel(const LnArgs a, int tpr) {
 // sends away the half that the lane does not keep) and one barrier, where row by row it was 40 and two.
 // Packed f32 pairs halve the instructions, which bounded the kernel (270 a warp and row, 2.4 a clock).
 // A thread takes about 85 registers without spills (they went to L2, the ring having taken L1: 44 us
-// for 16383 x 1536 with the fold instead of 35), so the blocks per SM follow from the threads of a row; rows of more
+// for 16383 x 1536 with the fold instead of 37), so the blocks per SM follow from the threads of a row; rows of more
 // than 5120 columns have 64 registers a thread and read the slot again instead of holding its values.
 constexpr int kLnMaxSlots = 8;
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {

@@ -2,7 +2,7 @@
 
 Tensor names and shapes are the ones dit_block / dit_head / dit_tail read (src/dit.h:164-323),
 shaped as PyTorch [out][in] (= ggml [in, out]); 1-D tensors are vectors.  Weights are drawn from
-N(0, std) (BASELINE: std 0.02), norms' gammas near 1, biases and adaLN offsets small.
+N(0, std) (the benchmark's std is 0.02), norms' gammas near 1, biases and adaLN offsets small.
 """
 import numpy as np
 
@@ -60,7 +60,7 @@ def synth_tensor(name, shape, rng, std):
 
 
 def default_targets(cfg):
-    """DoRA targets of BASELINE config 4: q/k/v (fused qkv), o and both MLP projections."""
+    """DoRA targets of the benchmark's step: q/k/v (fused qkv), o and both MLP projections."""
     names = []
     for l in range(cfg["depth"]):
         names += [f"dit.{l}.self.qkv.weight", f"dit.{l}.self.out.weight", f"dit.{l}.ff.proj.weight",
