@@ -427,7 +427,8 @@ int sa3k_attention_sink_bwd(sa3k_ctx* ctx, const sa3k_sink_attn* p, const sa3k_t
  * same), contiguous; residual and z may be NULL (z: the pre-activation, kept for the backward).
  * x, dx, bias and the adapter's arrays start on 16 bytes; S <= 2^20 - 16.
  * Products read IEEE half operands with f32 accumulation (SA3K_OPT notes above): x and W are
- * rounded to half, activation and residual are applied to the f32 value, and y is rounded once.
+ * rounded to half, activation and residual are applied to the f32 value, and y is rounded once (32 rows
+ * or fewer without an adapter read a quantized W's codes, which half holds exactly, and scale in f32).
  * Counterpart of dit_lin followed by its activation and add (src/dit.h:244-254); the DiT step has
  * passes of its own for these. */
 int sa3k_linear_act_fwd(sa3k_ctx* ctx, const sa3k_weight* w, const sa3k_adapter* ad, const float* bias, int act, int type,

@@ -287,7 +287,9 @@ def test_linear_act_adapter_widths(ctx, dora):
 
 # ------------------------------------------------------------------------------- scratch and captures
 def _used():
+    import gc
     import torch
+    gc.collect()          # (what earlier tests left is not freed between two looks)
     torch.cuda.synchronize()
     torch.cuda.empty_cache()
     free, total = torch.cuda.mem_get_info()
